@@ -75,6 +75,17 @@ SIGNATURES = {
     "hb_residual_rms": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                 c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_void_p,
                                 c_void_p, c_int64, c_int64, c_int]),
+    "hb_quant_rows": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int]),
+    "hb_rms_modulate_q8": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_int64,
+                                   c_int, c_void_p, c_int64, c_void_p, c_int64, c_int]),
+    "hb_residual_rms_q8": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                   c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                   c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int]),
+    "hb_glu_q8": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int]),
+    "hb_proj_q8": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                           c_int, c_int64, c_int64, c_int, c_int]),
+    "hb_proj_q4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
+                           c_void_p, c_int64, c_int, c_int, c_int]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,467 @@
+// Rows as 8-bit values with one scale each, for gfx950 (MI355X): the inputs of the 8-bit projections.
+//
+//   quant_rows       y = x
+//   rms_modulate_q8  y = x rsqrt(mean(x^2) + eps) w (1 + scale) + shift      (the DiT block norm, sa3jax/dit.py:44-57,
+//                    231-233, 246-247; without scale and shift dit.py:236)
+//   residual_rms_q8  h' = h + (x + bias) sigmoid(1 - gate) + local (dit.py:234, 237-241, 249-251), and y the norm of h'
+//   glu_q8           y = value silu(gate), [value | gate] = proj + bias      (dit.py:218-221)
+//
+// followed by s = max(max_c |y| / 448, 2^-100) and q = e4m3(y / s): 448 is the largest e4m3 value, so the row's largest
+// value meets it and no other saturates. The floor keeps 1 / s finite; a row of zeros gives zeros. A row that holds a
+// NaN gets the scale NaN and one whose largest magnitude is infinite the scale inf, with finite values 0 and infinite
+// ones NaN: every value the row stands for, q s, is then NaN.
+//
+// Everything between the inputs and the outputs is fp32, h' included: the norm reads the sum itself, not its value
+// rounded to the compute dtype, so that each output is rounded once.
+#include <cmath>
+
+#include "api.h"
+#include "common.h"
+
+namespace hb {
+namespace quant {
+
+// V consecutive elements of a row as fp32.
+template <typename T>
+struct Vec;
+template <>
+struct Vec<uint16_t> {  // bf16
+  static constexpr int N = 8;
+  __device__ static void load(const uint16_t* p, float (&x)[8]) { unpack8(ld16(p), x); }
+  __device__ static void store(uint16_t* p, const float (&x)[8]) { st16(p, pack8(x)); }
+};
+template <>
+struct Vec<_Float16> {
+  static constexpr int N = 8;
+  __device__ static void load(const _Float16* p, float (&x)[8]) { F16Io::unpack8(ld16(p), x); }
+  __device__ static void store(_Float16* p, const float (&x)[8]) {
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = F16Io::pack2(x[2 * i], x[2 * i + 1]);
+    st16(p, v);
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  __device__ static void load(const float* p, float (&x)[4]) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  }
+  __device__ static void store(float* p, const float (&x)[4]) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void load_f32(const float* p, float (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const f32x4 v = *reinterpret_cast<const f32x4_align4*>(p + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[i + j] = v[j];
+  }
+}
+
+// 1 / (1 + e^-u) with the hardware exponential and reciprocal, within a few fp32 units.
+__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * u)); }
+
+// Four fp32 values as e4m3, round to nearest even.
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true));
+}
+
+constexpr int kMaxWaves = 16;
+constexpr float kScaleFloor = 0x1p-100f;
+
+// Reductions over a row's workgroup: of each wave by lane exchange, then over the waves in their order through `buf`
+// (a slot per wave). Every lane gets the result. `buf` must be free of reads on entry.
+__device__ __forceinline__ float row_sum(float v, float* buf) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
+  const int waves = blockDim.x >> 6;
+  if (waves == 1) return v;
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int i = 0; i < waves; ++i) v += buf[i];
+  return v;
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* buf) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const uint32_t o = __shfl_xor(v, off, kWave);
+    v = v > o ? v : o;
+  }
+  const int waves = blockDim.x >> 6;
+  if (waves == 1) return v;
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int i = 0; i < waves; ++i) v = v > buf[i] ? v : buf[i];
+  return v;
+}
+
+// The row's scale and its values in 8 bits; y holds zeros past the row. Magnitudes are compared as their bits: a NaN's
+// are above every number's, so it reaches the scale.
+template <int V, int CH>
+__device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, float* s, int C, uint32_t* buf) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < CH; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t b = __float_as_uint(y[k][j]) & 0x7fffffffu;
+      m = m > b ? m : b;
+    }
+  const float amax = __uint_as_float(row_max(m, buf));
+  float sc = __fdiv_rn(amax, 448.f);
+  if (sc < kScaleFloor) sc = kScaleFloor;  // not for a NaN
+  const float inv = __fdiv_rn(1.f, sc);
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c0 = (k * blockDim.x + threadIdx.x) * V;
+    if (c0 < C) {
+      uint32_t w[V / 4];
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        w[i] = pack_e4m3x4(y[k][4 * i] * inv, y[k][4 * i + 1] * inv, y[k][4 * i + 2] * inv, y[k][4 * i + 3] * inv);
+      if constexpr (V == 8) *reinterpret_cast<u32x2*>(q + c0) = u32x2{w[0], w[1]};
+      else *reinterpret_cast<uint32_t*>(q + c0) = w[0];
+    }
+  }
+  if (threadIdx.x == 0) *s = sc;
+}
+
+enum Kind { kQuant = 0, kNorm = 1, kResidualNorm = 2, kGlu = 3 };
+
+template <typename T>
+struct Args {
+  const T* x;  // kGlu: the projection's output, values at column 0 and gates at column C
+  int64_t xs;
+  const T* h;  // kResidualNorm
+  int64_t hs;
+  const T* xbias;
+  const T* gate;
+  int64_t gate_stride;
+  const T* local;
+  int memory;
+  const float* fbias;  // kGlu: 2 C values
+  const float* w;      // norms
+  float eps;
+  const T* scale;
+  const T* shift;
+  int64_t mod_stride;
+  int L;  // rows per batch
+  T* out_h;
+  int64_t os;
+  uint8_t* q;
+  int64_t qs;
+  float* s;
+  int64_t N;
+  int C;
+};
+
+// A row per workgroup, held in registers: CH chunks of V values per lane, chunk k of lane t at column
+// (k * lanes + t) * V.
+template <typename T, int KIND, int CH>
+__global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float sum_buf[kMaxWaves];
+  __shared__ uint32_t max_buf[kMaxWaves];
+  const int C = a.C;
+  const int64_t n = blockIdx.x;
+  const int64_t b = n / a.L;
+  const bool add_local = KIND == kResidualNorm && a.local && n - b * a.L >= a.memory;
+  float y[CH][V];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const int c0 = (k * blockDim.x + threadIdx.x) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) y[k][j] = 0.f;
+    if (c0 < C) {
+      Vec<T>::load(a.x + n * a.xs + c0, y[k]);
+      if constexpr (KIND == kGlu) {
+        float g[V], t[V];
+        Vec<T>::load(a.x + n * a.xs + C + c0, g);
+        if (a.fbias) {
+          load_f32(a.fbias + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[k][j] += t[j];
+          load_f32(a.fbias + C + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] += t[j];
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[k][j] = y[k][j] * (g[j] * sigmoid(g[j]));
+      }
+      if constexpr (KIND == kResidualNorm) {
+        float t[V];
+        if (a.xbias) {
+          Vec<T>::load(a.xbias + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[k][j] += t[j];
+        }
+        if (a.gate) {
+          Vec<T>::load(a.gate + b * a.gate_stride + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[k][j] *= sigmoid(1.f - t[j]);
+        }
+        Vec<T>::load(a.h + n * a.hs + c0, t);
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[k][j] = t[j] + y[k][j];
+        if (add_local) {
+          Vec<T>::load(a.local + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[k][j] += t[j];
+        }
+        Vec<T>::store(a.out_h + n * a.os + c0, y[k]);
+      }
+    }
+  }
+  if constexpr (KIND == kNorm || KIND == kResidualNorm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) ss = __fmaf_rn(y[k][j], y[k][j], ss);
+    const float inv = rsqrtf(row_sum(ss, sum_buf) / static_cast<float>(C) + a.eps);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int c0 = (k * blockDim.x + threadIdx.x) * V;
+      if (c0 < C) {
+        float w[V];
+        load_f32(a.w + c0, w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[k][j] = (y[k][j] * inv) * w[j];
+        if (a.scale) {
+          float s[V], t[V];
+          Vec<T>::load(a.scale + b * a.mod_stride + c0, s);
+          Vec<T>::load(a.shift + b * a.mod_stride + c0, t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[k][j] = y[k][j] * (1.f + s[j]) + t[j];
+        }
+      }
+    }
+  }
+  store_q8<V, CH>(y, a.q + n * a.qs, a.s + n, C, max_buf);
+}
+
+// The longest row: 16 waves of 64 lanes of CH chunks.
+constexpr int kMaxC = 16384;
+
+template <typename T, int KIND>
+void launch(hipStream_t stream, const Args<T>& a) {
+  const int chunks = a.C / Vec<T>::N;
+  auto lanes = [&](int ch) { return dim3(static_cast<unsigned>(((chunks + ch - 1) / ch + 63) / 64 * 64)); };
+  const dim3 grid(static_cast<unsigned>(a.N));
+  if (chunks <= 1024) hipLaunchKernelGGL((row_kernel<T, KIND, 1>), grid, lanes(1), 0, stream, a);
+  else if (chunks <= 2048) hipLaunchKernelGGL((row_kernel<T, KIND, 2>), grid, lanes(2), 0, stream, a);
+  else hipLaunchKernelGGL((row_kernel<T, KIND, 4>), grid, lanes(4), 0, stream, a);
+}
+
+}  // namespace quant
+}  // namespace hb
+
+using namespace hb;
+
+namespace {
+
+// The operands of a call as its checks see them, in elements but for `esize`.
+struct Operand {
+  const char* name;
+  const void* p;
+  int esize;
+  int64_t rows, stride, cols;
+};
+
+int esize_of(int dtype) { return dtype == HB_F32 ? 4 : 2; }
+int vec_of(int dtype) { return dtype == HB_F32 ? 4 : 8; }
+
+int check_rows(const char* what, int dtype, int64_t N, int C, int L) {
+  if (dtype != HB_BF16 && dtype != HB_F32 && dtype != HB_F16)
+    return fail(HB_ERR_DTYPE, "%s: dtype %d is not HB_BF16 (0), HB_F32 (1) or HB_F16 (2)", what, dtype);
+  if (N < 1 || N >= (int64_t(1) << 31) || L < 1)
+    return fail(HB_ERR_SHAPE, "%s needs 1 <= N < 2^31 and rows_per_batch >= 1", what);
+  if (C < 1 || C > quant::kMaxC || C % vec_of(dtype))
+    return fail(HB_ERR_SHAPE, "%s needs rows of 1 to %d values, a multiple of %d (got %d)", what, quant::kMaxC,
+                vec_of(dtype), C);
+  return HB_OK;
+}
+
+// Pointer, alignment, stride and extent of every operand (NULL ones were accepted by the caller), then that no output
+// shares an element with an input or another output.
+int check_operands(const char* what, const Operand* outs, int n_out, const Operand* ins, int n_in, int64_t vec) {
+  int st;
+  for (int i = 0; i < n_out + n_in; ++i) {
+    const Operand& o = i < n_out ? outs[i] : ins[i - n_out];
+    if (!o.p) continue;
+    const int align = o.cols > 1 ? 16 : 4;  // rows; a scale per row
+    if (reinterpret_cast<uintptr_t>(o.p) % align)
+      return fail(HB_ERR_STRIDE, "%s: %s must be %d-byte aligned", what, o.name, align);
+    if (o.cols > 1 && (o.stride < o.cols || o.stride % vec))
+      return fail(HB_ERR_STRIDE, "%s: %s stride %lld must be >= %lld and a multiple of %lld", what, o.name,
+                  static_cast<long long>(o.stride), static_cast<long long>(o.cols), static_cast<long long>(vec));
+    if ((st = check_extent(what, o.name, o.rows, o.stride, o.cols))) return st;
+  }
+  for (int i = 0; i < n_out; ++i) {
+    const Operand& o = outs[i];
+    const int64_t ob = rows_bytes(o.rows, o.stride, o.cols, o.esize);
+    for (int j = 0; j < n_in + i; ++j) {
+      const Operand& r = j < n_in ? ins[j] : outs[j - n_in];
+      if (!r.p) continue;
+      if (r.rows == o.rows && r.esize == o.esize) {
+        if ((st = check_no_overlap(what, o.name, o.p, o.stride, o.cols, r.name, r.p, r.stride, r.cols, o.rows, o.esize,
+                                   false)))
+          return st;
+      } else if ((st = check_disjoint(what, o.name, o.p, ob, r.name, r.p,
+                                      rows_bytes(r.rows, r.stride, r.cols, r.esize)))) {
+        return st;
+      }
+    }
+  }
+  return HB_OK;
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(HB_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return HB_OK;
+}
+
+template <int KIND, typename T, typename F>
+int launch_as(hipStream_t stream, const F& fill) {
+  quant::Args<T> a = {};
+  fill(a);
+  quant::launch<T, KIND>(stream, a);
+  return 0;
+}
+
+// Runs row_kernel<KIND> for `dtype`; `fill` sets the arguments of any element type.
+template <int KIND, typename F>
+int launch_kind(const char* what, hipStream_t stream, int dtype, const F& fill) {
+  if (dtype == HB_BF16) launch_as<KIND, uint16_t>(stream, fill);
+  else if (dtype == HB_F16) launch_as<KIND, _Float16>(stream, fill);
+  else launch_as<KIND, float>(stream, fill);
+  return launched(what);
+}
+
+// `p` as the pointer type of `field`.
+template <typename T>
+void set(const T*& field, const void* p) { field = static_cast<const T*>(p); }
+template <typename T>
+void set(T*& field, void* p) { field = static_cast<T*>(p); }
+
+}  // namespace
+
+extern "C" {
+
+int hb_quant_rows(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, void* q, int64_t q_row_stride,
+                  float* q_scale, int64_t N, int C) {
+  clear_error();
+  const char* what = "quant_rows";
+  int st = check_rows(what, dtype, N, C, 1);
+  if (st) return st;
+  if (!x || !q || !q_scale) return fail(HB_ERR_NULL, "%s: x, q and q_scale must be non-NULL", what);
+  const Operand outs[] = {{"q", q, 1, N, q_row_stride, C}, {"q_scale", q_scale, 4, N, 1, 1}};
+  const Operand ins[] = {{"x", x, esize_of(dtype), N, x_row_stride, C}};
+  if ((st = check_operands(what, outs, 2, ins, 1, vec_of(dtype)))) return st;
+  return launch_kind<quant::kQuant>(what, stream, dtype, [&](auto& a) {
+    set(a.x, x), a.xs = x_row_stride, a.L = 1;
+    set(a.q, q), a.qs = q_row_stride, a.s = q_scale, a.N = N, a.C = C;
+  });
+}
+
+int hb_rms_modulate_q8(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, const float* weight,
+                       float eps, const void* scale, const void* shift, int64_t mod_batch_stride, int rows_per_batch,
+                       void* q, int64_t q_row_stride, float* q_scale, int64_t N, int C) {
+  clear_error();
+  const char* what = "rms_modulate_q8";
+  int st = check_rows(what, dtype, N, C, rows_per_batch);
+  if (st) return st;
+  if (!x || !weight || !q || !q_scale)
+    return fail(HB_ERR_NULL, "%s: x, weight, q and q_scale must be non-NULL", what);
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(HB_ERR_EPS, "%s: eps %g must be finite and >= 0", what, eps);
+  if (!scale != !shift) return fail(HB_ERR_NULL, "%s: scale and shift are given together or not at all", what);
+  if (scale && N % rows_per_batch) return fail(HB_ERR_SHAPE, "%s: N must be a multiple of rows_per_batch", what);
+  const int64_t nb = scale ? N / rows_per_batch : 1, ms = nb > 1 ? mod_batch_stride : C;
+  const int es = esize_of(dtype);
+  const Operand outs[] = {{"q", q, 1, N, q_row_stride, C}, {"q_scale", q_scale, 4, N, 1, 1}};
+  const Operand ins[] = {{"x", x, es, N, x_row_stride, C},
+                         {"scale", scale, es, nb, ms, C},
+                         {"shift", shift, es, nb, ms, C}};
+  if ((st = check_operands(what, outs, 2, ins, 3, vec_of(dtype)))) return st;
+  for (const Operand& o : outs)
+    if ((st = check_disjoint(what, o.name, o.p, rows_bytes(o.rows, o.stride, o.cols, o.esize), "weight", weight,
+                             static_cast<int64_t>(C) * 4)))
+      return st;
+  return launch_kind<quant::kNorm>(what, stream, dtype, [&](auto& a) {
+    set(a.x, x), a.xs = x_row_stride, a.w = weight, a.eps = eps;
+    set(a.scale, scale), set(a.shift, shift), a.mod_stride = ms, a.L = rows_per_batch;
+    set(a.q, q), a.qs = q_row_stride, a.s = q_scale, a.N = N, a.C = C;
+  });
+}
+
+int hb_residual_rms_q8(hipStream_t stream, const void* h, int dtype, int64_t h_row_stride, const void* x,
+                       int64_t x_row_stride, const void* x_bias, const void* gate, int64_t gate_batch_stride,
+                       const void* local, int memory, const float* weight, float eps, const void* scale,
+                       const void* shift, int64_t mod_batch_stride, int rows_per_batch, void* out_h,
+                       int64_t out_h_row_stride, void* q, int64_t q_row_stride, float* q_scale, int64_t N, int C) {
+  clear_error();
+  const char* what = "residual_rms_q8";
+  int st = check_rows(what, dtype, N, C, rows_per_batch);
+  if (st) return st;
+  if (!h || !x || !weight || !out_h || !q || !q_scale)
+    return fail(HB_ERR_NULL, "%s: h, x, weight, out_h, q and q_scale must be non-NULL", what);
+  if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(HB_ERR_EPS, "%s: eps %g must be finite and >= 0", what, eps);
+  if (!scale != !shift) return fail(HB_ERR_NULL, "%s: scale and shift are given together or not at all", what);
+  if (memory < 0) return fail(HB_ERR_SHAPE, "%s: memory must be >= 0", what);
+  if ((gate || scale) && N % rows_per_batch)
+    return fail(HB_ERR_SHAPE, "%s: N must be a multiple of rows_per_batch", what);
+  const int64_t nb = gate || scale ? N / rows_per_batch : 1;
+  const int64_t gs = nb > 1 ? gate_batch_stride : C, ms = nb > 1 ? mod_batch_stride : C;
+  const int es = esize_of(dtype);
+  const Operand outs[] = {{"out_h", out_h, es, N, out_h_row_stride, C},
+                          {"q", q, 1, N, q_row_stride, C},
+                          {"q_scale", q_scale, 4, N, 1, 1}};
+  const Operand ins[] = {{"h", h, es, N, h_row_stride, C},   {"x", x, es, N, x_row_stride, C},
+                         {"x_bias", x_bias, es, 1, C, C},    {"local", local, es, 1, C, C},
+                         {"gate", gate, es, nb, gs, C},      {"scale", scale, es, nb, ms, C},
+                         {"shift", shift, es, nb, ms, C}};
+  if ((st = check_operands(what, outs, 3, ins, 7, vec_of(dtype)))) return st;
+  for (const Operand& o : outs)
+    if ((st = check_disjoint(what, o.name, o.p, rows_bytes(o.rows, o.stride, o.cols, o.esize), "weight", weight,
+                             static_cast<int64_t>(C) * 4)))
+      return st;
+  return launch_kind<quant::kResidualNorm>(what, stream, dtype, [&](auto& a) {
+    set(a.h, h), a.hs = h_row_stride, set(a.x, x), a.xs = x_row_stride, set(a.xbias, x_bias);
+    set(a.gate, gate), a.gate_stride = gs, set(a.local, local), a.memory = memory;
+    a.w = weight, a.eps = eps, set(a.scale, scale), set(a.shift, shift), a.mod_stride = ms, a.L = rows_per_batch;
+    set(a.out_h, out_h), a.os = out_h_row_stride;
+    set(a.q, q), a.qs = q_row_stride, a.s = q_scale, a.N = N, a.C = C;
+  });
+}
+
+int hb_glu_q8(hipStream_t stream, const void* proj, int dtype, int64_t proj_row_stride, const float* bias, void* q,
+              int64_t q_row_stride, float* q_scale, int64_t N, int F) {
+  clear_error();
+  const char* what = "glu_q8";
+  int st = check_rows(what, dtype, N, F, 1);
+  if (st) return st;
+  if (!proj || !q || !q_scale) return fail(HB_ERR_NULL, "%s: proj, q and q_scale must be non-NULL", what);
+  const Operand outs[] = {{"q", q, 1, N, q_row_stride, F}, {"q_scale", q_scale, 4, N, 1, 1}};
+  const Operand ins[] = {{"proj", proj, esize_of(dtype), N, proj_row_stride, 2 * static_cast<int64_t>(F)}};
+  if ((st = check_operands(what, outs, 2, ins, 1, vec_of(dtype)))) return st;
+  for (const Operand& o : outs)
+    if ((st = check_disjoint(what, o.name, o.p, rows_bytes(o.rows, o.stride, o.cols, o.esize), "bias", bias,
+                             static_cast<int64_t>(F) * 8)))
+      return st;
+  return launch_kind<quant::kGlu>(what, stream, dtype, [&](auto& a) {
+    set(a.x, proj), a.xs = proj_row_stride, a.fbias = bias, a.L = 1;
+    set(a.q, q), a.qs = q_row_stride, a.s = q_scale, a.N = N, a.C = F;
+  });
+}
+
+}  // extern "C"

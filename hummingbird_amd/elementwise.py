@@ -2,8 +2,9 @@
 `hb_gated_residual`) on MI355X: the `attention="hip"` counterparts of `same_l._dyt` followed by the block's cast to
 the compute dtype (sa3jax/same_l.py:58-69, 191-192), of the GLU gate of `same_l._feed_forward`
 (sa3jax/same_l.py:172-183; the DiT's SwiGLU, sa3jax/dit.py:218-221, is the same gate), and of the DiT block's
-norms, adaLN modulations and residuals (sa3jax/dit.py:224-251). Tensors are torch tensors on a ROCm device; work
-is enqueued on torch's current stream.
+norms, adaLN modulations and residuals (sa3jax/dit.py:224-251). The `_q8` forms of the latter (`quantize_rows`,
+`rms_modulate_q8`, `residual_rms_q8`, `glu_q8`) end in 8-bit rows, the inputs of `projection.linear_q8`. Tensors are
+torch tensors on a ROCm device; work is enqueued on torch's current stream.
 """
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ import torch
 from hummingbird_amd import _lib
 from hummingbird_amd._derived import f32_vector
 from hummingbird_amd.band_attention import pack_dyt
-from hummingbird_amd.dense_attention import _require_gpu, dtype_code
+from hummingbird_amd.dense_attention import _f32_vector, _require_gpu, dtype_code
 
 
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int]:
@@ -212,3 +213,129 @@ def residual_rms(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: fl
 def residual_rms_supported(dtype: torch.dtype, channels: int) -> bool:
     """Whether `residual_rms` takes rows of `channels` values of `dtype` (held in registers)."""
     return channels <= 2048 and channels % (8 if dtype in (torch.bfloat16, torch.float16) else 4) == 0
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# 8-bit rows: e4m3 values `q` with one fp32 scale `s` per row, standing for q * s.
+
+Q8_DTYPE = torch.float8_e4m3fn
+Q8_MAX_WIDTH = 16384  # values of a row, held in registers
+
+
+def _same_device(dev: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+
+
+def _vector(t: torch.Tensor | None, channels: int, dtype: torch.dtype, name: str) -> int:
+    """The pointer of a `(C,)` vector of `dtype`, 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype != dtype or t.numel() != channels or t.stride(-1) != 1:
+        raise ValueError(f"{name} must be ({channels},) of {dtype} with unit stride")
+    return t.data_ptr()
+
+
+def _q8_out(shape: tuple, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty(shape, dtype=Q8_DTYPE, device=device),
+            torch.empty(shape[:-1], dtype=torch.float32, device=device))
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`x` `(..., C)` as 8-bit rows: `(q, s)`, q `(..., C)` e4m3 and s `(...)` fp32 with `s = max(max|x| / 448, 2^-100)`
+    and `q = e4m3(x / s)`, in one pass (`hb_quant_rows`). A row with a NaN or an infinity stands for NaNs. C a multiple
+    of 8 (fp32: 4), at most `Q8_MAX_WIDTH`."""
+    _require_gpu(x, "x")
+    rows, stride = _rows(x, "x")
+    q, s = _q8_out(x.shape, x.device)
+    channels = x.shape[-1]
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().hb_quant_rows(_lib.current_stream(x.device), x.data_ptr(), dtype_code(x.dtype), stride,
+                                             q.data_ptr(), channels, s.data_ptr(), rows, channels), "quantize_rows")
+    return q, s
+
+
+def rms_modulate_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: torch.Tensor | None = None,
+                    shift: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`rms_modulate(x, weight, eps, scale, shift)` on `(B, L, C)` in fp32 throughout, as 8-bit rows `(q, s)` (see
+    `quantize_rows`), in one pass (`hb_rms_modulate_q8`)."""
+    _require_gpu(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B, L, C), got {tuple(x.shape)}")
+    _same_device(x.device, weight=weight, scale=scale, shift=shift)
+    batch, length, channels = x.shape
+    rows, stride = _rows(x, "x")
+    w = _f32_vector(weight, x.device)
+    if w.numel() != channels:
+        raise ValueError(f"weight must have {channels} elements")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift are given together or not at all")
+    sp, ms = _per_batch(scale, batch, channels, x.dtype, "scale")
+    hp, ms2 = _per_batch(shift, batch, channels, x.dtype, "shift")
+    if ms != ms2:
+        raise ValueError("scale and shift must share their batch stride")
+    q, s = _q8_out(x.shape, x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().hb_rms_modulate_q8(_lib.current_stream(x.device), x.data_ptr(), dtype_code(x.dtype),
+                                                  stride, w.data_ptr(), float(eps), sp, hp, ms, length, q.data_ptr(),
+                                                  channels, s.data_ptr(), rows, channels), "rms_modulate_q8")
+    return q, s
+
+
+def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
+                    gate: torch.Tensor | None = None, x_bias: torch.Tensor | None = None,
+                    local: torch.Tensor | None = None, memory: int = 0, scale: torch.Tensor | None = None,
+                    shift: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`residual_rms(h, x, weight, eps, gate, x_bias, local, memory, scale, shift)` with the norm as 8-bit rows, in one
+    pass (`hb_residual_rms_q8`): `(h', q, s)`, h' in `h.dtype`, `(q, s)` as `quantize_rows` gives them. Both are
+    rounded once, from fp32: the norm reads h' before its rounding."""
+    _require_gpu(h, "h")
+    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype:
+        raise ValueError(f"h and x must be (B, L, C) of one shape and dtype, got {tuple(h.shape)}, {tuple(x.shape)}")
+    _same_device(h.device, x=x, weight=weight, gate=gate, x_bias=x_bias, local=local, scale=scale, shift=shift)
+    batch, length, channels = h.shape
+    _, hs = _rows(h, "h")
+    rows, xs = _rows(x, "x")
+    gp, gs = _per_batch(gate, batch, channels, h.dtype, "gate")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift are given together or not at all")
+    sp, ms = _per_batch(scale, batch, channels, h.dtype, "scale")
+    hp, ms2 = _per_batch(shift, batch, channels, h.dtype, "shift")
+    if ms != ms2:
+        raise ValueError("scale and shift must share their batch stride")
+    w = _f32_vector(weight, h.device)
+    if w.numel() != channels:
+        raise ValueError(f"weight must have {channels} elements")
+    out_h = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    q, s = _q8_out(h.shape, h.device)
+    with torch.cuda.device(h.device):
+        _lib.check(_lib.load().hb_residual_rms_q8(
+            _lib.current_stream(h.device), h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
+            _vector(x_bias, channels, h.dtype, "x_bias"), gp, gs, _vector(local, channels, h.dtype, "local"),
+            int(memory), w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
+            channels, s.data_ptr(), rows, channels), "residual_rms_q8")
+    return out_h, q, s
+
+
+def glu_q8(proj: torch.Tensor, bias: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`value * silu(gate)` for `[value | gate]` = the two halves of the last axis of `proj (+ bias)`, in fp32, as
+    8-bit rows `(q, s)` (see `quantize_rows`), in one pass (`hb_glu_q8`): the DiT's SwiGLU (sa3jax/dit.py:218-221).
+    `bias` `(2F,)` is the glu_proj layer's where `proj` is the bare product."""
+    _require_gpu(proj, "proj")
+    _same_device(proj.device, bias=bias)
+    width = proj.shape[-1]
+    if width % 2:
+        raise ValueError(f"the glu_proj output width {width} is not even")
+    inner = width // 2
+    rows, stride = _rows(proj, "proj")
+    if bias is not None:
+        bias = _f32_vector(bias, proj.device)
+        if bias.numel() != width:
+            raise ValueError(f"bias must have {width} elements")
+    q, s = _q8_out((*proj.shape[:-1], inner), proj.device)
+    with torch.cuda.device(proj.device):
+        _lib.check(_lib.load().hb_glu_q8(_lib.current_stream(proj.device), proj.data_ptr(), dtype_code(proj.dtype),
+                                         stride, bias.data_ptr() if bias is not None else 0, q.data_ptr(), inner,
+                                         s.data_ptr(), rows, inner), "glu_q8")
+    return q, s

@@ -7,6 +7,9 @@ and the next DyT in theirs (reference: sa3jax/same_l.py:161, 181-184, 191-192).
 queries as rows `[q | q_diff]` and the prepared keys and values (RMSNorm, RoPE, value mask) into the attention
 workspace. `attend_projected` runs the attention against them (`hb_dense_attend_qq`), and `linear` is `x @ W^T`
 (`hb_proj`). Together they compute what `h @ W_qkv^T -> dense_attention -> @ W_o^T` computes, in the same cast points.
+
+`linear_q8` multiplies 8-bit rows (`elementwise.quantize_rows` and its kin) with 8-bit weights (`hb_proj_q8`), and
+`linear_q4` a few rows with 4-bit weights (`quantize_q4`, `hb_proj_q4`).
 """
 from __future__ import annotations
 
@@ -206,3 +209,105 @@ def same_l_supported(dtype: torch.dtype, dim: int, ff_inner: int, qkv_width: int
     multiple of 256."""
     return (dtype in FUSED_DTYPES and dim % 256 == 0 and ff_inner % 256 == 0 and qkv_width % 256 == 0 and dim > 0
             and ff_inner > 0)
+
+
+def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+              bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """`(x * x_scale) @ (weight * weight_scale)^T (+ bias)` of 8-bit rows on the matrix cores (`hb_proj_q8`): `x`
+    `(..., K)` e4m3 with `x_scale` `(...)` fp32, `weight` `(F, K)` e4m3 with `weight_scale` `(F,)` fp32 (both as
+    `elementwise.quantize_rows` gives them), `bias` `(F,)`; the sum, the scales and the bias in fp32, one rounding to
+    `dtype` (bf16, half or fp32). K a multiple of 16; any number of rows and features."""
+    _require_gpu(x, "x")
+    dev = x.device
+    if x.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"linear_q8 takes float8_e4m3fn rows and weights, got {x.dtype} and {weight.dtype}")
+    if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"the scales must be float32, got {x_scale.dtype} and {weight_scale.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[-1]:
+        raise ValueError(f"x must be (..., K) and weight (F, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    f, k = weight.shape
+    for name, t in (("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    if x_scale.shape != x.shape[:-1] or not x_scale.is_contiguous():
+        raise ValueError(f"x_scale must be contiguous {tuple(x.shape[:-1])}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != (f,) or not weight_scale.is_contiguous():
+        raise ValueError(f"weight_scale must be contiguous ({f},), got {tuple(weight_scale.shape)}")
+    n, xs = _rows(x, "x")
+    _, ws = _rows(weight, "weight")
+    if bias is not None:
+        bias = _f32_vector(bias, dev)
+        if bias.numel() != f:
+            raise ValueError(f"bias must have {f} elements")
+    out = torch.empty((*x.shape[:-1], f), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().hb_proj_q8(_lib.current_stream(dev), x.data_ptr(), xs, x_scale.data_ptr(),
+                                          weight.data_ptr(), ws, weight_scale.data_ptr(),
+                                          bias.data_ptr() if bias is not None else 0, out.data_ptr(),
+                                          dtype_code(dtype), f, n, k, f), "linear_q8")
+    return out
+
+
+Q4_GROUP = 32  # columns that share a scale
+_E2M1_MIDDLES = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)  # between the magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6
+
+
+def quantize_q4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`(F, K)` weights as `(codes (F, K / 2) uint8, scales (F, K / 32) uint8)` for `linear_q4`: e2m1 codes, two per
+    byte (the low nibble the even column), and per group of 32 columns the e8m0 scale 2^(s - 127), the least power of
+    two that brings the group's largest magnitude to 6 or below, s kept within [8, 250]. Magnitudes round to the nearest,
+    ties to the even code. Done once per weight, in torch operations on the weight's device. K a multiple of 32; the
+    weights must be finite."""
+    if weight.dim() != 2 or weight.shape[1] % Q4_GROUP or weight.numel() == 0:
+        raise ValueError(f"weight must be (F, K) with K a multiple of {Q4_GROUP}, got {tuple(weight.shape)}")
+    f, k = weight.shape
+    w = weight.to(torch.float32).reshape(f, k // Q4_GROUP, Q4_GROUP)
+    amax = w.abs().amax(dim=-1)
+    if not bool(torch.isfinite(amax).all()):
+        raise ValueError("quantize_q4 needs finite weights")
+    mant, exp = torch.frexp(amax)  # amax = mant 2^exp, mant in [0.5, 1): above 6 2^(exp - 3) when mant > 0.75
+    e = torch.where(mant > 0.75, exp - 2, exp - 3)
+    e = torch.where(amax > 0, e, torch.zeros_like(e)).clamp(8 - 127, 250 - 127)
+    v = w * torch.exp2(-e[..., None].to(torch.float32))
+    mag = v.abs()
+    middles = torch.tensor(_E2M1_MIDDLES, device=weight.device)
+    below, upto = torch.bucketize(mag, middles), torch.bucketize(mag, middles, right=True)
+    code = torch.where(below % 2 == 0, below, upto)  # on a middle the two differ: the even one
+    code = (code + 8 * torch.signbit(v)).reshape(f, k)
+    return (code[:, 0::2] + 16 * code[:, 1::2]).to(torch.uint8).contiguous(), (e + 127).to(torch.uint8).contiguous()
+
+
+def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
+              silu: bool = False) -> torch.Tensor:
+    """`act(x @ W^T (+ bias))` for few rows `x` `(..., K)` and 4-bit weights (`hb_proj_q4`): `weight` `(F, K / 2)` and
+    `weight_scale` `(F, K / 32)`, both uint8, as `quantize_q4` gives them; `bias` `(F,)`; act = SiLU with `silu`. x
+    keeps all of its bits (bf16, half or fp32), the sum, bias and activation are fp32, rounded once to `x.dtype`. It
+    reads the weights once per 64 rows of bf16 (half: 32, fp32: 20), and serves the layers that see one row per batch
+    entry."""
+    _require_gpu(x, "x")
+    dev = x.device
+    code = dtype_code(x.dtype)
+    if weight.dtype != torch.uint8 or weight_scale.dtype != torch.uint8:
+        raise TypeError(f"linear_q4 takes uint8 codes and scales, got {weight.dtype} and {weight_scale.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != 2 * weight.shape[1]:
+        raise ValueError(f"x must be (..., K) and weight (F, K / 2), got {tuple(x.shape)} and {tuple(weight.shape)}")
+    k, f = x.shape[-1], weight.shape[0]
+    if k % Q4_GROUP or weight_scale.shape != (f, k // Q4_GROUP):
+        raise ValueError(f"K must be a multiple of {Q4_GROUP} and weight_scale (F, K / {Q4_GROUP}), got K = {k} and "
+                         f"{tuple(weight_scale.shape)}")
+    for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    n, xs = _rows(x, "x")
+    _, ws = _rows(weight, "weight")
+    _, ss = _rows(weight_scale, "weight_scale")
+    if bias is not None:
+        bias = _f32_vector(bias, dev)
+        if bias.numel() != f:
+            raise ValueError(f"bias must have {f} elements")
+    out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().hb_proj_q4(_lib.current_stream(dev), x.data_ptr(), code, xs, weight.data_ptr(), ws,
+                                          weight_scale.data_ptr(), ss, bias.data_ptr() if bias is not None else 0,
+                                          int(bool(silu)), out.data_ptr(), f, n, k, f), "linear_q4")
+    return out

@@ -17,6 +17,9 @@
  *   hb_rms_modulate,   replace   the elementwise steps of dit._block around its GEMMs and attention calls
  *   hb_gated_residual,           (sa3jax/dit.py:224-251), an XLA chain in the reference;
  *   hb_residual_rms
+ *   hb_quant_rows, hb_rms_modulate_q8, hb_residual_rms_q8, hb_glu_q8, hb_proj_q8, hb_proj_q4
+ *                      the denoiser's norms, GLU and projections on 8-bit rows and 8- or 4-bit weights (no
+ *                      counterpart in the reference, which keeps 16-bit weights);
  *   hb_rope_tables     replaces  band_attention.rope_tables / dit._rope_tables
  *                      (sa3jax/band_attention.py:43-58, sa3jax/dit.py:82-87) in a kernel-native layout.
  *
@@ -300,6 +303,50 @@ int hb_residual_rms(hipStream_t stream, const void* h, int dtype, int64_t h_row_
                     const void* local, int memory, const float* weight, float eps, const void* scale,
                     const void* shift, int64_t mod_batch_stride, int rows_per_batch, void* out_h, void* out_y,
                     int64_t out_row_stride, int64_t N, int C);
+
+/* ---- The denoiser on 8-bit rows and 8- or 4-bit weights ----------------------------------------------------
+ * An 8-bit row is C e4m3 values q (OCP: sign, 4 exponent bits, 3 mantissa bits, no infinities, largest 448) and one
+ * fp32 scale s; it stands for q * s. The four row entry points compute y in fp32 from inputs of `dtype` and write
+ * s = max(max |y| / 448, 2^-100) and q = e4m3(y / s), round to nearest even. A row with a NaN has the scale NaN, one
+ * whose largest magnitude is infinite the scale inf: all its values q * s are then NaN.
+ *   hb_quant_rows      : y = x.
+ *   hb_rms_modulate_q8 : y = x * rsqrt(mean(x^2) + eps) * weight, with `scale` and `shift` (both or neither) then
+ *                        y * (1 + scale) + shift: hb_rms_modulate without its roundings to the compute dtype.
+ *   hb_residual_rms_q8 : v = h + (x + x_bias) * sigmoid(1 - gate) (+ local from token `memory` on), each operand
+ *                        optional as for hb_gated_residual; out_h = cast(v), y = the norm above of v. Neither v nor
+ *                        any step is rounded before its output.
+ *   hb_glu_q8          : y = value * silu(gate), [value | gate] = proj + bias (2F floats, or NULL).
+ *   Operands as for hb_rms_modulate, hb_gated_residual and hb_glu; q: rows of C (F) bytes, 16-byte aligned with a row
+ *   stride that is a multiple of 8 (bf16, half) or 4 (fp32); q_scale: N floats. C, F <= 16384. No output shares an
+ *   element with an input or another output.
+ *
+ * hb_proj_q8 : out[m, f] = (sum_k x[m, k] w[f, k]) x_scale[m] w_scale[f] + bias[f], x (M, K) and w (F, K) e4m3 rows
+ *   (strides in bytes, multiples of 16, 16-byte aligned) with a scale per row, the sum and the epilogue in fp32, one
+ *   rounding to out_dtype; bias: F floats or NULL. K a multiple of 16, any M and F up to 2^21; out row stride >= F.
+ * hb_proj_q4 : out[n, f] = act(sum_k x[n, k] e2m1(w[f, k]) 2^(w_scale[f, k / 32] - 127) + bias[f]) for few rows x
+ *   (N, K) of `dtype`: w holds two 4-bit codes per byte (OCP e2m1: sign, 2 exponent bits, 1 mantissa bit; the low
+ *   nibble the even column), w_scale one e8m0 byte per 32 columns, in [8, 250] (others give scales that the products
+ *   do not hold). x keeps all of its bits; sums in fp32; act = SiLU when `silu` != 0, else none; out of `dtype`.
+ *   K a multiple of 32, any N up to 2^16 and F; w row stride (bytes) a multiple of 16, w and x 16-byte aligned, x row
+ *   stride a multiple of 8 (bf16, half) or 4 (fp32). */
+int hb_quant_rows(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, void* q, int64_t q_row_stride,
+                  float* q_scale, int64_t N, int C);
+int hb_rms_modulate_q8(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, const float* weight,
+                       float eps, const void* scale, const void* shift, int64_t mod_batch_stride, int rows_per_batch,
+                       void* q, int64_t q_row_stride, float* q_scale, int64_t N, int C);
+int hb_residual_rms_q8(hipStream_t stream, const void* h, int dtype, int64_t h_row_stride, const void* x,
+                       int64_t x_row_stride, const void* x_bias, const void* gate, int64_t gate_batch_stride,
+                       const void* local, int memory, const float* weight, float eps, const void* scale,
+                       const void* shift, int64_t mod_batch_stride, int rows_per_batch, void* out_h,
+                       int64_t out_h_row_stride, void* q, int64_t q_row_stride, float* q_scale, int64_t N, int C);
+int hb_glu_q8(hipStream_t stream, const void* proj, int dtype, int64_t proj_row_stride, const float* bias, void* q,
+              int64_t q_row_stride, float* q_scale, int64_t N, int F);
+int hb_proj_q8(hipStream_t stream, const void* x, int64_t x_row_stride, const float* x_scale, const void* w,
+               int64_t w_row_stride, const float* w_scale, const float* bias, void* out, int out_dtype,
+               int64_t out_row_stride, int64_t M, int K, int F);
+int hb_proj_q4(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, const void* w,
+               int64_t w_row_stride, const void* w_scale, int64_t w_scale_row_stride, const float* bias, int silu,
+               void* out, int64_t out_row_stride, int N, int K, int F);
 
 #ifdef __cplusplus
 }
