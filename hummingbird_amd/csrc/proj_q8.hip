@@ -15,6 +15,7 @@
 
 #include "api.h"
 #include "common.h"
+#include "tiles.h"
 
 namespace hb {
 namespace q8 {
@@ -33,6 +34,7 @@ struct Args {
   int64_t os;
   int64_t M;
   int K, F;
+  bool vec;  // out: 16-byte aligned rows of a multiple of eight features
 };
 
 // e4m3 x e4m3 without block scales, fp32 accumulation.
@@ -49,15 +51,6 @@ __device__ __forceinline__ _Float16 cast_out<_Float16>(float v) { return static_
 template <>
 __device__ __forceinline__ float cast_out<float>(float v) { return v; }
 
-// 32 columns of a row from column k on, zeros from column K on (K a multiple of 16).
-__device__ __forceinline__ i32x8 load32(const uint8_t* row, int k, int K) {
-  u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-  if (k < K) lo = ld16(row + k);
-  if (k + 16 < K) hi = ld16(row + k + 16);
-  return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
-               static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
-}
-
 // 8 e4m3 codes as bf16, exact.
 __device__ __forceinline__ u32x4 widen8(u32x2 c) {
   u32x4 v;
@@ -69,43 +62,605 @@ __device__ __forceinline__ u32x4 widen8(u32x2 c) {
   return v;
 }
 
-// One 32-feature x 32-row tile per wave, a workgroup 64 x 64.
-template <typename T>
-__global__ __launch_bounds__(256) void q8_kernel(const Args a) {
-  const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, wave = wave_id();
-  const int f0 = blockIdx.x * 64 + 32 * (wave & 1);
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 64 + 32 * (wave >> 1);
-  const int f = f0 + lr < a.F ? f0 + lr : a.F - 1;            // rows past an end read a real one;
-  const int64_t m = m0 + lr < a.M ? m0 + lr : a.M - 1;        // their results are not stored
-  const uint8_t* wrow = a.w + f * a.w_rs;
-  const uint8_t* xrow = a.x + m * a.x_rs;
-  f32x16 acc = {};
-  if constexpr (std::is_same<T, float>::value) {
-    auto load8 = [](const uint8_t* p) { return *reinterpret_cast<const u32x2*>(p); };
-    for (int k = 8 * lh; k < a.K; k += 16)
-      acc = mfma_bf16_32x32x16(widen8(load8(wrow + k)), widen8(load8(xrow + k)), acc);
-  } else {
-    for (int k = 0; k < a.K; k += 64)
-      acc = mfma_32x32x64(load32(wrow, k + 32 * lh, a.K), load32(xrow, k + 32 * lh, a.K), acc);
-  }
-  if (m0 + lr >= a.M) return;
-  const float sx = a.sx[m];
-  T* orow = static_cast<T*>(a.out) + m * a.os;
+// ---- Tiled product ------------------------------------------------------------------------------------------
+// A workgroup of WF x WM waves computes FT features x MT rows in steps of 128 columns of K, which stream through two
+// LDS stages: rows of 128 bytes whose 16-byte chunks are XOR-swizzled, filled by global_load_lds. A wave multiplies
+// NF x NM tiles of 32 x 32.
+constexpr int kStep = 128;  // bytes (columns) of K per stage
+
+template <int FT_, int MT_, int WF_, int WM_, int WAVES_>
+struct Tile {
+  static constexpr int FT = FT_, MT = MT_, WF = WF_, WM = WM_;
+  static constexpr int NW = WF * WM, NF = FT / WF / 32, NM = MT / WM / 32;
+  static constexpr int kWaves = WAVES_;  // per SIMD, of the workgroups that share a CU
+  static constexpr int kStage = (FT + MT) * kStep;
+  static constexpr int kBlocksA = FT / 8 / NW, kBlocksB = MT / 8 / NW;  // 1 KB copies per wave and stage
+  static_assert(FT % (8 * NW) == 0 && MT % (8 * NW) == 0 && NF >= 1 && NM >= 1, "whole copies and tiles per wave");
+};
+
+// As lds_dma16 with 4 bytes per lane: 256 bytes at LDS byte address `lds`.
+__device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(sbase) : "m0");
+}
+
+// Byte of logical 16-byte chunk `chunk` of row `row` in a stage: the reads of a fragment (one chunk of consecutive
+// rows) then spread over the banks.
+__device__ __forceinline__ int swz_byte(int row, int chunk) {
+  return row * kStep + 16 * (chunk ^ (row & 7) ^ ((row >> 3) & 1));
+}
+
+// All but the newest N of this wave's copies have landed (older loads and stores too).
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// This wave's LDS reads and writes are done.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The copies of a stage by one wave: blocks wv, wv + NW, ... of the A rows (features), then of the B rows. Lane i's 16
+// bytes land at byte 16 i of a block, row i / 8, position i % 8, so it fetches the chunk that the swizzle puts there.
+template <class TL>
+struct StageCopy {
+  const uint8_t* w0;
+  const uint8_t* x0;
+  uint32_t aoff[TL::kBlocksA], boff[TL::kBlocksB];
+  const int wv = wave_id() % TL::NW, r8 = (threadIdx.x & 63) >> 3, chunk = (threadIdx.x & 7) ^ r8 ^ (wv & 1);
+
+  // Aims the copies at the tile of feature f0 and row m0.
+  __device__ __forceinline__ void aim(const Args& a, int f0, int64_t m0) {
+    w0 = a.w + f0 * a.w_rs;
+    x0 = a.x + m0 * a.x_rs;
+    const int lastf = a.F - 1 - f0;
+    const int64_t lastm = a.M - 1 - m0;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int fo = f0 + 8 * (i >> 2) + 4 * lh + (i & 3);
-    if (fo < a.F) {
-      float v = (acc[i] * sx) * a.sw[fo];
-      if (a.bias) v += a.bias[fo];
-      orow[fo] = cast_out<T>(v);
+    for (int u = 0; u < TL::kBlocksA; ++u) {  // rows past an end read the last one; their results are not stored
+      const int r = 8 * (wv + TL::NW * u) + r8;
+      aoff[u] = static_cast<uint32_t>((r < lastf ? r : lastf) * a.w_rs) + 16 * chunk;
+    }
+#pragma unroll
+    for (int u = 0; u < TL::kBlocksB; ++u) {
+      const int r = 8 * (wv + TL::NW * u) + r8;
+      boff[u] = static_cast<uint32_t>((r < lastm ? r : lastm) * a.x_rs) + 16 * chunk;
+    }
+  }
+  // Copy u of a stage whose columns start at k, to the stage at LDS byte address `stage`.
+  __device__ __forceinline__ void one(int u, int k, uint32_t stage) const {
+    if (u < TL::kBlocksA) lds_dma16(w0 + k, aoff[u], stage + (wv + TL::NW * u) * 1024);
+    else
+      lds_dma16(x0 + k, boff[u - TL::kBlocksA],
+                stage + TL::FT * kStep + (wv + TL::NW * (u - TL::kBlocksA)) * 1024);
+  }
+  static constexpr int kCopies = TL::kBlocksA + TL::kBlocksB;
+  // The last stage where K ends inside it: through registers, zeros from column K on.
+  __device__ __forceinline__ void tail(int k, int K, uint8_t* stage) const {
+    const bool in = k + 16 * chunk < K;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < TL::kBlocksA; ++u) {
+      u32x4 v = {0, 0, 0, 0};
+      if (in) v = ld16(w0 + k + aoff[u]);
+      *reinterpret_cast<u32x4*>(stage + (wv + TL::NW * u) * 1024 + 16 * lane) = v;
+    }
+#pragma unroll
+    for (int u = 0; u < TL::kBlocksB; ++u) {
+      u32x4 v = {0, 0, 0, 0};
+      if (in) v = ld16(x0 + k + boff[u]);
+      *reinterpret_cast<u32x4*>(stage + TL::FT * kStep + (wv + TL::NW * u) * 1024 + 16 * lane) = v;
+    }
+  }
+};
+
+// Half a stage (64 columns) of a wave's operands: 32 bytes of each of its rows, lane half lh the chunks 4 kk + 2 lh + 0, 1.
+template <class TL>
+struct Frags {
+  u32x4 a[TL::NF][2], b[TL::NM][2];
+  static constexpr int kReads = 2 * (TL::NF + TL::NM);
+  __device__ __forceinline__ void read(int i, const uint8_t* st, int fw, int mw, int kk) {
+    const int lr = threadIdx.x & 31, lh = (threadIdx.x & 63) >> 5;
+    const int c = 4 * kk + 2 * lh + (i & 1), t = i >> 1;
+    if (t < TL::NF) a[t][i & 1] = *reinterpret_cast<const u32x4*>(st + swz_byte(fw + 32 * t + lr, c));
+    else
+      b[t - TL::NF][i & 1] =
+          *reinterpret_cast<const u32x4*>(st + TL::FT * kStep + swz_byte(mw + 32 * (t - TL::NF) + lr, c));
+  }
+};
+
+__device__ __forceinline__ i32x8 join(const u32x4 (&v)[2]) {
+  return i32x8{static_cast<int>(v[0][0]), static_cast<int>(v[0][1]), static_cast<int>(v[0][2]),
+               static_cast<int>(v[0][3]), static_cast<int>(v[1][0]), static_cast<int>(v[1][1]),
+               static_cast<int>(v[1][2]), static_cast<int>(v[1][3])};
+}
+
+// One tile's 64 columns: on the e4m3 cores, or (WIDE) as four 16-column products of widened codes on the bf16 cores.
+template <bool WIDE>
+__device__ __forceinline__ f32x16 multiply(const u32x4 (&a)[2], const u32x4 (&b)[2], f32x16 c) {
+  if constexpr (!WIDE) return mfma_32x32x64(join(a), join(b), c);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const u32x2 ga = {a[g >> 1][2 * (g & 1)], a[g >> 1][2 * (g & 1) + 1]};
+    const u32x2 gb = {b[g >> 1][2 * (g & 1)], b[g >> 1][2 * (g & 1) + 1]};
+    c = mfma_bf16_32x32x16(widen8(ga), widen8(gb), c);
+  }
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<uint16_t>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<_Float16>(float lo, float hi) { return F16Io::pack2(lo, hi); }
+
+// A lane half's registers exchanged: `x`'s upper half of the wave (or of each 32 lanes) against `y`'s lower one.
+__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {
+  const u32x2 r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = r[0], y = r[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
+  const u32x2 r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  x = r[0], y = r[1];
+}
+
+// A wave's results. Lane (lr, lh) holds, in registers 4 g .. 4 g + 3 of a 32 x 32 tile, features 8 g + 4 lh .. + 3 of row
+// lr. The results of a tile leave in stores of 16 rows of 64 bytes: for 16-bit types the wave's halves exchange so that
+// a lane holds eight consecutive features, and then its 16-lane rows so that four lanes hold 64 bytes of a row. (Through
+// LDS a tile waits for its own round trip, and one wave per SIMD has nothing else to do: 4.5 us for the 16 tiles of a
+// wave.) GENERAL: any row stride, alignment and number of features, element by element.
+// `sw`, `bias`, `sx`: the scales of this wave's features and rows, in LDS.
+template <typename T, class TL, bool GENERAL>
+__device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL::NF][TL::NM], int f0, int64_t m0,
+                                           const float* sw_, const float* bias_, const float* sx_) {
+  const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+  T* const out = static_cast<T*>(a.out);
+  float sx[TL::NM];
+#pragma unroll
+  for (int t = 0; t < TL::NM; ++t) sx[t] = sx_[32 * t + lr];
+#pragma unroll
+  for (int n = 0; n < TL::NF; ++n) {
+    const int fn = f0 + 32 * n;
+    __builtin_amdgcn_sched_barrier(0);  // the scales of one n at a time: registers
+    float sw[16], bias[16];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 s4 = *reinterpret_cast<const f32x4*>(sw_ + 32 * n + 8 * g + 4 * lh);
+      const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias_ + 32 * n + 8 * g + 4 * lh);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sw[4 * g + j] = s4[j], bias[4 * g + j] = b4[j];
+    }
+#pragma unroll
+    for (int t = 0; t < TL::NM; ++t) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(acc[n][t][i] * sx[t], sw[i], bias[i]);
+      if constexpr (GENERAL) {
+        const int64_t m = m0 + 32 * t + lr;
+        if (m < a.M) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int f = fn + 8 * (i >> 2) + 4 * lh + (i & 3);
+            if (f < a.F) out[m * a.os + f] = cast_out<T>(v[i]);
+          }
+        }
+      } else if constexpr (sizeof(T) == 4) {
+        uint32_t w[4][4];  // [g]: features 8 g + 4 lh .. + 3
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[g][j] = __float_as_uint(v[4 * g + j]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)  // 64 bytes of a row: groups 2 p and 2 p + 1
+#pragma unroll
+          for (int j = 0; j < 4; ++j) swap16(w[2 * p][j], w[2 * p + 1][j]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // rows 16 (q % 2) .. of the tile
+          const int64_t m = m0 + 32 * t + 16 * (q & 1) + (lr & 15);
+          const int f = fn + 16 * (q >> 1) + 8 * (lr >> 4) + 4 * lh;
+          if (m < a.M && f < a.F)
+            *reinterpret_cast<u32x4*>(out + m * a.os + f) = u32x4{w[q][0], w[q][1], w[q][2], w[q][3]};
+        }
+      } else {
+        uint32_t w[4][2];  // [g]: features 8 g + 4 lh .. + 3
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          w[g][0] = pack2<T>(v[4 * g], v[4 * g + 1]);
+          w[g][1] = pack2<T>(v[4 * g + 2], v[4 * g + 3]);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p)  // lane half lh: the eight features of group 2 p + lh
+#pragma unroll
+          for (int j = 0; j < 2; ++j) swap32(w[2 * p][j], w[2 * p + 1][j]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)  // rows 16 p .. of the tile, 16 lanes of groups 0, 1 and 16 of 2, 3 in each half
+#pragma unroll
+          for (int j = 0; j < 2; ++j) swap16(w[p][j], w[2 + p][j]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int64_t m = m0 + 32 * t + 16 * p + (lr & 15);
+          const int f = fn + 16 * (lr >> 4) + 8 * lh;
+          if (m < a.M && f < a.F)
+            *reinterpret_cast<u32x4*>(out + m * a.os + f) =
+                u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]};
+        }
+      }
     }
   }
 }
 
+template <class TL>
+int64_t tiles_of(const Args& a) {
+  return static_cast<int64_t>((a.F + TL::FT - 1) / TL::FT) * ((a.M + TL::MT - 1) / TL::MT);
+}
+
+// Workgroups stay: each takes every gridDim.x-th tile, and its copies run two steps ahead of the products across the
+// tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
+// copy that tile's columns again, for nothing: the loop has no branch around a copy, and the kernel waits for them
+// before it ends. GENERAL: K may end inside the last step, which is then copied through registers; see store_tile.
+template <typename T, class TL, bool GENERAL>
+__global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL::kWaves, TL::kWaves))) void tiled_kernel(
+    const Args a) {
+  constexpr bool WIDE = std::is_same<T, float>::value;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * TL::kStage];
+  // the scales and biases of a tile and of the next: features' scales, biases, rows' scales
+  __shared__ __attribute__((aligned(16))) float scales[2][2 * TL::FT + TL::MT];
+  const int nf = (a.F + TL::FT - 1) / TL::FT, nm = static_cast<int>((a.M + TL::MT - 1) / TL::MT), tiles = nf * nm;
+  // Groups of four feature tiles walk the row tiles together, and the workgroups of an XCD take consecutive tiles, so
+  // that both operands are read from its L2.
+  auto origin = [&](int p, int& f0, int64_t& m0) {
+    constexpr int GF = 4;
+    const int id = xcd_remap(p, tiles), g = id / (GF * nm), gs = nf - g * GF < GF ? nf - g * GF : GF;
+    const int in = id - g * GF * nm;
+    f0 = (g * GF + in % gs) * TL::FT;
+    m0 = static_cast<int64_t>(in / gs) * TL::MT;
+  };
+  const int wv = wave_id(), fw = wv % TL::WF * (32 * TL::NF), mw = wv / TL::WF * (32 * TL::NM);
+  const uint32_t lds0 = lds_addr(smem);
+  const int nk = (a.K + kStep - 1) / kStep;
+  const bool ragged = GENERAL && a.K % kStep != 0;
+
+  // What is copied next: step `cs` of tile `ct` (in the order of p).
+  StageCopy<TL> copy;
+  int ct = blockIdx.x, cs = 0;
+  auto aim = [&]() {
+    int f0;
+    int64_t m0;
+    origin(ct, f0, m0);
+    copy.aim(a, f0, m0);
+  };
+  auto advance = [&]() {
+    if (++cs < nk) return;
+    cs = 0;
+    if (ct + static_cast<int>(gridDim.x) >= tiles) return;
+    ct += gridDim.x;
+    aim();
+  };
+  auto slow = [&]() { return ragged && cs == nk - 1; };  // a step for copy.tail
+  constexpr int kTiles = TL::NF * TL::NM, kReads = Frags<TL>::kReads, kCopies = StageCopy<TL>::kCopies;
+  // A tile's scales, 64 of each kind by a wave, copied while its first step runs; tiles alternate between the sets.
+  auto copy_scales = [&](int f0, int64_t m0, int set) {
+    const uint32_t to = lds_addr(scales[set]) + 256 * wv;
+    const int lane = threadIdx.x & 63, i = 64 * wv + lane;
+    if (64 * wv < TL::FT) {
+      const int f = i < a.F - 1 - f0 ? i : a.F - 1 - f0;
+      lds_dma4(a.sw + f0, 4 * f, to);
+      if (a.bias) lds_dma4(a.bias + f0, 4 * f, to + 4 * TL::FT);
+    }
+    if (64 * wv < TL::MT) {
+      const int64_t last = a.M - 1 - m0;
+      lds_dma4(a.sx + m0, static_cast<uint32_t>(4 * (i < last ? i : last)), to + 8 * TL::FT);
+    }
+  };
+  if (!a.bias && threadIdx.x < TL::FT) scales[0][TL::FT + threadIdx.x] = scales[1][TL::FT + threadIdx.x] = 0.f;
+  aim();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (slow()) {
+      copy.tail(cs * kStep, a.K, smem + i * TL::kStage);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kCopies; ++u) copy.one(u, cs * kStep, lds0 + i * TL::kStage);
+    }
+    advance();
+  }
+  wait_copies<GENERAL ? 0 : kCopies>();
+  wait_lds();
+  barrier();
+  Frags<TL> lo, hi;
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) lo.read(i, smem, fw, mw, 0);
+
+  // A step of a wave is 2 kTiles products, lo's and hi's. In the first kFree the operands of hi are read; then every wave
+  // has the whole stage in registers (barrier) and the step after the next is copied into it, over kTiles products:
+  // faster, the copies wait for the address unit and hold up the products. Before hi's products the next step's copies,
+  // issued a step ago, have landed (barrier), and its lo is read during them.
+  constexpr int kFree = kTiles / 2;                                    // 0: one barrier does for both
+  constexpr int kEarly = (kTiles - kFree) * kCopies / kTiles;          // copies issued before the second barrier
+  uint32_t b = 0;                                                      // byte offset of the step's stage
+  int set = 0;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, set ^= 1) {
+    int f0;
+    int64_t m0;
+    origin(tile, f0, m0);
+    copy_scales(f0, m0, set);
+    f32x16 acc[TL::NF][TL::NM];
+#pragma unroll
+    for (int i = 0; i < TL::NF; ++i)
+#pragma unroll
+      for (int j = 0; j < TL::NM; ++j) acc[i][j] = f32x16{};
+    for (int s = 0; s < nk; ++s) {
+      const bool by_registers = slow();
+      const uint32_t stage = __builtin_amdgcn_readfirstlane(lds0 + b);
+      const int k = cs * kStep;
+      auto copies = [&](int j) {  // those of product j past the barrier
+        if (GENERAL && by_registers) return;
+#pragma unroll
+        for (int u = j * kCopies / kTiles; u < (j + 1) * kCopies / kTiles; ++u) copy.one(u, k, stage);
+      };
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        if (kFree == 0 || i < kFree) {
+          constexpr int n = kFree == 0 ? kTiles : kFree;
+#pragma unroll
+          for (int r = i * kReads / n; r < (i + 1) * kReads / n; ++r) hi.read(r, smem + b, fw, mw, 1);
+        }
+        if (kFree > 0 && i == kFree) {
+          wait_lds();
+          barrier();
+          if (by_registers) copy.tail(k, a.K, smem + b);
+        }
+        if (kFree > 0 && i >= kFree) copies(i - kFree);
+        acc[i / TL::NM][i % TL::NM] = multiply<WIDE>(lo.a[i / TL::NM], lo.b[i % TL::NM], acc[i / TL::NM][i % TL::NM]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_copies<GENERAL || kFree == 0 ? 0 : kEarly>();
+      if (GENERAL || kFree == 0) wait_lds();
+      barrier();
+      if (kFree == 0 && by_registers) copy.tail(k, a.K, smem + b);
+      b = TL::kStage - b;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        if (kFree == 0) copies(i);
+        else if (i < kFree) copies(kTiles - kFree + i);
+        // (after the very last step, of a stage that nothing needs)
+#pragma unroll
+        for (int r = i * kReads / kTiles; r < (i + 1) * kReads / kTiles; ++r) lo.read(r, smem + b, fw, mw, 0);
+        acc[i / TL::NM][i % TL::NM] = multiply<WIDE>(hi.a[i / TL::NM], hi.b[i % TL::NM], acc[i / TL::NM][i % TL::NM]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      advance();
+    }
+    const float* sc = scales[set];
+    store_tile<T, TL, GENERAL>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
+  }
+  wait_copies<0>();
+}
+
+template <typename T, class TL>
+void launch_tiled(hipStream_t stream, const Args& a) {
+  const int64_t tiles = tiles_of<TL>(a), slots = static_cast<int64_t>(TL::kWaves) * 4 / TL::NW * device_cus();
+  const dim3 grid(static_cast<unsigned>(tiles < slots ? tiles : slots)), block(64 * TL::NW);
+  if (a.K % kStep || !a.vec) hipLaunchKernelGGL((tiled_kernel<T, TL, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((tiled_kernel<T, TL, false>), grid, block, 0, stream, a);
+}
+
+// ---- Few tiles ------------------------------------------------------------------------------------------------
+// A product of fewer tiles than CUs, split along K inside the workgroup: kGroups groups of waves, each with stages of its
+// own, take consecutive steps of one tile, and their sums are added in the groups' order through LDS.
+constexpr int kGroups = 4;
+
+template <typename T, class TL, bool GENERAL>
+__global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args a) {
+  static_assert(TL::NF == 1 && TL::NM == 1, "a 32 x 32 tile per wave");
+  constexpr bool WIDE = std::is_same<T, float>::value;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kGroups * TL::kStage];
+  __shared__ __attribute__((aligned(16))) float scales[2 * TL::FT + TL::MT];
+  static_assert((kGroups - 1) * TL::NW * 4096 <= 2 * kGroups * TL::kStage, "the groups' sums fit the stages");
+  const int nf = (a.F + TL::FT - 1) / TL::FT;
+  const int f0 = static_cast<int>(blockIdx.x) % nf * TL::FT;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.x / nf) * TL::MT;
+  const int group = wave_id() / TL::NW, wv = wave_id() % TL::NW, lane = threadIdx.x & 63;
+  const int fw = wv % TL::WF * 32, mw = wv / TL::WF * 32;
+  const int nk = (a.K + kStep - 1) / kStep, per = (nk + kGroups - 1) / kGroups, first = group * per;
+  const int mine = nk - first < per ? nk - first : per;  // steps of this group, possibly none; barriers are for `per`
+  const bool ragged = GENERAL && a.K % kStep != 0;
+  uint8_t* const stages = smem + 2 * group * TL::kStage;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + 2 * group * TL::kStage);
+  if (threadIdx.x < TL::FT) {
+    const int f = f0 + static_cast<int>(threadIdx.x) < a.F ? f0 + static_cast<int>(threadIdx.x) : a.F - 1;
+    scales[threadIdx.x] = a.sw[f];
+    scales[TL::FT + threadIdx.x] = a.bias ? a.bias[f] : 0.f;
+  }
+  if (threadIdx.x < TL::MT) {
+    const int64_t m = m0 + threadIdx.x < a.M ? m0 + threadIdx.x : a.M - 1;
+    scales[2 * TL::FT + threadIdx.x] = a.sx[m];
+  }
+  StageCopy<TL> copy;
+  copy.aim(a, f0, m0);
+  constexpr int kReads = Frags<TL>::kReads, kCopies = StageCopy<TL>::kCopies;
+  auto fill = [&](int s) {  // the group's step s into stage s % 2
+    if (s >= mine) return;
+    const int k = (first + s) * kStep;
+    if (ragged && first + s == nk - 1) {
+      copy.tail(k, a.K, stages + (s & 1) * TL::kStage);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kCopies; ++u) copy.one(u, k, lds0 + (s & 1) * TL::kStage);
+    }
+  };
+  fill(0);
+  fill(1);
+  f32x16 acc[1][1] = {{f32x16{}}};
+  for (int s = 0; s < per; ++s) {
+    // step s has landed: all copies but those of step s + 1
+    if (!ragged && s + 1 < mine) wait_copies<kCopies>();
+    else wait_copies<0>();
+    wait_lds();
+    barrier();
+    Frags<TL> lo, hi;
+    if (s < mine) {
+      const uint8_t* st = stages + (s & 1) * TL::kStage;
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) lo.read(i, st, fw, mw, 0);
+#pragma unroll
+      for (int i = 0; i < kReads; ++i) hi.read(i, st, fw, mw, 1);
+    }
+    wait_lds();
+    barrier();  // the stage is free
+    fill(s + 2);
+    if (s < mine) {
+      acc[0][0] = multiply<WIDE>(lo.a[0], lo.b[0], acc[0][0]);
+      acc[0][0] = multiply<WIDE>(hi.a[0], hi.b[0], acc[0][0]);
+    }
+  }
+  // (every wave's reads ended before the last barrier, and no copy is in flight)
+  f32x4* const sums = reinterpret_cast<f32x4*>(smem);  // [group - 1][wave][4][64 lanes]
+  if (group > 0) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      sums[(((group - 1) * TL::NW + wv) * 4 + g) * 64 + lane] =
+          f32x4{acc[0][0][4 * g], acc[0][0][4 * g + 1], acc[0][0][4 * g + 2], acc[0][0][4 * g + 3]};
+  }
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int o = 0; o < kGroups - 1; ++o)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = sums[((o * TL::NW + wv) * 4 + g) * 64 + lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[0][0][4 * g + j] += v[j];
+    }
+  store_tile<T, TL, GENERAL>(a, acc, f0 + fw, m0 + mw, scales + fw, scales + TL::FT + fw, scales + 2 * TL::FT + mw);
+}
+
+template <typename T, class TL>
+void launch_split(hipStream_t stream, const Args& a) {
+  const dim3 grid(static_cast<unsigned>(tiles_of<TL>(a))), block(64 * TL::NW * kGroups);
+  if (a.K % kStep || !a.vec) hipLaunchKernelGGL((split_kernel<T, TL, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((split_kernel<T, TL, false>), grid, block, 0, stream, a);
+}
+
+// ---- Few rows -----------------------------------------------------------------------------------------------
+// Up to 16 CT rows, where the weights' bytes are the cost: each is read once, straight into the registers of the wave that
+// multiplies it. A workgroup computes 16 features for all rows; its waves take the 128-column chunks of K in turns and
+// their partial sums are added in the waves' order. On v_mfma_f32_16x16x128_f8f6f4 a lane holds 32 consecutive columns
+// of feature (or row) lane % 16.
+constexpr int kMaxWaves = 16;
+
+__device__ __forceinline__ f32x4 mfma_16x16x128(i32x8 a, i32x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_bf16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+
+template <bool WIDE>
+__device__ __forceinline__ f32x4 multiply16(const u32x4 (&a)[2], const u32x4 (&b)[2], f32x4 c) {
+  if constexpr (!WIDE) return mfma_16x16x128(join(a), join(b), c);
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const u32x2 ga = {a[g >> 1][2 * (g & 1)], a[g >> 1][2 * (g & 1) + 1]};
+    const u32x2 gb = {b[g >> 1][2 * (g & 1)], b[g >> 1][2 * (g & 1) + 1]};
+    c = mfma_bf16_16x16x32(widen8(ga), widen8(gb), c);
+  }
+  return c;
+}
+
+// 32 columns of a row from column k on, zeros from column K on (K a multiple of 16).
+__device__ __forceinline__ void load32(const uint8_t* row, int k, int K, u32x4 (&v)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[i] = u32x4{0, 0, 0, 0};
+    if (k + 16 * i < K) v[i] = ld16(row + k + 16 * i);
+  }
+}
+
+template <typename T, int CT>
+__global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(const Args a) {
+  constexpr bool WIDE = std::is_same<T, float>::value;
+  __shared__ float part[kMaxWaves][CT][16][17];  // [wave][row tile][row][feature]
+  const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4, wave = wave_id(), waves = blockDim.x >> 6;
+  const int f0 = blockIdx.x * 16, M = static_cast<int>(a.M);
+  const uint8_t* wrow = a.w + (f0 + lr < a.F ? f0 + lr : a.F - 1) * a.w_rs;  // past the end: not stored
+  const uint8_t* xrow[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) xrow[t] = a.x + (16 * t + lr < M ? 16 * t + lr : M - 1) * a.x_rs;
+  f32x4 acc[CT];
+#pragma unroll
+  for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int chunks = (a.K + kStep - 1) / kStep;
+  u32x4 w[2][2], x[2][CT][2];
+  auto load = [&](int c, int buf) {
+    const int k = c * kStep + 32 * lq;
+    load32(wrow, k, a.K, w[buf]);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) load32(xrow[t], k, a.K, x[buf][t]);
+  };
+  // The loads of a wave's next chunk are in flight while it multiplies this one.
+  int c = wave;
+  load(c, 0);
+  for (; c < chunks; c += 2 * waves) {
+    if (c + waves < chunks) load(c + waves, 1);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) acc[t] = multiply16<WIDE>(w[0], x[0][t], acc[t]);
+    if (c + waves >= chunks) break;
+    if (c + 2 * waves < chunks) load(c + 2 * waves, 0);
+#pragma unroll
+    for (int t = 0; t < CT; ++t) acc[t] = multiply16<WIDE>(w[1], x[1][t], acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < CT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[wave][t][lr][4 * lq + i] = acc[t][i];
+  __syncthreads();
+  T* const out = static_cast<T*>(a.out);
+  for (int e = threadIdx.x; e < 256 * CT; e += blockDim.x) {
+    const int r = e >> 4, fo = e & 15;
+    if (r >= M || f0 + fo >= a.F) continue;
+    float v = 0.f;
+    for (int i = 0; i < waves; ++i) v += part[i][r >> 4][r & 15][fo];
+    out[r * a.os + f0 + fo] = cast_out<T>(__fmaf_rn(v * a.sx[r], a.sw[f0 + fo], a.bias ? a.bias[f0 + fo] : 0.f));
+  }
+}
+
+template <typename T, int CT>
+void launch_few_rows(hipStream_t stream, const Args& a) {
+  const int chunks = (a.K + kStep - 1) / kStep;
+  hipLaunchKernelGGL((few_rows_kernel<T, CT>), dim3(static_cast<unsigned>((a.F + 15) / 16)),
+                     dim3(64 * (chunks < kMaxWaves ? chunks : kMaxWaves)), 0, stream, a);
+}
+
+// Which kernel, as measured (kernel times in us; K = 1536 unless said):
+//   few rows   up to 16 rows (7 x 7680: 5.3 against 6.3 split, 7.9 Small), and up to 32 of a narrow product (24 x 1536:
+//              4.7 against 5.9; but 32 x 7680: 7.6 against 6.4);
+//   split      at most a Small tile per CU and more than 8 steps of K (300 x 1536, K = 6144: 14.4 against 23.1; 64 x 7680:
+//              6.5 against 8.2; at K = 1024 nothing is gained);
+//   Small      products of fewer Medium tiles than keep the CUs busy (700 x 1536, 72 tiles: 8.6 against 9.0; 1300 x 1536,
+//              132 tiles: 10.1 against 9.7; the bf16 cores of fp32 outputs take longer, and the border lies at 192);
+//   Medium     two workgroups share a CU, one's epilogue beside the other's products (2584 x 12288: 50.6 against 57.5
+//              Large);
+//   Large      16-bit outputs whose last round of workgroups is not too empty: a round of Large takes 0.95 of one of
+//              Medium (5168 x 7680: 61.0 against 62.0; 5168 x 1536, K = 6144: 41.1 against 44.6).
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
-  const dim3 grid(static_cast<unsigned>((a.F + 63) / 64), static_cast<unsigned>((a.M + 63) / 64));
-  hipLaunchKernelGGL((q8_kernel<T>), grid, dim3(256), 0, stream, a);
+  using Small = Tile<64, 64, 2, 2, 3>;
+  using Medium = Tile<128, 128, 2, 2, 2>;
+  using Large = Tile<128, 256, 2, 2, 1>;
+  const int64_t cus = device_cus(), small = tiles_of<Small>(a), medium = tiles_of<Medium>(a);
+  if (a.M <= 16) return launch_few_rows<T, 1>(stream, a);
+  if (a.M <= 32 && small <= cus / 4) return launch_few_rows<T, 2>(stream, a);
+  if (small <= cus && a.K > 8 * kStep) return launch_split<T, Small>(stream, a);
+  if (medium <= (sizeof(T) == 4 ? cus * 3 / 4 : cus * 3 / 8)) return launch_tiled<T, Small>(stream, a);
+  if constexpr (sizeof(T) == 2) {
+    const int64_t rest = medium % (2 * cus);
+    const double rounds = static_cast<double>(medium / (2 * cus)) + (rest > cus ? 1.0 : rest > 0 ? 0.65 : 0.0);
+    const int64_t large = tiles_of<Large>(a);
+    if (0.95 * static_cast<double>((large + cus - 1) / cus) <= rounds) return launch_tiled<T, Large>(stream, a);
+  }
+  launch_tiled<T, Medium>(stream, a);
 }
 
 }  // namespace q8
@@ -120,17 +675,19 @@ extern "C" int hb_proj_q8(hipStream_t stream, const void* x, int64_t x_row_strid
   const char* what = "proj_q8";
   if (out_dtype != HB_BF16 && out_dtype != HB_F32 && out_dtype != HB_F16)
     return fail(HB_ERR_DTYPE, "%s: dtype %d is not HB_BF16 (0), HB_F32 (1) or HB_F16 (2)", what, out_dtype);
-  if (M < 1 || M > (1 << 21) || F < 1 || F > (1 << 21) || K < 16 || K > (1 << 24) || K % 16)
-    return fail(HB_ERR_SHAPE, "%s needs 1 <= M, F <= 2^21 and K a multiple of 16 up to 2^24 (M=%lld, K=%d, F=%d)", what,
+  if (M < 1 || M > (1 << 21) || F < 1 || F > (1 << 21) || K < 16 || K > (1 << 23) || K % 16)
+    return fail(HB_ERR_SHAPE, "%s needs 1 <= M, F <= 2^21 and K a multiple of 16 up to 2^23 (M=%lld, K=%d, F=%d)", what,
                 static_cast<long long>(M), K, F);
   if (!x || !x_scale || !w || !w_scale || !out)
     return fail(HB_ERR_NULL, "%s: x, x_scale, w, w_scale and out must be non-NULL", what);
   const int es = out_dtype == HB_F32 ? 4 : 2;
   auto misaligned = [](const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n != 0; };
-  if (misaligned(x, 16) || x_row_stride < K || x_row_stride % 16)
-    return fail(HB_ERR_STRIDE, "%s: x must be 16-byte aligned with a row stride >= K, a multiple of 16", what);
-  if (misaligned(w, 16) || w_row_stride < K || w_row_stride % 16)
-    return fail(HB_ERR_STRIDE, "%s: w must be 16-byte aligned with a row stride >= K, a multiple of 16", what);
+  // A tile's rows are addressed by 32-bit offsets from its first.
+  auto bad_rows = [&](const void* p, int64_t rs) { return misaligned(p, 16) || rs < K || rs % 16 || rs > (1 << 23); };
+  const char* rows_of = bad_rows(x, x_row_stride) ? "x" : bad_rows(w, w_row_stride) ? "w" : nullptr;
+  if (rows_of)
+    return fail(HB_ERR_STRIDE, "%s: %s must be 16-byte aligned with a row stride >= K, a multiple of 16 up to 2^23", what,
+                rows_of);
   if (misaligned(out, es) || out_row_stride < F)
     return fail(HB_ERR_STRIDE, "%s: out must be aligned to its elements with a row stride >= F", what);
   int st;
@@ -145,7 +702,8 @@ extern "C" int hb_proj_q8(hipStream_t stream, const void* x, int64_t x_row_strid
       (st = check_disjoint(what, "out", out, ob, "bias", bias, static_cast<int64_t>(F) * 4)))
     return st;
   const q8::Args a = {static_cast<const uint8_t*>(x), x_row_stride, x_scale, static_cast<const uint8_t*>(w),
-                      w_row_stride, w_scale, bias, out, out_row_stride, M, K, F};
+                      w_row_stride, w_scale, bias, out, out_row_stride, M, K, F,
+                      !misaligned(out, 16) && out_row_stride * es % 16 == 0 && F % 8 == 0};
   if (out_dtype == HB_BF16) q8::launch<uint16_t>(stream, a);
   else if (out_dtype == HB_F16) q8::launch<_Float16>(stream, a);
   else q8::launch<float>(stream, a);
