@@ -112,6 +112,18 @@ def current_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def launch(fn, what: str, device: torch.device, *args) -> None:
+    """`fn(stream, *args)` on `device`'s current stream with `device` the current one (a launch needs that), checked.
+    `torch.cuda.device` is entered only where it changes something: it costs 1.1 us, the query 0.1."""
+    if torch._C._cuda_getDevice() == device.index:
+        status = fn(torch._C._cuda_getCurrentRawStream(device.index), *args)
+    else:
+        with torch.cuda.device(device):
+            status = fn(torch._C._cuda_getCurrentRawStream(device.index), *args)
+    if status:
+        check(status, what)
+
+
 def check(status: int, what: str) -> None:
     """Raise the exception matching a non-zero status, with the library's message."""
     if status == HB_OK:

@@ -9,8 +9,8 @@
 // rows, an fp32 row three (each the next 8 bits of the value, the remainders exact), and those rows are further columns
 // of the same MFMA, whose 16 columns a single row leaves empty anyway. Sums are fp32.
 //
-// One workgroup computes 16 features for all columns; its waves take the 128-column chunks of K in turns and their
-// partial sums are added in the waves' order. On v_mfma_f32_16x16x32_bf16 a lane holds 8 consecutive columns of feature
+// A workgroup computes 16 or 64 features for up to 64 columns; its waves take the 128-column chunks of K in turns and
+// their partial sums are added in the waves' order. On v_mfma_f32_16x16x32_bf16 a lane holds 8 consecutive columns of feature
 // (or row) lane % 16; which 8 is free as long as both operands agree, so quarter lane / 16 takes columns 32 q + 8 i of
 // the chunk in MFMA i: a lane's 16 bytes of codes are then one scale group, read in one load.
 #include "api.h"
@@ -19,8 +19,8 @@
 namespace hb {
 namespace q4 {
 
-constexpr int kChunk = 128;  // columns of K per step: four groups
 constexpr int kGroup = 32;
+constexpr int kChunk = 128;  // columns of K per step of a wave: a group for each quarter of the lanes
 constexpr int kMaxWaves = 16;
 
 struct Args {
@@ -35,52 +35,61 @@ struct Args {
   void* out;  // (N, F), row stride os elements
   int64_t os;
   int N, K, F;
+  bool vec;  // out: rows of a multiple of four features, aligned to four
 };
 
-// Rows of x as bf16 rows whose sum they are: P pieces, each the leading 8 bits of what the earlier ones leave
-// (truncated, so that no piece overflows and every remainder is exact). An infinity or NaN is the first piece alone.
+// Rows of x as bf16 rows whose sum they are: P pieces, each the leading 8 bits of what the earlier ones leave (truncated,
+// so that no piece overflows and every remainder is exact). Piece p is x after p times y -= y & 0xffff0000, cut to its
+// upper half: a lane holds the masks of its piece, zero past it. An infinity or NaN leaves NaNs in the later pieces;
+// what counts then is the first one's sum (see the end of the kernel).
 template <typename T>
 struct Pieces;
 template <>
 struct Pieces<uint16_t> {  // bf16
   static constexpr int P = 1;
-  __device__ static u32x4 load8(const uint16_t* p, int) { return ld16(p); }
+  __device__ explicit Pieces(int) {}
+  __device__ u32x4 load8(const uint16_t* p) const { return ld16(p); }
 };
-__device__ __forceinline__ float piece_of(float x, int piece) {
-  const float hi = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-  const bool finite = (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
-  if (!finite) return piece == 0 ? round_bf16(x) : 0.f;
-  if (piece == 0) return hi;
-  const float r = x - hi, mid = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  return piece == 1 ? mid : r - mid;
-}
-__device__ __forceinline__ u32x4 pack_pieces(const float (&x)[8], int piece) {
-  float v[8];
+// The upper halves of eight fp32 values.
+__device__ __forceinline__ u32x4 upper8(const float (&x)[8]) {
+  u32x4 v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = piece_of(x[j], piece);
-  return pack8(v);  // each value is a bf16 already
+  for (int i = 0; i < 4; ++i)
+    v[i] = __builtin_amdgcn_perm(__float_as_uint(x[2 * i + 1]), __float_as_uint(x[2 * i]), 0x07060302u);
+  return v;
+}
+// y - (y & mask): x itself where the mask is zero (a signalling NaN quieted, so that its upper half stays one).
+__device__ __forceinline__ float without_upper(float y, uint32_t mask) {
+  return __fsub_rn(y, __uint_as_float(__float_as_uint(y) & mask));
 }
 template <>
 struct Pieces<_Float16> {
   static constexpr int P = 2;
-  __device__ static u32x4 load8(const _Float16* p, int piece) {
+  uint32_t m1;
+  __device__ explicit Pieces(int piece) : m1(piece >= 1 ? 0xffff0000u : 0u) {}
+  __device__ u32x4 load8(const _Float16* p) const {
     float x[8];
     F16Io::unpack8(ld16(p), x);
-    return pack_pieces(x, piece);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = without_upper(x[j], m1);
+    return upper8(x);
   }
 };
 template <>
 struct Pieces<float> {
   static constexpr int P = 3;
-  __device__ static u32x4 load8(const float* p, int piece) {
+  uint32_t m1, m2;
+  __device__ explicit Pieces(int piece)
+      : m1(piece >= 1 ? 0xffff0000u : 0u), m2(piece >= 2 ? 0xffff0000u : 0u) {}
+  __device__ u32x4 load8(const float* p) const {
     float x[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const f32x4 v = *reinterpret_cast<const f32x4*>(p + 4 * i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[4 * i + j] = v[j];
+      for (int j = 0; j < 4; ++j) x[4 * i + j] = without_upper(without_upper(v[j], m1), m2);
     }
-    return pack_pieces(x, piece);
+    return upper8(x);
   }
 };
 
@@ -108,80 +117,153 @@ __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
                                                  0);
 }
 
-// CT tiles of 16 columns (rows of x times pieces) starting at column blockIdx.y * 16 CT.
-template <typename T, int CT>
-__global__ __launch_bounds__(64 * kMaxWaves) void q4_kernel(const Args a) {
-  constexpr int P = Pieces<T>::P;
-  __shared__ float part[kMaxWaves][CT][16][17];  // [wave][tile][feature][column]
+// A wave's sums over the chunks wave, wave + waves, ... for FT tiles of 16 features and CT tiles of 16 columns (rows of x
+// times pieces), from feature 16 FT blockIdx.x and row `rows` blockIdx.y on. x is read once for the FT tiles.
+// Waves of a workgroup: the sums of all its waves, 1 KB for each of a wave's tiles, take at most 128 KB.
+constexpr int max_waves(int tiles) { return 128 / tiles < kMaxWaves ? 128 / tiles : kMaxWaves; }
+
+template <typename T, int CT, int FT>
+__global__ __launch_bounds__(64 * max_waves(CT * FT)) void q4_kernel(const Args a) {
+  constexpr int P = Pieces<T>::P, R = 16 / P;  // whole rows per tile
+  __shared__ __attribute__((aligned(16))) f32x4 sums[max_waves(CT * FT) * FT * CT * 64];  // [wave][FT][CT][64 lanes]
   const int lane = threadIdx.x & 63, lr = lane & 15, lq = lane >> 4, wave = wave_id(), waves = blockDim.x >> 6;
-  const int f0 = blockIdx.x * 16, f = f0 + lr < a.F ? f0 + lr : a.F - 1;  // features past the end are not stored
-  const int rows = 16 * CT / P;  // whole rows per workgroup
-  const int row0 = blockIdx.y * rows;
-  const uint8_t* wrow = a.w + f * a.w_rs;
-  const uint8_t* srow = a.ws + f * a.ws_rs;
-  const T* xrow[CT];
-  int piece[CT];
+  const int f0 = blockIdx.x * 16 * FT, row0 = blockIdx.y * R * CT;
+  const uint8_t* wrow[FT];
+  const uint8_t* srow[FT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    const int col = 16 * t + lr, r = col / P, row = row0 + r;
-    piece[t] = col - r * P;
-    xrow[t] = r < rows && row < a.N ? static_cast<const T*>(a.x) + row * a.xs : nullptr;
+  for (int t = 0; t < FT; ++t) {
+    const int f = f0 + 16 * t + lr < a.F ? f0 + 16 * t + lr : a.F - 1;  // features past the end are not stored
+    wrow[t] = a.w + f * a.w_rs;
+    srow[t] = a.ws + f * a.ws_rs;
   }
-  f32x4 acc[CT];
+  const T* xrow[CT];
+  const int r = lr / P, piece = lr - r * P;  // this lane's row in a tile and its piece
+  const Pieces<T> pieces(piece);
 #pragma unroll
-  for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int u = 0; u < CT; ++u) {
+    const int row = row0 + R * u + r;
+    xrow[u] = r < R && row < a.N ? static_cast<const T*>(a.x) + row * a.xs : nullptr;
+  }
+  float bias[FT][4];  // of this lane's results, loaded here so that nothing waits for them at the end
+#pragma unroll
+  for (int t = 0; t < FT; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int f = f0 + 16 * t + 4 * lq + j;
+      bias[t][j] = a.bias ? a.bias[f < a.F ? f : a.F - 1] : 0.f;
+    }
+  f32x4 acc[FT][CT];
+#pragma unroll
+  for (int t = 0; t < FT; ++t)
+#pragma unroll
+    for (int u = 0; u < CT; ++u) acc[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int chunks = (a.K + kChunk - 1) / kChunk;
   for (int c = wave; c < chunks; c += waves) {
     const int k0 = c * kChunk + kGroup * lq;  // this lane's group
-    const bool in = k0 < a.K;                 // K is a multiple of the group
-    u32x4 code = u32x4{0, 0, 0, 0};
-    float scale = 1.f;
-    if (in) {
-      code = ld16(wrow + (k0 >> 1));
-      scale = __uint_as_float(static_cast<uint32_t>(srow[k0 / kGroup]) << 23);
-    }
+    u32x4 code[FT];
+    uint32_t scale[FT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const u32x4 wv = dequant8(code[i], scale);
-#pragma unroll
-      for (int t = 0; t < CT; ++t) {
-        u32x4 xv = u32x4{0, 0, 0, 0};
-        if (in && xrow[t]) xv = Pieces<T>::load8(xrow[t] + k0 + 8 * i, piece[t]);
-        acc[t] = mfma_16x16x32(wv, xv, acc[t]);
+    for (int t = 0; t < FT; ++t) {
+      code[t] = u32x4{0, 0, 0, 0};
+      scale[t] = 127;
+      if (k0 < a.K) {  // K is a multiple of the group
+        code[t] = ld16(wrow[t] + (k0 >> 1));
+        scale[t] = srow[t][k0 / kGroup];
       }
     }
+    u32x4 x[CT][4];
+#pragma unroll
+    for (int u = 0; u < CT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[u][i] = u32x4{0, 0, 0, 0};
+        if (k0 < a.K && xrow[u]) x[u][i] = pieces.load8(xrow[u] + k0 + 8 * i);
+      }
+#pragma unroll
+    for (int t = 0; t < FT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 wv = dequant8(code[t][i], __uint_as_float(scale[t] << 23));
+#pragma unroll
+        for (int u = 0; u < CT; ++u) acc[t][u] = mfma_16x16x32(wv, x[u][i], acc[t][u]);
+      }
   }
+  if (waves > 1) {
 #pragma unroll
-  for (int t = 0; t < CT; ++t)
+    for (int t = 0; t < FT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[wave][t][4 * lq + i][lr] = acc[t][i];
-  __syncthreads();
-  for (int e = threadIdx.x; e < 16 * rows; e += blockDim.x) {
-    const int r = e >> 4, fo = e & 15, row = row0 + r;
-    if (row >= a.N || f0 + fo >= a.F) continue;
-    float v = 0.f;
-    for (int p = 0; p < P; ++p) {
-      const int col = r * P + p;
-      for (int w = 0; w < waves; ++w) v += part[w][col >> 4][fo][col & 15];
+      for (int u = 0; u < CT; ++u) sums[((wave * FT + t) * CT + u) * 64 + lane] = acc[t][u];
+    __syncthreads();
+  }
+  // Tile (t, u) is finished by wave (t CT + u) % waves: lane (lr, lq) has column lr and features 4 lq .. + 3.
+#pragma unroll
+  for (int t = 0; t < FT; ++t)
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+      if ((t * CT + u) % waves != wave) continue;
+      f32x4 v = acc[t][u];
+      if (waves > 1) {
+        v = sums[(t * CT + u) * 64 + lane];
+        for (int i = 1; i < waves; ++i) {
+          const f32x4 o = sums[((i * FT + t) * CT + u) * 64 + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += o[j];
+        }
+      }
+      // A row's pieces are in P neighbouring columns: added where the row starts, unless the first sum is not finite.
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float mine = v[j];
+        float sum = mine;
+#pragma unroll
+        for (int p = 1; p < P; ++p) sum += __shfl_down(mine, p, kWave);
+        v[j] = __builtin_isfinite(mine) ? sum : mine;
+      }
+      const int row = row0 + R * u + r, f = f0 + 16 * t + 4 * lq;
+      if (piece != 0 || r >= R || row >= a.N) continue;
+      T y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float z = v[j] + bias[t][j];
+        if (a.silu) z = z * __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z));
+        y[j] = cast_out<T>(z);
+      }
+      T* o = static_cast<T*>(a.out) + row * a.os + f;
+      if (a.vec) {
+        if (f < a.F) __builtin_memcpy(__builtin_assume_aligned(o, 4 * sizeof(T)), y, sizeof(y));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (f + j < a.F) o[j] = y[j];
+      }
     }
-    if (a.bias) v += a.bias[f0 + fo];
-    if (a.silu) v = v * __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * v));
-    static_cast<T*>(a.out)[row * a.os + f0 + fo] = cast_out<T>(v);
-  }
 }
 
+template <typename T, int CT, int FT>
+void launch_tiles(hipStream_t stream, const Args& a) {
+  constexpr int R = 16 / Pieces<T>::P, kMax = max_waves(CT * FT);
+  const int chunks = (a.K + kChunk - 1) / kChunk;
+  const dim3 grid(static_cast<unsigned>((a.F + 16 * FT - 1) / (16 * FT)),
+                  static_cast<unsigned>((a.N + R * CT - 1) / (R * CT)));
+  hipLaunchKernelGGL((q4_kernel<T, CT, FT>), grid, dim3(64 * (chunks < kMax ? chunks : kMax)), 0, stream, a);
+}
+
+template <typename T, int FT>
+void launch_rows(hipStream_t stream, const Args& a) {
+  constexpr int R = 16 / Pieces<T>::P;
+  if (a.N <= R) launch_tiles<T, 1, FT>(stream, a);
+  else if (a.N <= 2 * R) launch_tiles<T, 2, FT>(stream, a);
+  else if (a.N <= 3 * R) launch_tiles<T, 3, FT>(stream, a);
+  else launch_tiles<T, 4, FT>(stream, a);
+}
+
+// Four tiles of features per wave read x a fourth as often, and leave enough workgroups from half a CU's worth each on
+// (bf16, kernel times: 33 x 6144 -> 12288 28 us against 51 with one tile, 8 x 1536 -> 9216 6.3 against 7.0; but 1 x 6144 ->
+// 1536, 24 workgroups, 14.7 against 6.9).
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
-  const int cols = a.N * Pieces<T>::P;  // N <= 2^20
-  const int chunks = (a.K + kChunk - 1) / kChunk;
-  const dim3 block(64 * (chunks < kMaxWaves ? chunks : kMaxWaves));
-  const unsigned fx = static_cast<unsigned>((a.F + 15) / 16);
-  auto grid = [&](int ct) {
-    const int rows = 16 * ct / Pieces<T>::P;
-    return dim3(fx, static_cast<unsigned>((a.N + rows - 1) / rows));
-  };
-  if (cols <= 16 / Pieces<T>::P * Pieces<T>::P) hipLaunchKernelGGL((q4_kernel<T, 1>), grid(1), block, 0, stream, a);
-  else hipLaunchKernelGGL((q4_kernel<T, 2>), grid(2), block, 0, stream, a);
+  if (a.F >= 64 * (device_cus() / 2)) launch_rows<T, 4>(stream, a);
+  else launch_rows<T, 1>(stream, a);
 }
 
 }  // namespace q4
@@ -224,7 +306,8 @@ extern "C" int hb_proj_q4(hipStream_t stream, const void* x, int dtype, int64_t 
     return st;
   const q4::Args a = {x, x_row_stride, static_cast<const uint8_t*>(w), w_row_stride,
                       static_cast<const uint8_t*>(w_scale), w_scale_row_stride, bias, silu ? 1 : 0, out,
-                      out_row_stride, N, K, F};
+                      out_row_stride, N, K, F,
+                      !misaligned(out, 4 * es) && out_row_stride % 4 == 0 && F % 4 == 0};
   if (dtype == HB_BF16) q4::launch<uint16_t>(stream, a);
   else if (dtype == HB_F16) q4::launch<_Float16>(stream, a);
   else q4::launch<float>(stream, a);

@@ -222,37 +222,67 @@ Q8_DTYPE = torch.float8_e4m3fn
 Q8_MAX_WIDTH = 16384  # values of a row, held in registers
 
 
-def _same_device(dev: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+def _layout(t: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, row stride, row width) of a device tensor of rows, as `_rows` with a quick way out for contiguous ones."""
+    if not t.is_cuda:
+        _require_gpu(t, name)
+    width = t.shape[-1] if t.dim() else 0
+    if width == 0:
+        raise ValueError(f"{name} must have rows of at least one value, got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.numel() // width, width, width
+    return (*_rows(t, name), width)
 
 
-def _vector(t: torch.Tensor | None, channels: int, dtype: torch.dtype, name: str) -> int:
-    """The pointer of a `(C,)` vector of `dtype`, 0 for None."""
+def _batch_rows(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tensor, name: str) -> tuple[int, int]:
+    """`_per_batch` of a tensor on `x`'s device, with a quick way out for None."""
+    if t is None:
+        return 0, 0
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    return _per_batch(t, batch, channels, x.dtype, name)
+
+
+def _channel_vector(t: torch.Tensor | None, channels: int, x: torch.Tensor, name: str) -> int:
+    """The pointer of a `(C,)` vector of `x`'s dtype and device, 0 for None."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.numel() != channels or t.stride(-1) != 1:
-        raise ValueError(f"{name} must be ({channels},) of {dtype} with unit stride")
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    if t.dtype != x.dtype or t.numel() != channels or t.stride(-1) != 1:
+        raise ValueError(f"{name} must be ({channels},) of {x.dtype} with unit stride")
     return t.data_ptr()
 
 
-def _q8_out(shape: tuple, device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty(shape, dtype=Q8_DTYPE, device=device),
-            torch.empty(shape[:-1], dtype=torch.float32, device=device))
+def _f32_channels(t: torch.Tensor, channels: int, device: torch.device, name: str) -> torch.Tensor:
+    """`t` as `channels` fp32 values on `device`, where it must live (converted where it is not fp32)."""
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    t = _f32_vector(t, device)
+    if t.numel() != channels:
+        raise ValueError(f"{name} must have {channels} elements")
+    return t
+
+
+def _q8_out(like: torch.Tensor, width: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """Contiguous 8-bit rows of `width` values and their scales, for the rows of `like`."""
+    rows = like.shape[:-1]
+    if width == like.shape[-1] and like.is_contiguous():
+        q = torch.empty_like(like, dtype=Q8_DTYPE)
+    else:
+        q = torch.empty((*rows, width), dtype=Q8_DTYPE, device=like.device)
+    return q, torch.empty(rows, dtype=torch.float32, device=like.device)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """`x` `(..., C)` as 8-bit rows: `(q, s)`, q `(..., C)` e4m3 and s `(...)` fp32 with `s = max(max|x| / 448, 2^-100)`
     and `q = e4m3(x / s)`, in one pass (`hb_quant_rows`). A row with a NaN or an infinity stands for NaNs. C a multiple
     of 8 (fp32: 4), at most `Q8_MAX_WIDTH`."""
-    _require_gpu(x, "x")
-    rows, stride = _rows(x, "x")
-    q, s = _q8_out(x.shape, x.device)
-    channels = x.shape[-1]
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().hb_quant_rows(_lib.current_stream(x.device), x.data_ptr(), dtype_code(x.dtype), stride,
-                                             q.data_ptr(), channels, s.data_ptr(), rows, channels), "quantize_rows")
+    rows, stride, channels = _layout(x, "x")
+    code = dtype_code(x.dtype)
+    q, s = _q8_out(x, channels)
+    _lib.launch(_lib.load().hb_quant_rows, "quantize_rows", x.device, x.data_ptr(), code, stride, q.data_ptr(), channels,
+                s.data_ptr(), rows, channels)
     return q, s
 
 
@@ -260,26 +290,21 @@ def rms_modulate_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: to
                     shift: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """`rms_modulate(x, weight, eps, scale, shift)` on `(B, L, C)` in fp32 throughout, as 8-bit rows `(q, s)` (see
     `quantize_rows`), in one pass (`hb_rms_modulate_q8`)."""
-    _require_gpu(x, "x")
+    rows, stride, channels = _layout(x, "x")
     if x.dim() != 3:
         raise ValueError(f"x must be (B, L, C), got {tuple(x.shape)}")
-    _same_device(x.device, weight=weight, scale=scale, shift=shift)
-    batch, length, channels = x.shape
-    rows, stride = _rows(x, "x")
-    w = _f32_vector(weight, x.device)
-    if w.numel() != channels:
-        raise ValueError(f"weight must have {channels} elements")
+    code = dtype_code(x.dtype)
+    batch, length, _ = x.shape
+    w = _f32_channels(weight, channels, x.device, "weight")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift are given together or not at all")
-    sp, ms = _per_batch(scale, batch, channels, x.dtype, "scale")
-    hp, ms2 = _per_batch(shift, batch, channels, x.dtype, "shift")
+    sp, ms = _batch_rows(scale, batch, channels, x, "scale")
+    hp, ms2 = _batch_rows(shift, batch, channels, x, "shift")
     if ms != ms2:
         raise ValueError("scale and shift must share their batch stride")
-    q, s = _q8_out(x.shape, x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().hb_rms_modulate_q8(_lib.current_stream(x.device), x.data_ptr(), dtype_code(x.dtype),
-                                                  stride, w.data_ptr(), float(eps), sp, hp, ms, length, q.data_ptr(),
-                                                  channels, s.data_ptr(), rows, channels), "rms_modulate_q8")
+    q, s = _q8_out(x, channels)
+    _lib.launch(_lib.load().hb_rms_modulate_q8, "rms_modulate_q8", x.device, x.data_ptr(), code, stride, w.data_ptr(), float(eps),
+                sp, hp, ms, length, q.data_ptr(), channels, s.data_ptr(), rows, channels)
     return q, s
 
 
@@ -290,31 +315,27 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
     """`residual_rms(h, x, weight, eps, gate, x_bias, local, memory, scale, shift)` with the norm as 8-bit rows, in one
     pass (`hb_residual_rms_q8`): `(h', q, s)`, h' in `h.dtype`, `(q, s)` as `quantize_rows` gives them. Both are
     rounded once, from fp32: the norm reads h' before its rounding."""
-    _require_gpu(h, "h")
-    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype:
-        raise ValueError(f"h and x must be (B, L, C) of one shape and dtype, got {tuple(h.shape)}, {tuple(x.shape)}")
-    _same_device(h.device, x=x, weight=weight, gate=gate, x_bias=x_bias, local=local, scale=scale, shift=shift)
-    batch, length, channels = h.shape
-    _, hs = _rows(h, "h")
-    rows, xs = _rows(x, "x")
-    gp, gs = _per_batch(gate, batch, channels, h.dtype, "gate")
+    rows, hs, channels = _layout(h, "h")
+    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
+        raise ValueError(f"h and x must be (B, L, C) of one shape, dtype and device, got {tuple(h.shape)} {h.dtype} "
+                         f"{h.device}, {tuple(x.shape)} {x.dtype} {x.device}")
+    _, xs, _ = _layout(x, "x")
+    code = dtype_code(h.dtype)
+    batch, length, _ = h.shape
+    gp, gs = _batch_rows(gate, batch, channels, h, "gate")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift are given together or not at all")
-    sp, ms = _per_batch(scale, batch, channels, h.dtype, "scale")
-    hp, ms2 = _per_batch(shift, batch, channels, h.dtype, "shift")
+    sp, ms = _batch_rows(scale, batch, channels, h, "scale")
+    hp, ms2 = _batch_rows(shift, batch, channels, h, "shift")
     if ms != ms2:
         raise ValueError("scale and shift must share their batch stride")
-    w = _f32_vector(weight, h.device)
-    if w.numel() != channels:
-        raise ValueError(f"weight must have {channels} elements")
-    out_h = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    q, s = _q8_out(h.shape, h.device)
-    with torch.cuda.device(h.device):
-        _lib.check(_lib.load().hb_residual_rms_q8(
-            _lib.current_stream(h.device), h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
-            _vector(x_bias, channels, h.dtype, "x_bias"), gp, gs, _vector(local, channels, h.dtype, "local"),
-            int(memory), w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
-            channels, s.data_ptr(), rows, channels), "residual_rms_q8")
+    w = _f32_channels(weight, channels, h.device, "weight")
+    bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
+    out_h = torch.empty_like(h) if h.is_contiguous() else torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    q, s = _q8_out(h, channels)
+    _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs, bp,
+                gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
+                channels, s.data_ptr(), rows, channels)
     return out_h, q, s
 
 
@@ -322,20 +343,16 @@ def glu_q8(proj: torch.Tensor, bias: torch.Tensor | None = None) -> tuple[torch.
     """`value * silu(gate)` for `[value | gate]` = the two halves of the last axis of `proj (+ bias)`, in fp32, as
     8-bit rows `(q, s)` (see `quantize_rows`), in one pass (`hb_glu_q8`): the DiT's SwiGLU (sa3jax/dit.py:218-221).
     `bias` `(2F,)` is the glu_proj layer's where `proj` is the bare product."""
-    _require_gpu(proj, "proj")
-    _same_device(proj.device, bias=bias)
-    width = proj.shape[-1]
+    rows, stride, width = _layout(proj, "proj")
+    code = dtype_code(proj.dtype)
     if width % 2:
         raise ValueError(f"the glu_proj output width {width} is not even")
     inner = width // 2
-    rows, stride = _rows(proj, "proj")
+    bp = 0
     if bias is not None:
-        bias = _f32_vector(bias, proj.device)
-        if bias.numel() != width:
-            raise ValueError(f"bias must have {width} elements")
-    q, s = _q8_out((*proj.shape[:-1], inner), proj.device)
-    with torch.cuda.device(proj.device):
-        _lib.check(_lib.load().hb_glu_q8(_lib.current_stream(proj.device), proj.data_ptr(), dtype_code(proj.dtype),
-                                         stride, bias.data_ptr() if bias is not None else 0, q.data_ptr(), inner,
-                                         s.data_ptr(), rows, inner), "glu_q8")
+        bias = _f32_channels(bias, width, proj.device, "bias")
+        bp = bias.data_ptr()
+    q, s = _q8_out(proj, inner)
+    _lib.launch(_lib.load().hb_glu_q8, "glu_q8", proj.device, proj.data_ptr(), code, stride, bp, q.data_ptr(), inner,
+                s.data_ptr(), rows, inner)
     return q, s

@@ -19,6 +19,7 @@ from hummingbird_amd import _lib
 from hummingbird_amd._derived import f32_vector
 from hummingbird_amd.band_attention import pack_dyt
 from hummingbird_amd.dense_attention import _f32, _f32_vector, _require_gpu, dtype_code
+from hummingbird_amd.elementwise import _f32_channels, _layout
 
 FUSED_DTYPES = (torch.bfloat16, torch.float16)
 
@@ -217,34 +218,30 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     `(..., K)` e4m3 with `x_scale` `(...)` fp32, `weight` `(F, K)` e4m3 with `weight_scale` `(F,)` fp32 (both as
     `elementwise.quantize_rows` gives them), `bias` `(F,)`; the sum, the scales and the bias in fp32, one rounding to
     `dtype` (bf16, half or fp32). K a multiple of 16; any number of rows and features."""
-    _require_gpu(x, "x")
+    n, xs, k = _layout(x, "x")
     dev = x.device
     if x.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:
         raise TypeError(f"linear_q8 takes float8_e4m3fn rows and weights, got {x.dtype} and {weight.dtype}")
     if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
         raise TypeError(f"the scales must be float32, got {x_scale.dtype} and {weight_scale.dtype}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[-1]:
+    if weight.dim() != 2 or weight.shape[1] != k:
         raise ValueError(f"x must be (..., K) and weight (F, K), got {tuple(x.shape)} and {tuple(weight.shape)}")
-    f, k = weight.shape
-    for name, t in (("x_scale", x_scale), ("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    code = dtype_code(dtype)
+    f, ws, _ = _layout(weight, "weight")
+    if weight.device != dev or x_scale.device != dev or weight_scale.device != dev:
+        raise ValueError(f"weight and the scales must be on {dev}, got {weight.device}, {x_scale.device}, "
+                         f"{weight_scale.device}")
     if x_scale.shape != x.shape[:-1] or not x_scale.is_contiguous():
         raise ValueError(f"x_scale must be contiguous {tuple(x.shape[:-1])}, got {tuple(x_scale.shape)}")
     if weight_scale.shape != (f,) or not weight_scale.is_contiguous():
         raise ValueError(f"weight_scale must be contiguous ({f},), got {tuple(weight_scale.shape)}")
-    n, xs = _rows(x, "x")
-    _, ws = _rows(weight, "weight")
+    bp = 0
     if bias is not None:
-        bias = _f32_vector(bias, dev)
-        if bias.numel() != f:
-            raise ValueError(f"bias must have {f} elements")
+        bias = _f32_channels(bias, f, dev, "bias")
+        bp = bias.data_ptr()
     out = torch.empty((*x.shape[:-1], f), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().hb_proj_q8(_lib.current_stream(dev), x.data_ptr(), xs, x_scale.data_ptr(),
-                                          weight.data_ptr(), ws, weight_scale.data_ptr(),
-                                          bias.data_ptr() if bias is not None else 0, out.data_ptr(),
-                                          dtype_code(dtype), f, n, k, f), "linear_q8")
+    _lib.launch(_lib.load().hb_proj_q8, "linear_q8", dev, x.data_ptr(), xs, x_scale.data_ptr(), weight.data_ptr(), ws,
+                weight_scale.data_ptr(), bp, out.data_ptr(), code, f, n, k, f)
     return out
 
 
@@ -282,32 +279,27 @@ def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     """`act(x @ W^T (+ bias))` for few rows `x` `(..., K)` and 4-bit weights (`hb_proj_q4`): `weight` `(F, K / 2)` and
     `weight_scale` `(F, K / 32)`, both uint8, as `quantize_q4` gives them; `bias` `(F,)`; act = SiLU with `silu`. x
     keeps all of its bits (bf16, half or fp32), the sum, bias and activation are fp32, rounded once to `x.dtype`. It
-    reads the weights once per 64 rows of bf16 (half: 32, fp32: 20), and serves the layers that see one row per batch
-    entry."""
-    _require_gpu(x, "x")
+    serves the layers that see one row per batch entry; any number of rows is taken."""
+    n, xs, k = _layout(x, "x")
     dev = x.device
     code = dtype_code(x.dtype)
     if weight.dtype != torch.uint8 or weight_scale.dtype != torch.uint8:
         raise TypeError(f"linear_q4 takes uint8 codes and scales, got {weight.dtype} and {weight_scale.dtype}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != 2 * weight.shape[1]:
-        raise ValueError(f"x must be (..., K) and weight (F, K / 2), got {tuple(x.shape)} and {tuple(weight.shape)}")
-    k, f = x.shape[-1], weight.shape[0]
-    if k % Q4_GROUP or weight_scale.shape != (f, k // Q4_GROUP):
-        raise ValueError(f"K must be a multiple of {Q4_GROUP} and weight_scale (F, K / {Q4_GROUP}), got K = {k} and "
+    if weight.dim() != 2 or k != 2 * weight.shape[1] or k % Q4_GROUP:
+        raise ValueError(f"x must be (..., K) and weight (F, K / 2), K a multiple of {Q4_GROUP}, got {tuple(x.shape)} "
+                         f"and {tuple(weight.shape)}")
+    if weight.device != dev or weight_scale.device != dev:
+        raise ValueError(f"weight and weight_scale must be on {dev}, got {weight.device} and {weight_scale.device}")
+    f, ws, _ = _layout(weight, "weight")
+    if weight_scale.shape != (f, k // Q4_GROUP):
+        raise ValueError(f"weight_scale must be (F, K / {Q4_GROUP}) = ({f}, {k // Q4_GROUP}), got "
                          f"{tuple(weight_scale.shape)}")
-    for name, t in (("weight", weight), ("weight_scale", weight_scale), ("bias", bias)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on {dev}, got {t.device}")
-    n, xs = _rows(x, "x")
-    _, ws = _rows(weight, "weight")
-    _, ss = _rows(weight_scale, "weight_scale")
+    _, ss, _ = _layout(weight_scale, "weight_scale")
+    bp = 0
     if bias is not None:
-        bias = _f32_vector(bias, dev)
-        if bias.numel() != f:
-            raise ValueError(f"bias must have {f} elements")
+        bias = _f32_channels(bias, f, dev, "bias")
+        bp = bias.data_ptr()
     out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().hb_proj_q4(_lib.current_stream(dev), x.data_ptr(), code, xs, weight.data_ptr(), ws,
-                                          weight_scale.data_ptr(), ss, bias.data_ptr() if bias is not None else 0,
-                                          int(bool(silu)), out.data_ptr(), f, n, k, f), "linear_q4")
+    _lib.launch(_lib.load().hb_proj_q4, "linear_q4", dev, x.data_ptr(), code, xs, weight.data_ptr(), ws,
+                weight_scale.data_ptr(), ss, bp, int(bool(silu)), out.data_ptr(), f, n, k, f)
     return out
