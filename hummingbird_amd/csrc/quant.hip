@@ -76,38 +76,50 @@ __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float
 constexpr int kMaxWaves = 16;
 constexpr float kScaleFloor = 0x1p-100f;
 
-// Reductions over a row's workgroup: of each wave by lane exchange, then over the waves in their order through `buf`
-// (a slot per wave). Every lane gets the result. `buf` must be free of reads on entry.
-__device__ __forceinline__ float row_sum(float v, float* buf) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
-  const int waves = blockDim.x >> 6;
-  if (waves == 1) return v;
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int i = 0; i < waves; ++i) v += buf[i];
-  return v;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
 }
-__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* buf) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    const uint32_t o = __shfl_xor(v, off, kWave);
-    v = v > o ? v : o;
-  }
-  const int waves = blockDim.x >> 6;
-  if (waves == 1) return v;
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < waves; ++i) v = v > buf[i] ? v : buf[i];
-  return v;
+// `op` over a wave's 64 lanes, in one order, the result in every lane: pairs, quads, halves of 16 and rows of 16 by DPP,
+// then the rows by lane swaps (against LDS permutations: residual_rms_q8 on 5168 x 1536 bf16 15.6 -> 14.6 us).
+template <typename F>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, const F& op) {
+  v = op(v, dpp<0xb1>(v));   // quad_perm 1, 0, 3, 2
+  v = op(v, dpp<0x4e>(v));   // quad_perm 2, 3, 0, 1
+  v = op(v, dpp<0x141>(v));  // row_half_mirror
+  v = op(v, dpp<0x140>(v));  // row_mirror
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = op(a[0], a[1]);
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(b[0], b[1]);
 }
 
-// The row's scale and its values in 8 bits; y holds zeros past the row. Magnitudes are compared as their bits: a NaN's
-// are above every number's, so it reaches the scale.
+// `op` over a row: of its wave, or (waves > 1) of the workgroup's waves in their order through `buf`, a slot per wave and
+// free of reads on entry.
+template <typename F>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t v, int waves, uint32_t* buf, const F& op) {
+  v = wave_reduce(v, op);
+  if (waves == 1) return v;
+  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = buf[0];
+  for (int i = 1; i < waves; ++i) v = op(v, buf[i]);
+  return v;
+}
+__device__ __forceinline__ float row_sum(float v, int waves, uint32_t* buf) {
+  return __uint_as_float(row_reduce(__float_as_uint(v), waves, buf, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ uint32_t row_max(uint32_t v, int waves, uint32_t* buf) {
+  return row_reduce(v, waves, buf, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+// The row's scale and its values in 8 bits; y holds zeros past the row, `lane` of the row's `lanes`. Magnitudes are
+// compared as their bits: a NaN's are above every number's, so it reaches the scale.
 template <int V, int CH>
-__device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, float* s, int C, uint32_t* buf) {
+__device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, float* s, int C, int lane, int lanes,
+                                         uint32_t* buf) {
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < CH; ++k)
@@ -116,13 +128,13 @@ __device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, fl
       const uint32_t b = __float_as_uint(y[k][j]) & 0x7fffffffu;
       m = m > b ? m : b;
     }
-  const float amax = __uint_as_float(row_max(m, buf));
+  const float amax = __uint_as_float(row_max(m, lanes / 64, buf));
   float sc = __fdiv_rn(amax, 448.f);
   if (sc < kScaleFloor) sc = kScaleFloor;  // not for a NaN
   const float inv = __fdiv_rn(1.f, sc);
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    const int c0 = (k * blockDim.x + threadIdx.x) * V;
+    const int c0 = (k * lanes + lane) * V;
     if (c0 < C) {
       uint32_t w[V / 4];
 #pragma unroll
@@ -132,7 +144,7 @@ __device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, fl
       else *reinterpret_cast<uint32_t*>(q + c0) = w[0];
     }
   }
-  if (threadIdx.x == 0) *s = sc;
+  if (lane == 0) *s = sc;
 }
 
 enum Kind { kQuant = 0, kNorm = 1, kResidualNorm = 2, kGlu = 3 };
@@ -165,20 +177,20 @@ struct Args {
 };
 
 // A row per workgroup, held in registers: CH chunks of V values per lane, chunk k of lane t at column
-// (k * lanes + t) * V.
+// (k * lanes + t) * V. What bounds it is memory: residual_rms_q8 on 5168 x 1536 bf16 (55.6 MB) takes 13.7 us, 2.3 of them
+// a launch's own, glu_q8 on 5168 x 6144 bf16 (159 MB) 31.9 us, the rate of a large copy (5.1 TB/s).
 template <typename T, int KIND, int CH>
 __global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
   constexpr int V = Vec<T>::N;
-  __shared__ float sum_buf[kMaxWaves];
-  __shared__ uint32_t max_buf[kMaxWaves];
-  const int C = a.C;
+  __shared__ uint32_t sum_buf[kMaxWaves], max_buf[kMaxWaves];
+  const int C = a.C, lane = threadIdx.x, lanes = blockDim.x;
   const int64_t n = blockIdx.x;
-  const int64_t b = n / a.L;
+  const int64_t b = static_cast<uint32_t>(n) / static_cast<uint32_t>(a.L);  // N < 2^31
   const bool add_local = KIND == kResidualNorm && a.local && n - b * a.L >= a.memory;
   float y[CH][V];
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
-    const int c0 = (k * blockDim.x + threadIdx.x) * V;
+    const int c0 = (k * lanes + lane) * V;
 #pragma unroll
     for (int j = 0; j < V; ++j) y[k][j] = 0.f;
     if (c0 < C) {
@@ -227,10 +239,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
     for (int k = 0; k < CH; ++k)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss = __fmaf_rn(y[k][j], y[k][j], ss);
-    const float inv = rsqrtf(row_sum(ss, sum_buf) / static_cast<float>(C) + a.eps);
+    const float inv = rsqrtf(row_sum(ss, lanes / 64, sum_buf) / static_cast<float>(C) + a.eps);
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int c0 = (k * blockDim.x + threadIdx.x) * V;
+      const int c0 = (k * lanes + lane) * V;
       if (c0 < C) {
         float w[V];
         load_f32(a.w + c0, w);
@@ -246,20 +258,31 @@ __global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
       }
     }
   }
-  store_q8<V, CH>(y, a.q + n * a.qs, a.s + n, C, max_buf);
+  store_q8<V, CH>(y, a.q + n * a.qs, a.s + n, C, lane, lanes, max_buf);
 }
 
 // The longest row: 16 waves of 64 lanes of CH chunks.
 constexpr int kMaxC = 16384;
 
+template <typename T, int KIND, int CH>
+void launch_ch(hipStream_t stream, const Args<T>& a) {
+  const int lanes = (a.C / Vec<T>::N + CH - 1) / CH;
+  hipLaunchKernelGGL((row_kernel<T, KIND, CH>), dim3(static_cast<unsigned>(a.N)), dim3((lanes + 63) / 64 * 64), 0, stream,
+                     a);
+}
+
+// One chunk per lane is quickest while the card holds all waves at once (residual_rms_q8, bf16: 1292 x 1536 6.1 us against
+// 7.6 with three), and for the GLU, whose lanes have two loads each anyway (5168 x 6144: 31.9 against 34.5); beyond that
+// three (5168 x 1536: 13.7 against 14.6, 1000 x 8192: 14.6 against 16.4, fp32 rms_modulate_q8 on 8249 x 1024: 12.2 against
+// 13.8). Wider rows take what holds them.
 template <typename T, int KIND>
 void launch(hipStream_t stream, const Args<T>& a) {
   const int chunks = a.C / Vec<T>::N;
-  auto lanes = [&](int ch) { return dim3(static_cast<unsigned>(((chunks + ch - 1) / ch + 63) / 64 * 64)); };
-  const dim3 grid(static_cast<unsigned>(a.N));
-  if (chunks <= 1024) hipLaunchKernelGGL((row_kernel<T, KIND, 1>), grid, lanes(1), 0, stream, a);
-  else if (chunks <= 2048) hipLaunchKernelGGL((row_kernel<T, KIND, 2>), grid, lanes(2), 0, stream, a);
-  else hipLaunchKernelGGL((row_kernel<T, KIND, 4>), grid, lanes(4), 0, stream, a);
+  const int64_t waves = a.N * ((chunks + 63) / 64);
+  const bool many = KIND != kGlu && chunks > 64 && waves > 32 * static_cast<int64_t>(device_cus());
+  if (chunks > 3 * 64 * kMaxWaves) launch_ch<T, KIND, 4>(stream, a);
+  else if (many || chunks > 64 * kMaxWaves) launch_ch<T, KIND, 3>(stream, a);
+  else launch_ch<T, KIND, 1>(stream, a);
 }
 
 }  // namespace quant
