@@ -182,6 +182,74 @@ def local_constants(blocks: list, compute: torch.dtype) -> torch.Tensor:
                                b["to_local_embed"]["out"]["bias"]) for b in blocks])
 
 
+_Q8_LAYERS = (("self_attn", "to_qkv"), ("self_attn", "to_out"), ("cross_attn", "to_q"), ("cross_attn", "to_out"),
+              ("ff", "glu_proj"), ("ff", "proj_out"))
+
+
+def quantize_params(params: dict) -> dict:
+    """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
+    rows (`elementwise.quantize_rows`, a scale per output feature) and the timestep and global conditioning layers as
+    4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q8"` and `"q4"` of each layer. The other
+    tensors are shared, not copied. Done once per model, on the weights' device; `prepare_static` then takes the result
+    as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
+    def sequence(seq):
+        return {k: {**layer, "q4": (*projection.quantize_q4(layer["weight"]),
+                                    None if layer.get("bias") is None else layer["bias"].float())}
+                for k, layer in seq.items()}
+
+    def block(b):
+        out = dict(b)
+        for part, layer in _Q8_LAYERS:
+            out[part] = {**out[part], layer: {**b[part][layer], "q8": ew.quantize_rows(b[part][layer]["weight"])}}
+        return out
+    net = params["transformer"]
+    return {**params, "to_timestep_embed": sequence(params["to_timestep_embed"]),
+            "transformer": {**net, "global_cond_embedder": sequence(net["global_cond_embedder"]),
+                            "blocks": [block(b) for b in net["blocks"]]}}
+
+
+def _sequential_q4(seq: dict, x: torch.Tensor) -> torch.Tensor:
+    """`sequential` on 4-bit weights, the activation in the first product's epilogue."""
+    return projection.linear_q4(projection.linear_q4(x, *seq["in"]["q4"], silu=True), *seq["out"]["q4"])
+
+
+def _blocks_q8(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tensor, cfg: DiTConfig) -> torch.Tensor:
+    """`_blocks_fused` on 8-bit rows and weights: each norm, GLU and attention output leaves as the 8-bit rows that the
+    next projection multiplies. `adaln` is `(depth, B, 6 E)`."""
+    eps, E, dt = cfg.norm_eps, h.shape[-1], h.dtype
+    depth = len(blocks)
+
+    def chunks(i):
+        return adaln[i].reshape(adaln.shape[1], 6, E).unbind(1)  # (B, E) views: scale, shift, gate x 2
+
+    def product(rows, layer):
+        return projection.linear_q8(*rows, *layer["q8"], dtype=dt)
+    s_self, sh_self, g_self, s_ff, sh_ff, g_ff = chunks(0)
+    rows = ew.rms_modulate_q8(h, blocks[0]["pre_norm"]["weight"], eps, s_self, sh_self)
+    for i, block in enumerate(blocks):
+        s_self, sh_self, g_self, s_ff, sh_ff, g_ff = chunks(i)
+        attn, cross, ff = block["self_attn"], block["cross_attn"], block["ff"]
+        a = dense_attention.dense_attention(product(rows, attn["to_qkv"]), attn["q_norm"]["weight"],
+                                            attn["k_norm"]["weight"], static["hip_cos"], static["hip_sin"],
+                                            static["hip_mask"], cfg.num_heads, cfg.head_dim, cfg.rope_dim // 2,
+                                            cfg.qk_norm_eps, workspace=static.get("hip_workspace"))
+        h, *rows = ew.residual_rms_q8(h, product(ew.quantize_rows(a), attn["to_out"]),
+                                      block["cross_attend_norm"]["weight"], eps, gate=g_self)
+        c = xattn.cross_attention(product(rows, cross["to_q"]), static["cross"][i], cross["q_norm"]["weight"],
+                                  cfg.qk_norm_eps)
+        h, *rows = ew.residual_rms_q8(h, product(ew.quantize_rows(c), cross["to_out"]), block["ff_norm"]["weight"], eps,
+                                      local=static["local"][i], memory=cfg.num_memory_tokens, scale=s_ff, shift=sh_ff)
+        f = product(ew.glu_q8(product(rows, ff["glu_proj"]), ff["glu_proj"]["bias"]), ff["proj_out"])
+        bias = ff["proj_out"]["bias"].to(dt)
+        if i + 1 < depth:
+            ns, nsh = chunks(i + 1)[:2]
+            h, *rows = ew.residual_rms_q8(h, f, blocks[i + 1]["pre_norm"]["weight"], eps, gate=g_ff, x_bias=bias,
+                                          scale=ns, shift=nsh)
+        else:
+            h = ew.gated_residual(h, f, gate=g_ff, x_bias=bias)
+    return h
+
+
 def block_forward(h: torch.Tensor, block: dict, static: dict, gcond: torch.Tensor, index: int, cfg: DiTConfig,
                   projections: str = "torch", adaln: torch.Tensor | None = None) -> torch.Tensor:
     """One transformer block with adaLN (sa3jax/dit.py:224-251): `h + attn(rms(h) (1 + scale) + shift) *
@@ -315,21 +383,32 @@ def dit_forward(params: dict, x: torch.Tensor, t: torch.Tensor, static: dict, cf
                 projections: str = "torch") -> torch.Tensor:
     """One denoiser evaluation (sa3jax/dit.py:340-361): `(B, io_channels, T)` latents and `(B,)` timesteps -> the
     velocity, same shape, in the compute dtype. `static` comes from `prepare_static`. `projections` is passed to
-    `self_attention`."""
+    `self_attention`, or "q8": the blocks' projections on 8-bit rows and weights and the conditioning layers on 4-bit
+    weights, with `params` (of `static` too) from `quantize_params`; `attention="hip"` only."""
     net = params["transformer"]
     compute = dtype.compute
+    q8 = projections == "q8"
+    if q8 and "q4" not in net["global_cond_embedder"]["in"]:
+        raise ValueError('projections="q8" needs the params of quantize_params')
     h = x.to(compute)
     h = conv1x1(h, params["preprocess_conv"]["weight"]) + h
     h = linear(h.transpose(1, 2), net["project_in"]["weight"])
     memory = net["memory_tokens"].to(compute).expand(h.shape[0], cfg.num_memory_tokens, cfg.embed_dim)
     h = torch.cat([memory, h], dim=1)
 
-    timestep = sequential(params["to_timestep_embed"], expo_fourier(t.to(compute), cfg.fourier_dim))
-    gcond = sequential(net["global_cond_embedder"], static["gcond_proj"] + timestep)
+    if q8 and not use_hip(cfg, h):
+        raise ValueError('projections="q8" needs attention="hip" and the differential model')
+    embed = _sequential_q4 if q8 else sequential
+    timestep = embed(params["to_timestep_embed"], expo_fourier(t.to(compute), cfg.fourier_dim))
+    gcond = embed(net["global_cond_embedder"], static["gcond_proj"] + timestep)
 
     adaln = static["adaln"][:, None, :] + gcond[None] if "adaln" in static else None  # every block's, one launch
     blocks = static.get("blocks", net["blocks"])
-    if adaln is not None and blocks and use_hip(cfg, h) and ew.residual_rms_supported(h.dtype, cfg.embed_dim):
+    if q8:
+        if not blocks or "q8" not in blocks[0]["ff"]["proj_out"]:
+            raise ValueError('projections="q8" needs prepare_static to be given the params of quantize_params')
+        h = _blocks_q8(h, blocks, static, adaln, cfg)
+    elif adaln is not None and blocks and use_hip(cfg, h) and ew.residual_rms_supported(h.dtype, cfg.embed_dim):
         h = _blocks_fused(h, blocks, static, adaln, cfg, projections)
     else:
         for index, block in enumerate(blocks):
