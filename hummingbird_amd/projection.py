@@ -19,7 +19,7 @@ from hummingbird_amd import _lib
 from hummingbird_amd._derived import f32_vector
 from hummingbird_amd.band_attention import pack_dyt
 from hummingbird_amd.dense_attention import _f32, _f32_vector, _require_gpu, dtype_code
-from hummingbird_amd.elementwise import _f32_channels, _layout
+from hummingbird_amd.elementwise import _f32_channels, _layout, _new
 
 FUSED_DTYPES = (torch.bfloat16, torch.float16)
 
@@ -239,7 +239,7 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     if bias is not None:
         bias = _f32_channels(bias, f, dev, "bias")
         bp = bias.data_ptr()
-    out = torch.empty((*x.shape[:-1], f), dtype=dtype, device=dev)
+    out = _new((*x.shape[:-1], f), dtype, dev)
     _lib.launch(_lib.load().hb_proj_q8, "linear_q8", dev, x.data_ptr(), xs, x_scale.data_ptr(), weight.data_ptr(), ws,
                 weight_scale.data_ptr(), bp, out.data_ptr(), code, f, n, k, f)
     return out
@@ -299,7 +299,7 @@ def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     if bias is not None:
         bias = _f32_channels(bias, f, dev, "bias")
         bp = bias.data_ptr()
-    out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
+    out = _new((*x.shape[:-1], f), x.dtype, dev)
     _lib.launch(_lib.load().hb_proj_q4, "linear_q4", dev, x.data_ptr(), code, xs, weight.data_ptr(), ws,
                 weight_scale.data_ptr(), ss, bp, int(bool(silu)), out.data_ptr(), f, n, k, f)
     return out
