@@ -35,7 +35,6 @@ struct Args {
   void* out;  // (N, F), row stride os elements
   int64_t os;
   int N, K, F;
-  bool vec;  // out: rows of a multiple of four features, aligned to four
 };
 
 // Rows of x as bf16 rows whose sum they are: P pieces, each the leading 8 bits of what the earlier ones leave (truncated,
@@ -229,11 +228,11 @@ __global__ __launch_bounds__(64 * max_waves(CT * FT)) void q4_kernel(const Args 
         y[j] = cast_out<T>(z);
       }
       T* o = static_cast<T*>(a.out) + row * a.os + f;
-      if (a.vec) {
-        if (f < a.F) __builtin_memcpy(__builtin_assume_aligned(o, 4 * sizeof(T)), y, sizeof(y));
+      if (f + 4 <= a.F) {
+        __builtin_memcpy(o, y, sizeof(y));  // one store, of any alignment of the elements
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 3; ++j)
           if (f + j < a.F) o[j] = y[j];
       }
     }
@@ -290,6 +289,7 @@ extern "C" int hb_proj_q4(hipStream_t stream, const void* x, int dtype, int64_t 
     return fail(HB_ERR_STRIDE, "%s: w must be 16-byte aligned with a row stride >= K / 2 bytes, a multiple of 16", what);
   if (w_scale_row_stride < K / q4::kGroup)
     return fail(HB_ERR_STRIDE, "%s: w_scale's row stride must be >= K / %d", what, q4::kGroup);
+  if (misaligned(bias, 4)) return fail(HB_ERR_STRIDE, "%s: bias must be 4-byte aligned", what);
   if (misaligned(out, es) || out_row_stride < F)
     return fail(HB_ERR_STRIDE, "%s: out must be aligned to its elements with a row stride >= F", what);
   int st;
@@ -306,8 +306,7 @@ extern "C" int hb_proj_q4(hipStream_t stream, const void* x, int dtype, int64_t 
     return st;
   const q4::Args a = {x, x_row_stride, static_cast<const uint8_t*>(w), w_row_stride,
                       static_cast<const uint8_t*>(w_scale), w_scale_row_stride, bias, silu ? 1 : 0, out,
-                      out_row_stride, N, K, F,
-                      !misaligned(out, 4 * es) && out_row_stride % 4 == 0 && F % 4 == 0};
+                      out_row_stride, N, K, F};
   if (dtype == HB_BF16) q4::launch<uint16_t>(stream, a);
   else if (dtype == HB_F16) q4::launch<_Float16>(stream, a);
   else q4::launch<float>(stream, a);

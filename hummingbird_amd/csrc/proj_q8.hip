@@ -34,7 +34,6 @@ struct Args {
   int64_t os;
   int64_t M;
   int K, F;
-  bool vec;  // out: 16-byte aligned rows of a multiple of eight features
 };
 
 // e4m3 x e4m3 without block scales, fp32 accumulation.
@@ -83,6 +82,11 @@ __device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint3
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(sbase) : "m0");
 }
 
+// As lds_dma16 with an address per lane.
+__device__ __forceinline__ void lds_dma16_any(const void* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "m0");
+}
+
 // Byte of logical 16-byte chunk `chunk` of row `row` in a stage: the reads of a fragment (one chunk of consecutive
 // rows) then spread over the banks.
 __device__ __forceinline__ int swz_byte(int row, int chunk) {
@@ -102,7 +106,10 @@ __device__ __forceinline__ void barrier() {
 
 // The copies of a stage by one wave: blocks wv, wv + NW, ... of the A rows (features), then of the B rows. Lane i's 16
 // bytes land at byte 16 i of a block, row i / 8, position i % 8, so it fetches the chunk that the swizzle puts there.
-template <class TL>
+// RAGGED: K may end inside a stage; chunks from column K on come from `zeros`.
+__device__ __attribute__((aligned(16))) const uint8_t zeros[16] = {};
+
+template <class TL, bool RAGGED>
 struct StageCopy {
   const uint8_t* w0;
   const uint8_t* x0;
@@ -127,30 +134,15 @@ struct StageCopy {
     }
   }
   // Copy u of a stage whose columns start at k, to the stage at LDS byte address `stage`.
-  __device__ __forceinline__ void one(int u, int k, uint32_t stage) const {
-    if (u < TL::kBlocksA) lds_dma16(w0 + k, aoff[u], stage + (wv + TL::NW * u) * 1024);
-    else
-      lds_dma16(x0 + k, boff[u - TL::kBlocksA],
-                stage + TL::FT * kStep + (wv + TL::NW * (u - TL::kBlocksA)) * 1024);
+  __device__ __forceinline__ void one(int u, int k, int K, uint32_t stage) const {
+    const bool a = u < TL::kBlocksA;
+    const uint8_t* base = (a ? w0 : x0) + k;
+    const uint32_t off = a ? aoff[a ? u : 0] : boff[a ? 0 : u - TL::kBlocksA];
+    const uint32_t to = stage + (a ? 0 : TL::FT * kStep) + (wv + TL::NW * (a ? u : u - TL::kBlocksA)) * 1024;
+    if constexpr (RAGGED) lds_dma16_any(k + 16 * chunk < K ? base + off : zeros, to);
+    else lds_dma16(base, off, to);
   }
   static constexpr int kCopies = TL::kBlocksA + TL::kBlocksB;
-  // The last stage where K ends inside it: through registers, zeros from column K on.
-  __device__ __forceinline__ void tail(int k, int K, uint8_t* stage) const {
-    const bool in = k + 16 * chunk < K;
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int u = 0; u < TL::kBlocksA; ++u) {
-      u32x4 v = {0, 0, 0, 0};
-      if (in) v = ld16(w0 + k + aoff[u]);
-      *reinterpret_cast<u32x4*>(stage + (wv + TL::NW * u) * 1024 + 16 * lane) = v;
-    }
-#pragma unroll
-    for (int u = 0; u < TL::kBlocksB; ++u) {
-      u32x4 v = {0, 0, 0, 0};
-      if (in) v = ld16(x0 + k + boff[u]);
-      *reinterpret_cast<u32x4*>(stage + TL::FT * kStep + (wv + TL::NW * u) * 1024 + 16 * lane) = v;
-    }
-  }
 };
 
 // Half a stage (64 columns) of a wave's operands: 32 bytes of each of its rows, lane half lh the chunks 4 kk + 2 lh + 0, 1.
@@ -204,13 +196,29 @@ __device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
   x = r[0], y = r[1];
 }
 
+// 16 bytes of consecutive results from feature f of a row on, those past the last feature left out. Rows of any stride and
+// width: the 16-byte store takes any alignment of its elements.
+template <typename T>
+__device__ __forceinline__ void store16(T* row, int f, int F, u32x4 v) {
+  constexpr int N = 16 / static_cast<int>(sizeof(T));
+  if (f + N <= F) {
+    __builtin_memcpy(row + f, &v, 16);
+  } else if (f < F) {
+#pragma unroll
+    for (int j = 0; j < N - 1; ++j) {
+      if (f + j >= F) continue;
+      if constexpr (sizeof(T) == 4) row[f + j] = __uint_as_float(v[j]);
+      else row[f + j] = __builtin_bit_cast(T, static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1))));
+    }
+  }
+}
+
 // A wave's results. Lane (lr, lh) holds, in registers 4 g .. 4 g + 3 of a 32 x 32 tile, features 8 g + 4 lh .. + 3 of row
 // lr. The results of a tile leave in stores of 16 rows of 64 bytes: for 16-bit types the wave's halves exchange so that
-// a lane holds eight consecutive features, and then its 16-lane rows so that four lanes hold 64 bytes of a row. (Through
-// LDS a tile waits for its own round trip, and one wave per SIMD has nothing else to do: 4.5 us for the 16 tiles of a
-// wave.) GENERAL: any row stride, alignment and number of features, element by element.
-// `sw`, `bias`, `sx`: the scales of this wave's features and rows, in LDS.
-template <typename T, class TL, bool GENERAL>
+// a lane holds eight consecutive features, and then its 16-lane rows so that four lanes hold 64 bytes of a row (through
+// LDS a tile waits for its own round trip: 5168 x 6144 -> 1536 54 against 43 us). `sw`, `bias`, `sx`: the scales of this
+// wave's features and rows, in LDS.
+template <typename T, class TL>
 __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL::NF][TL::NM], int f0, int64_t m0,
                                            const float* sw_, const float* bias_, const float* sx_) {
   const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
@@ -235,16 +243,7 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(acc[n][t][i] * sx[t], sw[i], bias[i]);
-      if constexpr (GENERAL) {
-        const int64_t m = m0 + 32 * t + lr;
-        if (m < a.M) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int f = fn + 8 * (i >> 2) + 4 * lh + (i & 3);
-            if (f < a.F) out[m * a.os + f] = cast_out<T>(v[i]);
-          }
-        }
-      } else if constexpr (sizeof(T) == 4) {
+      if constexpr (sizeof(T) == 4) {
         uint32_t w[4][4];  // [g]: features 8 g + 4 lh .. + 3
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -258,8 +257,7 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
         for (int q = 0; q < 4; ++q) {  // rows 16 (q % 2) .. of the tile
           const int64_t m = m0 + 32 * t + 16 * (q & 1) + (lr & 15);
           const int f = fn + 16 * (q >> 1) + 8 * (lr >> 4) + 4 * lh;
-          if (m < a.M && f < a.F)
-            *reinterpret_cast<u32x4*>(out + m * a.os + f) = u32x4{w[q][0], w[q][1], w[q][2], w[q][3]};
+          if (m < a.M) store16(out + m * a.os, f, a.F, u32x4{w[q][0], w[q][1], w[q][2], w[q][3]});
         }
       } else {
         uint32_t w[4][2];  // [g]: features 8 g + 4 lh .. + 3
@@ -280,9 +278,8 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
         for (int p = 0; p < 2; ++p) {
           const int64_t m = m0 + 32 * t + 16 * p + (lr & 15);
           const int f = fn + 16 * (lr >> 4) + 8 * lh;
-          if (m < a.M && f < a.F)
-            *reinterpret_cast<u32x4*>(out + m * a.os + f) =
-                u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]};
+          if (m < a.M)
+            store16(out + m * a.os, f, a.F, u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]});
         }
       }
     }
@@ -297,8 +294,8 @@ int64_t tiles_of(const Args& a) {
 // Workgroups stay: each takes every gridDim.x-th tile, and its copies run two steps ahead of the products across the
 // tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
 // copy that tile's columns again, for nothing: the loop has no branch around a copy, and the kernel waits for them
-// before it ends. GENERAL: K may end inside the last step, which is then copied through registers; see store_tile.
-template <typename T, class TL, bool GENERAL>
+// before it ends.
+template <typename T, class TL, bool RAGGED>
 __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL::kWaves, TL::kWaves))) void tiled_kernel(
     const Args a) {
   constexpr bool WIDE = std::is_same<T, float>::value;
@@ -318,10 +315,9 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   const int wv = wave_id(), fw = wv % TL::WF * (32 * TL::NF), mw = wv / TL::WF * (32 * TL::NM);
   const uint32_t lds0 = lds_addr(smem);
   const int nk = (a.K + kStep - 1) / kStep;
-  const bool ragged = GENERAL && a.K % kStep != 0;
 
   // What is copied next: step `cs` of tile `ct` (in the order of p).
-  StageCopy<TL> copy;
+  StageCopy<TL, RAGGED> copy;
   int ct = blockIdx.x, cs = 0;
   auto aim = [&]() {
     int f0;
@@ -336,8 +332,7 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     ct += gridDim.x;
     aim();
   };
-  auto slow = [&]() { return ragged && cs == nk - 1; };  // a step for copy.tail
-  constexpr int kTiles = TL::NF * TL::NM, kReads = Frags<TL>::kReads, kCopies = StageCopy<TL>::kCopies;
+  constexpr int kTiles = TL::NF * TL::NM, kReads = Frags<TL>::kReads, kCopies = StageCopy<TL, RAGGED>::kCopies;
   // A tile's scales, 64 of each kind by a wave, copied while its first step runs; tiles alternate between the sets.
   auto copy_scales = [&](int f0, int64_t m0, int set) {
     const uint32_t to = lds_addr(scales[set]) + 256 * wv;
@@ -356,15 +351,11 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   aim();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (slow()) {
-      copy.tail(cs * kStep, a.K, smem + i * TL::kStage);
-    } else {
 #pragma unroll
-      for (int u = 0; u < kCopies; ++u) copy.one(u, cs * kStep, lds0 + i * TL::kStage);
-    }
+    for (int u = 0; u < kCopies; ++u) copy.one(u, cs * kStep, a.K, lds0 + i * TL::kStage);
     advance();
   }
-  wait_copies<GENERAL ? 0 : kCopies>();
+  wait_copies<kCopies>();
   wait_lds();
   barrier();
   Frags<TL> lo, hi;
@@ -390,13 +381,11 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
 #pragma unroll
       for (int j = 0; j < TL::NM; ++j) acc[i][j] = f32x16{};
     for (int s = 0; s < nk; ++s) {
-      const bool by_registers = slow();
       const uint32_t stage = __builtin_amdgcn_readfirstlane(lds0 + b);
       const int k = cs * kStep;
       auto copies = [&](int j) {  // those of product j past the barrier
-        if (GENERAL && by_registers) return;
 #pragma unroll
-        for (int u = j * kCopies / kTiles; u < (j + 1) * kCopies / kTiles; ++u) copy.one(u, k, stage);
+        for (int u = j * kCopies / kTiles; u < (j + 1) * kCopies / kTiles; ++u) copy.one(u, k, a.K, stage);
       };
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
@@ -408,16 +397,14 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
         if (kFree > 0 && i == kFree) {
           wait_lds();
           barrier();
-          if (by_registers) copy.tail(k, a.K, smem + b);
         }
         if (kFree > 0 && i >= kFree) copies(i - kFree);
         acc[i / TL::NM][i % TL::NM] = multiply<WIDE>(lo.a[i / TL::NM], lo.b[i % TL::NM], acc[i / TL::NM][i % TL::NM]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_copies<GENERAL || kFree == 0 ? 0 : kEarly>();
-      if (GENERAL || kFree == 0) wait_lds();
+      wait_copies<kFree == 0 ? 0 : kEarly>();
+      if (kFree == 0) wait_lds();
       barrier();
-      if (kFree == 0 && by_registers) copy.tail(k, a.K, smem + b);
       b = TL::kStage - b;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
@@ -432,7 +419,7 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
       advance();
     }
     const float* sc = scales[set];
-    store_tile<T, TL, GENERAL>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
+    store_tile<T, TL>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
   }
   wait_copies<0>();
 }
@@ -441,7 +428,7 @@ template <typename T, class TL>
 void launch_tiled(hipStream_t stream, const Args& a) {
   const int64_t tiles = tiles_of<TL>(a), slots = static_cast<int64_t>(TL::kWaves) * 4 / TL::NW * device_cus();
   const dim3 grid(static_cast<unsigned>(tiles < slots ? tiles : slots)), block(64 * TL::NW);
-  if (a.K % kStep || !a.vec) hipLaunchKernelGGL((tiled_kernel<T, TL, true>), grid, block, 0, stream, a);
+  if (a.K % kStep) hipLaunchKernelGGL((tiled_kernel<T, TL, true>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((tiled_kernel<T, TL, false>), grid, block, 0, stream, a);
 }
 
@@ -450,7 +437,7 @@ void launch_tiled(hipStream_t stream, const Args& a) {
 // own, take consecutive steps of one tile, and their sums are added in the groups' order through LDS.
 constexpr int kGroups = 4;
 
-template <typename T, class TL, bool GENERAL>
+template <typename T, class TL, bool RAGGED>
 __global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args a) {
   static_assert(TL::NF == 1 && TL::NM == 1, "a 32 x 32 tile per wave");
   constexpr bool WIDE = std::is_same<T, float>::value;
@@ -464,7 +451,6 @@ __global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args
   const int fw = wv % TL::WF * 32, mw = wv / TL::WF * 32;
   const int nk = (a.K + kStep - 1) / kStep, per = (nk + kGroups - 1) / kGroups, first = group * per;
   const int mine = nk - first < per ? nk - first : per;  // steps of this group, possibly none; barriers are for `per`
-  const bool ragged = GENERAL && a.K % kStep != 0;
   uint8_t* const stages = smem + 2 * group * TL::kStage;
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_addr(smem) + 2 * group * TL::kStage);
   if (threadIdx.x < TL::FT) {
@@ -476,25 +462,21 @@ __global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args
     const int64_t m = m0 + threadIdx.x < a.M ? m0 + threadIdx.x : a.M - 1;
     scales[2 * TL::FT + threadIdx.x] = a.sx[m];
   }
-  StageCopy<TL> copy;
+  StageCopy<TL, RAGGED> copy;
   copy.aim(a, f0, m0);
-  constexpr int kReads = Frags<TL>::kReads, kCopies = StageCopy<TL>::kCopies;
+  constexpr int kReads = Frags<TL>::kReads, kCopies = StageCopy<TL, RAGGED>::kCopies;
   auto fill = [&](int s) {  // the group's step s into stage s % 2
     if (s >= mine) return;
     const int k = (first + s) * kStep;
-    if (ragged && first + s == nk - 1) {
-      copy.tail(k, a.K, stages + (s & 1) * TL::kStage);
-    } else {
 #pragma unroll
-      for (int u = 0; u < kCopies; ++u) copy.one(u, k, lds0 + (s & 1) * TL::kStage);
-    }
+    for (int u = 0; u < kCopies; ++u) copy.one(u, k, a.K, lds0 + (s & 1) * TL::kStage);
   };
   fill(0);
   fill(1);
   f32x16 acc[1][1] = {{f32x16{}}};
   for (int s = 0; s < per; ++s) {
     // step s has landed: all copies but those of step s + 1
-    if (!ragged && s + 1 < mine) wait_copies<kCopies>();
+    if (s + 1 < mine) wait_copies<kCopies>();
     else wait_copies<0>();
     wait_lds();
     barrier();
@@ -532,13 +514,13 @@ __global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[0][0][4 * g + j] += v[j];
     }
-  store_tile<T, TL, GENERAL>(a, acc, f0 + fw, m0 + mw, scales + fw, scales + TL::FT + fw, scales + 2 * TL::FT + mw);
+  store_tile<T, TL>(a, acc, f0 + fw, m0 + mw, scales + fw, scales + TL::FT + fw, scales + 2 * TL::FT + mw);
 }
 
 template <typename T, class TL>
 void launch_split(hipStream_t stream, const Args& a) {
   const dim3 grid(static_cast<unsigned>(tiles_of<TL>(a))), block(64 * TL::NW * kGroups);
-  if (a.K % kStep || !a.vec) hipLaunchKernelGGL((split_kernel<T, TL, true>), grid, block, 0, stream, a);
+  if (a.K % kStep) hipLaunchKernelGGL((split_kernel<T, TL, true>), grid, block, 0, stream, a);
   else hipLaunchKernelGGL((split_kernel<T, TL, false>), grid, block, 0, stream, a);
 }
 
@@ -688,6 +670,8 @@ extern "C" int hb_proj_q8(hipStream_t stream, const void* x, int64_t x_row_strid
   if (rows_of)
     return fail(HB_ERR_STRIDE, "%s: %s must be 16-byte aligned with a row stride >= K, a multiple of 16 up to 2^23", what,
                 rows_of);
+  if (misaligned(x_scale, 4) || misaligned(w_scale, 4) || misaligned(bias, 4))
+    return fail(HB_ERR_STRIDE, "%s: x_scale, w_scale and bias must be 4-byte aligned", what);
   if (misaligned(out, es) || out_row_stride < F)
     return fail(HB_ERR_STRIDE, "%s: out must be aligned to its elements with a row stride >= F", what);
   int st;
@@ -702,8 +686,7 @@ extern "C" int hb_proj_q8(hipStream_t stream, const void* x, int64_t x_row_strid
       (st = check_disjoint(what, "out", out, ob, "bias", bias, static_cast<int64_t>(F) * 4)))
     return st;
   const q8::Args a = {static_cast<const uint8_t*>(x), x_row_stride, x_scale, static_cast<const uint8_t*>(w),
-                      w_row_stride, w_scale, bias, out, out_row_stride, M, K, F,
-                      !misaligned(out, 16) && out_row_stride * es % 16 == 0 && F % 8 == 0};
+                      w_row_stride, w_scale, bias, out, out_row_stride, M, K, F};
   if (out_dtype == HB_BF16) q8::launch<uint16_t>(stream, a);
   else if (out_dtype == HB_F16) q8::launch<_Float16>(stream, a);
   else q8::launch<float>(stream, a);

@@ -407,6 +407,7 @@ int hb_rms_modulate_q8(hipStream_t stream, const void* x, int dtype, int64_t x_r
   if (!x || !weight || !q || !q_scale)
     return fail(HB_ERR_NULL, "%s: x, weight, q and q_scale must be non-NULL", what);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(HB_ERR_EPS, "%s: eps %g must be finite and >= 0", what, eps);
+  if (reinterpret_cast<uintptr_t>(weight) % 4) return fail(HB_ERR_STRIDE, "%s: weight must be 4-byte aligned", what);
   if (!scale != !shift) return fail(HB_ERR_NULL, "%s: scale and shift are given together or not at all", what);
   if (scale && N % rows_per_batch) return fail(HB_ERR_SHAPE, "%s: N must be a multiple of rows_per_batch", what);
   const int64_t nb = scale ? N / rows_per_batch : 1, ms = nb > 1 ? mod_batch_stride : C;
@@ -439,6 +440,7 @@ int hb_residual_rms_q8(hipStream_t stream, const void* h, int dtype, int64_t h_r
   if (!h || !x || !weight || !out_h || !q || !q_scale)
     return fail(HB_ERR_NULL, "%s: h, x, weight, out_h, q and q_scale must be non-NULL", what);
   if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(HB_ERR_EPS, "%s: eps %g must be finite and >= 0", what, eps);
+  if (reinterpret_cast<uintptr_t>(weight) % 4) return fail(HB_ERR_STRIDE, "%s: weight must be 4-byte aligned", what);
   if (!scale != !shift) return fail(HB_ERR_NULL, "%s: scale and shift are given together or not at all", what);
   if (memory < 0) return fail(HB_ERR_SHAPE, "%s: memory must be >= 0", what);
   if ((gate || scale) && N % rows_per_batch)
@@ -474,6 +476,7 @@ int hb_glu_q8(hipStream_t stream, const void* proj, int dtype, int64_t proj_row_
   int st = check_rows(what, dtype, N, F, 1);
   if (st) return st;
   if (!proj || !q || !q_scale) return fail(HB_ERR_NULL, "%s: proj, q and q_scale must be non-NULL", what);
+  if (reinterpret_cast<uintptr_t>(bias) % 4) return fail(HB_ERR_STRIDE, "%s: bias must be 4-byte aligned", what);
   const Operand outs[] = {{"q", q, 1, N, q_row_stride, F}, {"q_scale", q_scale, 4, N, 1, 1}};
   const Operand ins[] = {{"proj", proj, esize_of(dtype), N, proj_row_stride, 2 * static_cast<int64_t>(F)}};
   if ((st = check_operands(what, outs, 2, ins, 1, vec_of(dtype)))) return st;

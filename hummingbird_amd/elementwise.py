@@ -227,8 +227,8 @@ def _layout(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     if not t.is_cuda:
         _require_gpu(t, name)
     width = t.shape[-1] if t.dim() else 0
-    if width == 0:
-        raise ValueError(f"{name} must have rows of at least one value, got {tuple(t.shape)}")
+    if not 0 < width < 1 << 31:
+        raise ValueError(f"{name} must have rows of 1 to 2^31 - 1 values, got {tuple(t.shape)}")
     if t.is_contiguous():
         return t.numel() // width, width, width
     return (*_rows(t, name), width)
@@ -288,8 +288,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, stride, channels = _layout(x, "x")
     code = dtype_code(x.dtype)
     q, s = _q8_out(x, channels)
-    _lib.launch(_lib.load().hb_quant_rows, "quantize_rows", x.device, x.data_ptr(), code, stride, q.data_ptr(), channels,
-                s.data_ptr(), rows, channels)
+    _lib.launch(_lib.load().hb_quant_rows, "quantize_rows", x.device, x.data_ptr(), code, stride, q.data_ptr(),
+                channels, s.data_ptr(), rows, channels)
     return q, s
 
 
@@ -310,8 +310,8 @@ def rms_modulate_q8(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: to
     if ms != ms2:
         raise ValueError("scale and shift must share their batch stride")
     q, s = _q8_out(x, channels)
-    _lib.launch(_lib.load().hb_rms_modulate_q8, "rms_modulate_q8", x.device, x.data_ptr(), code, stride, w.data_ptr(), float(eps),
-                sp, hp, ms, length, q.data_ptr(), channels, s.data_ptr(), rows, channels)
+    _lib.launch(_lib.load().hb_rms_modulate_q8, "rms_modulate_q8", x.device, x.data_ptr(), code, stride, w.data_ptr(),
+                float(eps), sp, hp, ms, length, q.data_ptr(), channels, s.data_ptr(), rows, channels)
     return q, s
 
 
@@ -340,8 +340,8 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
     bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
     out_h = _new((batch, length, channels), h.dtype, h.device)
     q, s = _q8_out(h, channels)
-    _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs, bp,
-                gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
+    _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs,
+                bp, gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
                 channels, s.data_ptr(), rows, channels)
     return out_h, q, s
 

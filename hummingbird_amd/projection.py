@@ -252,16 +252,16 @@ _E2M1_MIDDLES = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)  # between the magnitude
 def quantize_q4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """`(F, K)` weights as `(codes (F, K / 2) uint8, scales (F, K / 32) uint8)` for `linear_q4`: e2m1 codes, two per
     byte (the low nibble the even column), and per group of 32 columns the e8m0 scale 2^(s - 127), the least power of
-    two that brings the group's largest magnitude to 6 or below, s kept within [8, 250]. Magnitudes round to the nearest,
-    ties to the even code. Done once per weight, in torch operations on the weight's device. K a multiple of 32; the
-    weights must be finite."""
+    two that brings the group's largest magnitude to 6 or below, with s at least 8. Magnitudes round to the nearest, ties
+    to the even code. Done once per weight, in torch operations on the weight's device. K a multiple of 32; magnitudes
+    must be at most 6 * 2^123 (s = 250)."""
     if weight.dim() != 2 or weight.shape[1] % Q4_GROUP or weight.numel() == 0:
         raise ValueError(f"weight must be (F, K) with K a multiple of {Q4_GROUP}, got {tuple(weight.shape)}")
     f, k = weight.shape
     w = weight.to(torch.float32).reshape(f, k // Q4_GROUP, Q4_GROUP)
     amax = w.abs().amax(dim=-1)
-    if not bool(torch.isfinite(amax).all()):
-        raise ValueError("quantize_q4 needs finite weights")
+    if not bool((amax <= 6 * 2.0 ** 123).all()):
+        raise ValueError("quantize_q4 needs finite weights of magnitudes up to 6 * 2^123")
     mant, exp = torch.frexp(amax)  # amax = mant 2^exp, mant in [0.5, 1): above 6 2^(exp - 3) when mant > 0.75
     e = torch.where(mant > 0.75, exp - 2, exp - 3)
     e = torch.where(amax > 0, e, torch.zeros_like(e)).clamp(8 - 127, 250 - 127)
@@ -279,7 +279,7 @@ def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     """`act(x @ W^T (+ bias))` for few rows `x` `(..., K)` and 4-bit weights (`hb_proj_q4`): `weight` `(F, K / 2)` and
     `weight_scale` `(F, K / 32)`, both uint8, as `quantize_q4` gives them; `bias` `(F,)`; act = SiLU with `silu`. x
     keeps all of its bits (bf16, half or fp32), the sum, bias and activation are fp32, rounded once to `x.dtype`. It
-    serves the layers that see one row per batch entry; any number of rows is taken."""
+    serves the layers that see one row per batch entry; up to 2^16 rows are taken."""
     n, xs, k = _layout(x, "x")
     dev = x.device
     code = dtype_code(x.dtype)

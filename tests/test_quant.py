@@ -70,7 +70,7 @@ def test_row_refusals(lib, call, kw, status):
 
 @pytest.mark.parametrize("kw,status", [
     ({"w": 0}, NULL), ({"eps": -1.0}, EPS), ({"eps": float("nan")}, EPS), ({"scale": 0}, NULL), ({"shift": 0}, NULL),
-    ({"L": 3}, SHAPE), ({"L": 0}, SHAPE), ({"ms": 32}, STRIDE), ({"q": addr(3)}, STRIDE), ({"s": addr(3) + 252}, STRIDE),
+    ({"w": addr(3) + 2}, STRIDE), ({"L": 3}, SHAPE), ({"L": 0}, SHAPE), ({"ms": 32}, STRIDE), ({"q": addr(3)}, STRIDE), ({"s": addr(3) + 252}, STRIDE),
     ({"q": addr(4) + 128}, STRIDE), ({"scale": addr(4) + 2}, STRIDE),
 ])
 @pytest.mark.parametrize("call", [rms_q8, residual_q8])
@@ -91,6 +91,7 @@ def test_glu_refusals(lib):
     assert glu_q8(lib, q=addr(3)) == STRIDE
     assert glu_q8(lib, s=addr(3) + 508) == STRIDE
     assert glu_q8(lib, xs=64) == STRIDE
+    assert glu_q8(lib, bias=addr(3) + 2) == STRIDE
 
 
 def proj_q8(lib, **kw):
@@ -104,6 +105,8 @@ def proj_q8(lib, **kw):
     ({"dtype": 3}, DTYPE), ({"M": 0}, SHAPE), ({"F": 0}, SHAPE), ({"K": 0}, SHAPE), ({"K": 40}, SHAPE),
     ({"M": (1 << 21) + 1}, SHAPE), ({"F": (1 << 21) + 1}, SHAPE), ({"x": 0}, NULL), ({"sx": 0}, NULL), ({"w": 0}, NULL),
     ({"sw": 0}, NULL), ({"out": 0}, NULL), ({"x": addr(0) + 8}, STRIDE), ({"w": addr(2) + 8}, STRIDE),
+    ({"sx": addr(1) + 2}, STRIDE), ({"sw": addr(3) + 2}, STRIDE), ({"bias": addr(4) + 2}, STRIDE),
+    ({"xs": (1 << 23) + 16}, STRIDE), ({"ws": (1 << 23) + 16}, STRIDE), ({"K": (1 << 23) + 16}, SHAPE),
     ({"xs": 48}, STRIDE), ({"ws": 48}, STRIDE), ({"xs": 72}, STRIDE), ({"ws": 72}, STRIDE), ({"os": 23}, STRIDE),
     ({"out": addr(5) + 1}, STRIDE), ({"dtype": F32, "out": addr(5) + 2}, STRIDE), ({"xs": 1 << 61}, STRIDE),
     ({"ws": 1 << 61}, STRIDE), ({"os": 1 << 61}, STRIDE), ({"out": addr(0) + 128}, STRIDE), ({"out": addr(2)}, STRIDE),
@@ -123,7 +126,7 @@ def proj_q4(lib, **kw):
 @pytest.mark.parametrize("kw,status", [
     ({"dtype": 3}, DTYPE), ({"N": 0}, SHAPE), ({"N": (1 << 16) + 1}, SHAPE), ({"F": 0}, SHAPE), ({"K": 0}, SHAPE),
     ({"K": 48}, SHAPE), ({"x": 0}, NULL), ({"w": 0}, NULL), ({"sc": 0}, NULL), ({"out": 0}, NULL),
-    ({"x": addr(0) + 8}, STRIDE), ({"xs": 56}, STRIDE), ({"xs": 68}, STRIDE), ({"w": addr(1) + 8}, STRIDE),
+    ({"bias": addr(3) + 2}, STRIDE), ({"x": addr(0) + 8}, STRIDE), ({"xs": 56}, STRIDE), ({"xs": 68}, STRIDE), ({"w": addr(1) + 8}, STRIDE),
     ({"ws": 16}, STRIDE), ({"ws": 40}, STRIDE), ({"ss": 1}, STRIDE), ({"os": 23}, STRIDE), ({"out": addr(4) + 1}, STRIDE),
     ({"dtype": F32, "out": addr(4) + 2}, STRIDE), ({"xs": 1 << 61}, STRIDE), ({"ws": 1 << 61}, STRIDE),
     ({"ss": 1 << 61}, STRIDE), ({"os": 1 << 61}, STRIDE), ({"out": addr(0) + 128}, STRIDE), ({"out": addr(1)}, STRIDE),
@@ -190,6 +193,6 @@ def test_quantize_q4_is_the_nearest_code(case):
 
 def test_quantize_q4_refusals():
     for bad in (torch.zeros(4, 40), torch.zeros(32), torch.zeros(0, 32), torch.full((1, 32), float("inf")),
-                torch.full((1, 32), float("nan"))):
+                torch.full((1, 32), float("nan")), torch.full((1, 32), 1e38)):
         with pytest.raises(ValueError):
             projection.quantize_q4(bad)

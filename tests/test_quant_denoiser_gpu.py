@@ -5,7 +5,7 @@
   codes, by one step. A border is within 1e-6 of a fraction 1e-6 / 2^-4 of the values, and a step is at most 2^-3 of the
   value, so a quantised tensor differs by about sqrt(1.6e-5) 2^-3 = 5e-4 of its norm; 12 of them follow each other in two
   blocks: 1e-2 is allowed.
-* Against the unquantised denoiser, bf16: a rounding to e4m3 is off by at most 2^-4, 2^-4 / sqrt(3) = 3.6 % on average,
+* Against the unquantised denoiser, bf16 and half: a rounding to e4m3 is off by at most 2^-4, 2^-4 / sqrt(3) = 3.6 % on average,
   on both operands of a product, 5 % of its result, and a branch holds up to three products in a row, 9 %. The branches'
   errors are independent and smaller than the residual stream they are added to: 25 % of the output's norm is allowed,
   and the error must not vanish.
@@ -20,7 +20,7 @@ import torch
 
 from hummingbird_amd import dit, elementwise, projection, sampling
 from hummingbird_amd.config import MEDIUM_DIT
-from hummingbird_amd.dtypes import BF16, FP32_PARITY
+from hummingbird_amd.dtypes import BF16, FP16, FP32_PARITY
 from tests.test_sampler import TINY
 from tests.test_sampler_gpu import MEDIUM2, case
 
@@ -98,14 +98,16 @@ def test_dit_forward_q8_vs_plain_operations(monkeypatch, batch, tokens):
     assert rel(got, ref) <= 1e-2, rel(got, ref)
 
 
-def test_dit_forward_q8_is_near_the_unquantised_one():
-    announce("dit_forward medium q8 vs bf16")
-    params, cond, mask, x = case(MEDIUM2, BF16, 2, 300, seed=24, ctx_tokens=257)
+@pytest.mark.parametrize("preset", ["bf16", "fp16"])
+def test_dit_forward_q8_is_near_the_unquantised_one(preset):
+    announce(f"dit_forward medium q8 vs {preset}")
+    dtype = {"bf16": BF16, "fp16": FP16}[preset]
+    params, cond, mask, x = case(MEDIUM2, dtype, 2, 300, seed=24, ctx_tokens=257)
     params = dit.quantize_params(params)
-    static = dit.prepare_static(params, cond, mask, MEDIUM2, BF16)
+    static = dit.prepare_static(params, cond, mask, MEDIUM2, dtype)
     t = torch.tensor([0.9, 0.35], device=DEV)
-    got = dit.dit_forward(params, x, t, static, MEDIUM2, BF16, projections="q8")
-    ref = dit.dit_forward(params, x, t, static, MEDIUM2, BF16)
+    got = dit.dit_forward(params, x, t, static, MEDIUM2, dtype, projections="q8")
+    ref = dit.dit_forward(params, x, t, static, MEDIUM2, dtype)
     off = rel(got, ref)
     print(f"off by {off:.3f} of the output's norm")
     assert 1e-4 < off <= 0.25

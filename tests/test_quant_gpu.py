@@ -206,7 +206,9 @@ def q8_rows(gen, n, k, spread=1.0):
 
 # rows, columns, features: one of each, few rows, tiles' edges on both sides, a short and a long reduction, odd sizes
 Q8_SHAPES = [(1, 16, 1), (1, 1536, 7680), (7, 1536, 512), (16, 64, 100), (17, 80, 33), (33, 256, 257), (64, 6144, 96),
-             (65, 144, 64), (128, 128, 128), (129, 1536, 255), (257, 1040, 513), (300, 6144, 320), (1000, 512, 1536)]
+             (65, 144, 64), (128, 128, 128), (129, 1536, 255), (257, 1040, 513), (300, 6144, 320), (1000, 512, 1536),
+             # several tiles a workgroup, of 128 x 128 and 128 x 256, one and several steps of K, odd features
+             (1300, 272, 1600), (2600, 144, 2570), (5000, 128, 2600), (2048, 144, 5120), (4100, 640, 2817)]
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
@@ -263,6 +265,33 @@ def test_linear_q8_rows_behind_and_beside_are_left():
             assert st == 0
             assert torch.equal(out[:M, :F], pr.linear_q8(x, sx, w, sw, dtype=dtype))
             assert (out[M:] == 77).all() and (out[:, F:] == 77).all()
+
+
+def test_linear_q4_and_rows_leave_their_surroundings():
+    """As above for the 4-bit product and the row operators (the C entries with wider outputs)."""
+    from hummingbird_amd import _lib
+    announce("linear_q4, rows: surroundings")
+    lib = _lib.load()
+    for N, K, F in ((3, 64, 33), (7, 160, 130), (17, 96, 8193)):
+        gen = generator(N, K, F)
+        codes, scales = pr.quantize_q4(rand(gen, F, K))
+        for dtype, code in ((torch.bfloat16, 0), (torch.float32, 1), (torch.float16, 2)):
+            x = rand(gen, N, K, dtype=dtype)
+            out = torch.full((N + 2, F + 5), 77.0, device=DEV, dtype=dtype)
+            st = lib.hb_proj_q4(_lib.current_stream(x.device), x.data_ptr(), code, K, codes.data_ptr(), K // 2,
+                                scales.data_ptr(), K // 32, 0, 0, out.data_ptr(), F + 5, N, K, F)
+            assert st == 0
+            assert torch.equal(out[:N, :F], pr.linear_q4(x, codes, scales))
+            assert (out[N:] == 77).all() and (out[:, F:] == 77).all()
+    for N, C in ((5, 72), (3, 2056)):
+        x = rand(generator(N, C), N, C, dtype=torch.bfloat16)
+        q = torch.full((N + 1, C + 8), 1.0, device=DEV).to(torch.float8_e4m3fn)
+        s = torch.full((N + 2,), 77.0, device=DEV)
+        assert lib.hb_quant_rows(_lib.current_stream(x.device), x.data_ptr(), 0, C, q.data_ptr(), C + 8, s.data_ptr(), N,
+                                 C) == 0
+        ref = ew.quantize_rows(x)
+        assert torch.equal(q[:N, :C].float(), ref[0].float()) and torch.equal(s[:N], ref[1])
+        assert (q[N:].float() == 1).all() and (q[:, C:].float() == 1).all() and (s[N:] == 77).all()
 
 
 def test_linear_q8_slices_and_special_values():
