@@ -20,6 +20,11 @@
 namespace hb {
 namespace q8 {
 
+// Outputs of more bytes than half of the last cache (256 MB) are stored past it: what reads them next would not find
+// them there, and they would drive the operands out (8249 x 1536 -> 12288, 203 MB: 172 -> 160 us). Smaller ones stay:
+// without, the denoiser's 120 s render, whose norms read them at once, takes 40.6 ms instead of 40.0.
+constexpr int64_t kStreamBytes = int64_t(128) << 20;
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct Args {
@@ -198,11 +203,15 @@ __device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
 
 // 16 bytes of consecutive results from feature f of a row on, those past the last feature left out. Rows of any stride and
 // width: the 16-byte store takes any alignment of its elements.
-template <typename T>
+// STREAM: past the caches (see kStreamBytes).
+typedef u32x4 u32x4_align2 __attribute__((aligned(2)));
+template <bool STREAM, typename T>
 __device__ __forceinline__ void store16(T* row, int f, int F, u32x4 v) {
   constexpr int N = 16 / static_cast<int>(sizeof(T));
   if (f + N <= F) {
-    __builtin_memcpy(row + f, &v, 16);
+    u32x4_align2* p = reinterpret_cast<u32x4_align2*>(row + f);
+    if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+    else *p = v;
   } else if (f < F) {
 #pragma unroll
     for (int j = 0; j < N - 1; ++j) {
@@ -218,7 +227,7 @@ __device__ __forceinline__ void store16(T* row, int f, int F, u32x4 v) {
 // a lane holds eight consecutive features, and then its 16-lane rows so that four lanes hold 64 bytes of a row (through
 // LDS a tile waits for its own round trip: 5168 x 6144 -> 1536 54 against 43 us). `sw`, `bias`, `sx`: the scales of this
 // wave's features and rows, in LDS.
-template <typename T, class TL>
+template <typename T, class TL, bool STREAM>
 __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL::NF][TL::NM], int f0, int64_t m0,
                                            const float* sw_, const float* bias_, const float* sx_) {
   const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
@@ -257,7 +266,7 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
         for (int q = 0; q < 4; ++q) {  // rows 16 (q % 2) .. of the tile
           const int64_t m = m0 + 32 * t + 16 * (q & 1) + (lr & 15);
           const int f = fn + 16 * (q >> 1) + 8 * (lr >> 4) + 4 * lh;
-          if (m < a.M) store16(out + m * a.os, f, a.F, u32x4{w[q][0], w[q][1], w[q][2], w[q][3]});
+          if (m < a.M) store16<STREAM>(out + m * a.os, f, a.F, u32x4{w[q][0], w[q][1], w[q][2], w[q][3]});
         }
       } else {
         uint32_t w[4][2];  // [g]: features 8 g + 4 lh .. + 3
@@ -279,7 +288,8 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
           const int64_t m = m0 + 32 * t + 16 * p + (lr & 15);
           const int f = fn + 16 * (lr >> 4) + 8 * lh;
           if (m < a.M)
-            store16(out + m * a.os, f, a.F, u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]});
+            store16<STREAM>(out + m * a.os, f, a.F,
+                            u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]});
         }
       }
     }
@@ -295,7 +305,7 @@ int64_t tiles_of(const Args& a) {
 // tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
 // copy that tile's columns again, for nothing: the loop has no branch around a copy, and the kernel waits for them
 // before it ends.
-template <typename T, class TL, bool RAGGED>
+template <typename T, class TL, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL::kWaves, TL::kWaves))) void tiled_kernel(
     const Args a) {
   constexpr bool WIDE = std::is_same<T, float>::value;
@@ -303,10 +313,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   // the scales and biases of a tile and of the next: features' scales, biases, rows' scales
   __shared__ __attribute__((aligned(16))) float scales[2][2 * TL::FT + TL::MT];
   const int nf = (a.F + TL::FT - 1) / TL::FT, nm = static_cast<int>((a.M + TL::MT - 1) / TL::MT), tiles = nf * nm;
-  // Groups of four feature tiles walk the row tiles together, and the workgroups of an XCD take consecutive tiles, so
+  // Groups of eight feature tiles walk the row tiles together (of four: 8249 x 1536 -> 12288 177 against 172 us), and the workgroups of an XCD take consecutive tiles, so
   // that both operands are read from its L2.
   auto origin = [&](int p, int& f0, int64_t& m0) {
-    constexpr int GF = 4;
+    constexpr int GF = 8;
     const int id = xcd_remap(p, tiles), g = id / (GF * nm), gs = nf - g * GF < GF ? nf - g * GF : GF;
     const int in = id - g * GF * nm;
     f0 = (g * GF + in % gs) * TL::FT;
@@ -419,17 +429,24 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
       advance();
     }
     const float* sc = scales[set];
-    store_tile<T, TL>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
+    store_tile<T, TL, STREAM>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
   }
   wait_copies<0>();
 }
 
 template <typename T, class TL>
-void launch_tiled(hipStream_t stream, const Args& a) {
+void launch_tiled(hipStream_t stream_, const Args& a) {
   const int64_t tiles = tiles_of<TL>(a), slots = static_cast<int64_t>(TL::kWaves) * 4 / TL::NW * device_cus();
   const dim3 grid(static_cast<unsigned>(tiles < slots ? tiles : slots)), block(64 * TL::NW);
-  if (a.K % kStep) hipLaunchKernelGGL((tiled_kernel<T, TL, true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((tiled_kernel<T, TL, false>), grid, block, 0, stream, a);
+  auto with = [&](auto ragged, auto stream) {
+    hipLaunchKernelGGL((tiled_kernel<T, TL, decltype(ragged)::value, decltype(stream)::value>), grid, block, 0, stream_, a);
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if constexpr (TL::FT > 64) {  // (small tiles have small outputs)
+    if (a.M * a.F * static_cast<int64_t>(sizeof(T)) > kStreamBytes) return a.K % kStep ? with(yes, yes) : with(no, yes);
+  }
+  a.K % kStep ? with(yes, no) : with(no, no);
 }
 
 // ---- Few tiles ------------------------------------------------------------------------------------------------
@@ -514,7 +531,7 @@ __global__ __launch_bounds__(64 * TL::NW * kGroups) void split_kernel(const Args
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[0][0][4 * g + j] += v[j];
     }
-  store_tile<T, TL>(a, acc, f0 + fw, m0 + mw, scales + fw, scales + TL::FT + fw, scales + 2 * TL::FT + mw);
+  store_tile<T, TL, false>(a, acc, f0 + fw, m0 + mw, scales + fw, scales + TL::FT + fw, scales + 2 * TL::FT + mw);
 }
 
 template <typename T, class TL>

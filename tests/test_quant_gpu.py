@@ -208,7 +208,8 @@ def q8_rows(gen, n, k, spread=1.0):
 Q8_SHAPES = [(1, 16, 1), (1, 1536, 7680), (7, 1536, 512), (16, 64, 100), (17, 80, 33), (33, 256, 257), (64, 6144, 96),
              (65, 144, 64), (128, 128, 128), (129, 1536, 255), (257, 1040, 513), (300, 6144, 320), (1000, 512, 1536),
              # several tiles a workgroup, of 128 x 128 and 128 x 256, one and several steps of K, odd features
-             (1300, 272, 1600), (2600, 144, 2570), (5000, 128, 2600), (2048, 144, 5120), (4100, 640, 2817)]
+             (1300, 272, 1600), (2600, 144, 2570), (5000, 128, 2600), (2048, 144, 5120), (4100, 640, 2817),
+             (8200, 64, 8197), (16500, 128, 4104)]  # outputs past 128 MB
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
