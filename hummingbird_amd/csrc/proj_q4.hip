@@ -9,7 +9,7 @@
 // rows, an fp32 row three (each the next 8 bits of the value, the remainders exact), and those rows are further columns
 // of the same MFMA, whose 16 columns a single row leaves empty anyway. Sums are fp32.
 //
-// A workgroup computes 16 or 64 features for up to 64 columns; its waves take the 128-column chunks of K in turns and
+// A workgroup computes 16 to 64 features for up to 64 columns; its waves take the 128-column chunks of K in turns and
 // their partial sums are added in the waves' order. On v_mfma_f32_16x16x32_bf16 a lane holds 8 consecutive columns of feature
 // (or row) lane % 16; which 8 is free as long as both operands agree, so quarter lane / 16 takes columns 32 q + 8 i of
 // the chunk in MFMA i: a lane's 16 bytes of codes are then one scale group, read in one load.
@@ -256,13 +256,19 @@ void launch_rows(hipStream_t stream, const Args& a) {
   else launch_tiles<T, 4, FT>(stream, a);
 }
 
-// Four tiles of features per wave read x a fourth as often, and leave enough workgroups from half a CU's worth each on
-// (bf16, kernel times: 33 x 6144 -> 12288 28 us against 51 with one tile, 8 x 1536 -> 9216 6.3 against 7.0; but 1 x 6144 ->
-// 1536, 24 workgroups, 14.7 against 6.9).
+// Tiles of features per wave: as few as let every workgroup run at once, one per CU, and four where none do. Fewer read x
+// more often and leave a second, mostly empty round of workgroups; more leave CUs without work (bf16, kernel times with one,
+// two, three and four: 1 x 6144 -> 12288 15.8, 17.8, 13.3 and 16.3 us, 1 x 1536 -> 9216 5.8, 6.1, 5.5 and 6.0,
+// 33 x 6144 -> 12288 51, 41, 28 and 28; with one to three, 1 x 12288 -> 6144 18.8, 16.6 and 21.1). The conversions do not
+// show: without them the kernel is no faster.
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
-  if (a.F >= 64 * (device_cus() / 2)) launch_rows<T, 4>(stream, a);
-  else launch_rows<T, 1>(stream, a);
+  constexpr int R = 16 / Pieces<T>::P;
+  const int64_t tiles = static_cast<int64_t>((a.F + 15) / 16) * ((a.N + 4 * R - 1) / (4 * R)), cus = device_cus();
+  if (tiles <= cus) launch_rows<T, 1>(stream, a);
+  else if (tiles <= 2 * cus) launch_rows<T, 2>(stream, a);
+  else if (tiles <= 3 * cus) launch_rows<T, 3>(stream, a);
+  else launch_rows<T, 4>(stream, a);
 }
 
 }  // namespace q4

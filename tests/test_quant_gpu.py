@@ -322,7 +322,8 @@ def dequant_q4(codes, scales):
 # rows, columns, features: every count of columns about a tile, one group, chunks' ends, one feature
 Q4_SHAPES = [(1, 32, 1), (1, 256, 1536), (2, 1536, 9216), (3, 96, 17), (5, 160, 48), (6, 128, 31), (8, 544, 64),
              (9, 2048, 40), (10, 4128, 33), (11, 224, 16), (16, 6144, 100), (17, 512, 129), (20, 64, 64), (32, 1536, 65),
-             (33, 1536, 65), (64, 1568, 130), (65, 96, 130), (150, 256, 70)]
+             (33, 1536, 65), (64, 1568, 130), (65, 96, 130), (150, 256, 70),
+             (1, 96, 4113), (7, 160, 8190), (18, 64, 8209), (35, 128, 12275), (12, 192, 12305)]
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
