@@ -3,7 +3,8 @@
 //
 //   out[m, f] = (sum_k x[m, k] w[f, k]) sx[m] sw[f] + bias[f],   x, w e4m3, sx, sw, bias and the sum fp32,
 //
-// rounded once to the output type. C^T = W x^T as in the 16-bit projections: a lane of a 32x32 MFMA's result holds one
+// rounded once to the output type. The weights' scales come first: a sum with a row's scale alone can pass the largest
+// fp32 value where the result does not (rows of 1e34 and weights of 1e-4), one with a weight's does not. C^T = W x^T as in the 16-bit projections: a lane of a 32x32 MFMA's result holds one
 // row of x and 16 features, four of them consecutive.
 //
 // The e4m3 matrix cores (v_mfma_f32_32x32x64_f8f6f4, and v_mfma_f32_32x32x16_fp8_fp8 alike) do not add in full fp32:
@@ -251,7 +252,7 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
     for (int t = 0; t < TL::NM; ++t) {
       float v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(acc[n][t][i] * sx[t], sw[i], bias[i]);
+      for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(acc[n][t][i] * sw[i], sx[t], bias[i]);
       if constexpr (sizeof(T) == 4) {
         uint32_t w[4][4];  // [g]: features 8 g + 4 lh .. + 3
 #pragma unroll
@@ -313,8 +314,8 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   // the scales and biases of a tile and of the next: features' scales, biases, rows' scales
   __shared__ __attribute__((aligned(16))) float scales[2][2 * TL::FT + TL::MT];
   const int nf = (a.F + TL::FT - 1) / TL::FT, nm = static_cast<int>((a.M + TL::MT - 1) / TL::MT), tiles = nf * nm;
-  // Groups of eight feature tiles walk the row tiles together (of four: 8249 x 1536 -> 12288 177 against 172 us), and the workgroups of an XCD take consecutive tiles, so
-  // that both operands are read from its L2.
+  // Groups of eight feature tiles walk the row tiles together (of four: 8249 x 1536 -> 12288 177 against 172 us), and the
+  // workgroups of an XCD take consecutive tiles, so that both operands are read from its L2.
   auto origin = [&](int p, int& f0, int64_t& m0) {
     constexpr int GF = 8;
     const int id = xcd_remap(p, tiles), g = id / (GF * nm), gs = nf - g * GF < GF ? nf - g * GF : GF;
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(const Args a) 
     if (r >= M || f0 + fo >= a.F) continue;
     float v = 0.f;
     for (int i = 0; i < waves; ++i) v += part[i][r >> 4][r & 15][fo];
-    out[r * a.os + f0 + fo] = cast_out<T>(__fmaf_rn(v * a.sx[r], a.sw[f0 + fo], a.bias ? a.bias[f0 + fo] : 0.f));
+    out[r * a.os + f0 + fo] = cast_out<T>(__fmaf_rn(v * a.sw[f0 + fo], a.sx[r], a.bias ? a.bias[f0 + fo] : 0.f));
   }
 }
 

@@ -184,7 +184,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
   constexpr int V = Vec<T>::N;
   __shared__ uint32_t sum_buf[kMaxWaves], max_buf[kMaxWaves];
   const int C = a.C, lane = threadIdx.x, lanes = blockDim.x;
-  const int64_t n = blockIdx.x;
+  const int64_t n = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  if (n >= a.N) return;
   const int64_t b = static_cast<uint32_t>(n) / static_cast<uint32_t>(a.L);  // N < 2^31
   const bool add_local = KIND == kResidualNorm && a.local && n - b * a.L >= a.memory;
   float y[CH][V];
@@ -267,8 +268,10 @@ constexpr int kMaxC = 16384;
 template <typename T, int KIND, int CH>
 void launch_ch(hipStream_t stream, const Args<T>& a) {
   const int lanes = (a.C / Vec<T>::N + CH - 1) / CH;
-  hipLaunchKernelGGL((row_kernel<T, KIND, CH>), dim3(static_cast<unsigned>(a.N)), dim3((lanes + 63) / 64 * 64), 0, stream,
-                     a);
+  constexpr int64_t kAcross = 1 << 21;  // a dimension of a grid has less than 2^32 threads
+  const dim3 grid(static_cast<unsigned>(a.N < kAcross ? a.N : kAcross),
+                  static_cast<unsigned>((a.N + kAcross - 1) / kAcross));
+  hipLaunchKernelGGL((row_kernel<T, KIND, CH>), grid, dim3((lanes + 63) / 64 * 64), 0, stream, a);
 }
 
 // One chunk per lane is quickest while the card holds all waves at once (residual_rms_q8, bf16: 1292 x 1536 6.1 us against

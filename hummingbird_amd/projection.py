@@ -217,7 +217,7 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     """`(x * x_scale) @ (weight * weight_scale)^T (+ bias)` of 8-bit rows on the matrix cores (`hb_proj_q8`): `x`
     `(..., K)` e4m3 with `x_scale` `(...)` fp32, `weight` `(F, K)` e4m3 with `weight_scale` `(F,)` fp32 (both as
     `elementwise.quantize_rows` gives them), `bias` `(F,)`; the sum, the scales and the bias in fp32, one rounding to
-    `dtype` (bf16, half or fp32). K a multiple of 16; any number of rows and features."""
+    `dtype` (bf16, half or fp32). K a multiple of 16; up to 2^21 rows and 2^21 features."""
     n, xs, k = _layout(x, "x")
     dev = x.device
     if x.dtype != torch.float8_e4m3fn or weight.dtype != torch.float8_e4m3fn:

@@ -252,6 +252,31 @@ def test_linear_q8_normal_operands(name, M, K, F):
         assert rel <= half_step + (2.0 ** -20 if name == "fp32" else 2.0 ** -13), rel
 
 
+@pytest.mark.parametrize("M,K,F", [(7, 512, 100), (70, 1536, 64), (300, 256, 1600), (2048, 256, 5120)])
+def test_linear_q8_of_large_rows_and_small_weights(M, K, F):
+    """Rows near the largest value: the result is in range where the sum times a row's scale alone is not."""
+    announce("linear_q8 large rows", M, K, F)
+    gen = generator(M, K, F, 2)
+    (x, sx), (w, sw) = q8_rows(gen, M, K, 0.1), q8_rows(gen, F, K, 0.1)
+    sx, sw = sx * 2.0 ** 115, sw * 2.0 ** -20
+    assert (x.float() @ w.float().t()).abs().amax() * sx.amin() > torch.finfo(torch.float32).max
+    for dtype in (torch.bfloat16, torch.float32):
+        got = pr.linear_q8(x, sx, w, sw, dtype=dtype)
+        ref = pr.linear_q8(x, sx * 2.0 ** -115, w, sw * 2.0 ** 20, dtype=dtype)
+        assert torch.equal(got, ref * 2.0 ** 95)  # powers of two: the same bits
+
+
+def test_quantize_rows_of_many_rows():
+    """More rows than one dimension of a grid holds."""
+    announce("quantize_rows, many rows")
+    x = rand(generator(11), 2 ** 21 + 5, 8, dtype=torch.bfloat16)
+    q, s = ew.quantize_rows(x)
+    for rows in (slice(0, 7), slice(2 ** 21 - 3, None)):
+        got = ew.quantize_rows(x[rows])
+        assert torch.equal(q[rows].float(), got[0].float()) and torch.equal(s[rows], got[1])
+    check_q8(q, s, x.double(), x.double().abs(), "many rows")
+
+
 def test_linear_q8_rows_behind_and_beside_are_left():
     """The output's surroundings keep their values at odd sizes (the C entry with a wider output)."""
     from hummingbird_amd import _lib
