@@ -189,7 +189,8 @@ _Q8_LAYERS = (("self_attn", "to_qkv"), ("self_attn", "to_out"), ("cross_attn", "
 def quantize_params(params: dict) -> dict:
     """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
     rows (`elementwise.quantize_rows`, a scale per output feature) and the timestep and global conditioning layers as
-    4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q8"` and `"q4"` of each layer. The other
+    4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q8"` and `"q4"` of each layer, and the GLU's
+    bias in fp32 under `"q8_bias"`. The other
     tensors are shared, not copied. Done once per model, on the weights' device; `prepare_static` then takes the result
     as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
     def sequence(seq):
@@ -201,6 +202,8 @@ def quantize_params(params: dict) -> dict:
         out = dict(b)
         for part, layer in _Q8_LAYERS:
             out[part] = {**out[part], layer: {**b[part][layer], "q8": ew.quantize_rows(b[part][layer]["weight"])}}
+        # in fp32 as the GLU reads it: converted at each call it takes a launch of 2.6 us per block and step
+        out["ff"]["glu_proj"]["q8_bias"] = b["ff"]["glu_proj"]["bias"].float()
         return out
     net = params["transformer"]
     return {**params, "to_timestep_embed": sequence(params["to_timestep_embed"]),
@@ -239,7 +242,7 @@ def _blocks_q8(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tensor,
                                   cfg.qk_norm_eps)
         h, *rows = ew.residual_rms_q8(h, product(ew.quantize_rows(c), cross["to_out"]), block["ff_norm"]["weight"], eps,
                                       local=static["local"][i], memory=cfg.num_memory_tokens, scale=s_ff, shift=sh_ff)
-        f = product(ew.glu_q8(product(rows, ff["glu_proj"]), ff["glu_proj"]["bias"]), ff["proj_out"])
+        f = product(ew.glu_q8(product(rows, ff["glu_proj"]), ff["glu_proj"]["q8_bias"]), ff["proj_out"])
         bias = ff["proj_out"]["bias"].to(dt)
         if i + 1 < depth:
             ns, nsh = chunks(i + 1)[:2]
