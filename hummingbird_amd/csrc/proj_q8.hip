@@ -68,16 +68,19 @@ __device__ __forceinline__ u32x4 widen8(u32x2 c) {
 }
 
 // ---- Tiled product ------------------------------------------------------------------------------------------
-// A workgroup of WF x WM waves computes FT features x MT rows in steps of 128 columns of K, which stream through two
-// LDS stages: rows of 128 bytes whose 16-byte chunks are XOR-swizzled, filled by global_load_lds. A wave multiplies
-// NF x NM tiles of 32 x 32.
+// A workgroup of WF x WM waves computes FT features x MT rows in steps of 128 columns of K, which stream through
+// kStages LDS stages: rows of 128 bytes whose 16-byte chunks are XOR-swizzled, filled by global_load_lds. A wave
+// multiplies NF x NM tiles of 32 x 32. Two stages suffice where a CU has two workgroups or a step takes longer than a
+// copy; a workgroup that has its CU to itself waits for its copies with two (0.5 us a step, whatever the tile) and gains
+// from three or four (2584 x 6144 -> 1536, Medium, 27.5 -> 25.3 us; 400 x 6144 -> 1536, Small, 14.5 -> 12.3).
 constexpr int kStep = 128;  // bytes (columns) of K per stage
 
-template <int FT_, int MT_, int WF_, int WM_, int WAVES_>
+template <int FT_, int MT_, int WF_, int WM_, int WAVES_, int STAGES_ = 2>
 struct Tile {
   static constexpr int FT = FT_, MT = MT_, WF = WF_, WM = WM_;
   static constexpr int NW = WF * WM, NF = FT / WF / 32, NM = MT / WM / 32;
   static constexpr int kWaves = WAVES_;  // per SIMD, of the workgroups that share a CU
+  static constexpr int kStages = STAGES_;
   static constexpr int kStage = (FT + MT) * kStep;
   static constexpr int kBlocksA = FT / 8 / NW, kBlocksB = MT / 8 / NW;  // 1 KB copies per wave and stage
   static_assert(FT % (8 * NW) == 0 && MT % (8 * NW) == 0 && NF >= 1 && NM >= 1, "whole copies and tiles per wave");
@@ -302,15 +305,15 @@ int64_t tiles_of(const Args& a) {
   return static_cast<int64_t>((a.F + TL::FT - 1) / TL::FT) * ((a.M + TL::MT - 1) / TL::MT);
 }
 
-// Workgroups stay: each takes every gridDim.x-th tile, and its copies run two steps ahead of the products across the
-// tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
+// Workgroups stay: each takes every gridDim.x-th tile, and its copies run kStages steps ahead of the products across
+// the tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
 // copy that tile's columns again, for nothing: the loop has no branch around a copy, and the kernel waits for them
 // before it ends.
 template <typename T, class TL, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL::kWaves, TL::kWaves))) void tiled_kernel(
     const Args a) {
   constexpr bool WIDE = std::is_same<T, float>::value;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * TL::kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t smem[TL::kStages * TL::kStage];
   // the scales and biases of a tile and of the next: features' scales, biases, rows' scales
   __shared__ __attribute__((aligned(16))) float scales[2][2 * TL::FT + TL::MT];
   const int nf = (a.F + TL::FT - 1) / TL::FT, nm = static_cast<int>((a.M + TL::MT - 1) / TL::MT), tiles = nf * nm;
@@ -361,12 +364,12 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   if (!a.bias && threadIdx.x < TL::FT) scales[0][TL::FT + threadIdx.x] = scales[1][TL::FT + threadIdx.x] = 0.f;
   aim();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < TL::kStages; ++i) {
 #pragma unroll
     for (int u = 0; u < kCopies; ++u) copy.one(u, cs * kStep, a.K, lds0 + i * TL::kStage);
     advance();
   }
-  wait_copies<kCopies>();
+  wait_copies<(TL::kStages - 1) * kCopies>();
   wait_lds();
   barrier();
   Frags<TL> lo, hi;
@@ -374,11 +377,12 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   for (int i = 0; i < kReads; ++i) lo.read(i, smem, fw, mw, 0);
 
   // A step of a wave is 2 kTiles products, lo's and hi's. In the first kFree the operands of hi are read; then every wave
-  // has the whole stage in registers (barrier) and the step after the next is copied into it, over kTiles products:
-  // faster, the copies wait for the address unit and hold up the products. Before hi's products the next step's copies,
-  // issued a step ago, have landed (barrier), and its lo is read during them.
+  // has the whole stage in registers (barrier) and the step kStages on is copied into it, over kTiles products: faster,
+  // the copies wait for the address unit and hold up the products. Before hi's products the next step's copies, issued
+  // kStages - 1 steps ago, have landed (barrier), and its lo is read during them.
   constexpr int kFree = kTiles / 2;                                    // 0: one barrier does for both
   constexpr int kEarly = (kTiles - kFree) * kCopies / kTiles;          // copies issued before the second barrier
+  constexpr int kLater = (TL::kStages - 2) * kCopies;                  // copies of the steps between the next and that one
   uint32_t b = 0;                                                      // byte offset of the step's stage
   int set = 0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, set ^= 1) {
@@ -413,10 +417,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
         acc[i / TL::NM][i % TL::NM] = multiply<WIDE>(lo.a[i / TL::NM], lo.b[i % TL::NM], acc[i / TL::NM][i % TL::NM]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_copies<kFree == 0 ? 0 : kEarly>();
+      wait_copies<kLater + (kFree == 0 ? 0 : kEarly)>();
       if (kFree == 0) wait_lds();
       barrier();
-      b = TL::kStage - b;
+      b = b == (TL::kStages - 1) * TL::kStage ? 0 : b + TL::kStage;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         if (kFree == 0) copies(i);
@@ -428,6 +432,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
         __builtin_amdgcn_sched_barrier(0);
       }
       advance();
+    }
+    if (nk < TL::kStages - 1) {  // the scales' copies are among those that the last wait left
+      wait_copies<0>();
+      barrier();
     }
     const float* sc = scales[set];
     store_tile<T, TL, STREAM>(a, acc, f0 + fw, m0 + mw, sc + fw, sc + TL::FT + fw, sc + 2 * TL::FT + mw);
@@ -444,7 +452,7 @@ void launch_tiled(hipStream_t stream_, const Args& a) {
   };
   const std::true_type yes;
   const std::false_type no;
-  if constexpr (TL::FT > 64) {  // (small tiles have small outputs)
+  if constexpr (TL::FT * TL::MT >= 128 * 128 && TL::kStages == 2) {  // (the others are for small outputs)
     if (a.M * a.F * static_cast<int64_t>(sizeof(T)) > kStreamBytes) return a.K % kStep ? with(yes, yes) : with(no, yes);
   }
   a.K % kStep ? with(yes, no) : with(no, no);
@@ -633,33 +641,52 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
                      dim3(64 * (chunks < kMaxWaves ? chunks : kMaxWaves)), 0, stream, a);
 }
 
-// Which kernel, as measured (kernel times in us; K = 1536 unless said):
-//   few rows   up to 16 rows (7 x 7680: 5.3 against 6.3 split, 7.9 Small), and up to 32 of a narrow product (24 x 1536:
-//              4.7 against 5.9; but 32 x 7680: 7.6 against 6.4);
-//   split      at most a Small tile per CU and more than 8 steps of K (300 x 1536, K = 6144: 14.4 against 23.1; 64 x 7680:
-//              6.5 against 8.2; at K = 1024 nothing is gained);
-//   Small      products of fewer Medium tiles than keep the CUs busy (700 x 1536, 72 tiles: 8.6 against 9.0; 1300 x 1536,
-//              132 tiles: 10.1 against 9.7; the bf16 cores of fp32 outputs take longer, and the border lies at 192);
-//   Medium     two workgroups share a CU, one's epilogue beside the other's products (2584 x 12288: 50.6 against 57.5
-//              Large);
-//   Large      16-bit outputs whose last round of workgroups is not too empty: a round of Large takes 0.95 of one of
-//              Medium (5168 x 7680: 61.0 against 62.0; 5168 x 1536, K = 6144: 41.1 against 44.6).
+// Which kernel, as measured (times in us, with the 2.5 of a launch; K = 1536 unless said). In order:
+//   few rows   up to 16 rows (7 x 7680: 5.3 against 7.9 Small), and up to 32 of a narrow product (24 x 1536: 4.1 against
+//              5.0, K = 6144 9.4 against 11.6; but 24 x 7680: 5.8 against 5.3);
+//   Small      at most one per CU, with four stages from more than 8 steps on (400 x 1536, K = 6144: 12.3 against 14.0
+//              with three and 16.5 Half; 100 x 1536, K = 256: 3.6 against 3.3 with two);
+//   Half       at most one per CU (1292 x 1536, K = 6144: 16.8 against 21.4 Medium with three stages, 25.0 Small with two);
+//   Medium     at most one per CU, with three stages (2584 x 1536, K = 6144: 25.3 against 27.5 with two); beyond that two
+//              workgroups share a CU, one's epilogue beside the other's products (2584 x 12288: 53 against 56 with three
+//              stages, one per CU, and 61 Large);
+//   then what takes the least time, in rounds of Medium: a round of Large (one per CU) takes 0.95 of one of Medium (two
+//              per CU; 5168 x 7680: 61.0 against 62.0; 5168 x 1536, K = 6144: 41.1 against 44.6) and one of Half 0.7
+//              (504 tiles of Half, 11.3, against the same product's 264 of Medium, 13.9), and a last round of at most
+//              one workgroup per CU 0.65 and 0.5.
+// fp32 outputs are bound by the bf16 cores and the conversions, not by copies: two stages but for Half's and, with a tile
+// per CU and more than 8 steps, K split among 16 waves (400 x 1536, K = 6144: 17.7 against 19.6); Small up to 3/4 Medium
+// tiles per CU (154 x 12288: 13.1 against 14.7 Half); 257 x 12288: 16.3 Half against 21.8 Medium.
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
   using Small = Tile<64, 64, 2, 2, 3>;
+  using Half = Tile<128, 64, 2, 2, 2, 3>;
   using Medium = Tile<128, 128, 2, 2, 2>;
-  using Large = Tile<128, 256, 2, 2, 1>;
-  const int64_t cus = device_cus(), small = tiles_of<Small>(a), medium = tiles_of<Medium>(a);
+  constexpr bool wide = sizeof(T) == 4;
+  const int64_t cus = device_cus(), small = tiles_of<Small>(a), half = tiles_of<Half>(a), medium = tiles_of<Medium>(a);
+  const bool is_long = a.K > 8 * kStep;
   if (a.M <= 16) return launch_few_rows<T, 1>(stream, a);
   if (a.M <= 32 && small <= cus / 4) return launch_few_rows<T, 2>(stream, a);
-  if (small <= cus && a.K > 8 * kStep) return launch_split<T, Small>(stream, a);
-  if (medium <= (sizeof(T) == 4 ? cus * 3 / 4 : cus * 3 / 8)) return launch_tiled<T, Small>(stream, a);
-  if constexpr (sizeof(T) == 2) {
-    const int64_t rest = medium % (2 * cus);
-    const double rounds = static_cast<double>(medium / (2 * cus)) + (rest > cus ? 1.0 : rest > 0 ? 0.65 : 0.0);
-    const int64_t large = tiles_of<Large>(a);
-    if (0.95 * static_cast<double>((large + cus - 1) / cus) <= rounds) return launch_tiled<T, Large>(stream, a);
+  if constexpr (wide) {
+    if (small <= cus && is_long) return launch_split<T, Small>(stream, a);
+    if (medium <= cus * 3 / 4) return launch_tiled<T, Small>(stream, a);
+  } else {
+    if (small <= cus && is_long) return launch_tiled<T, Tile<64, 64, 2, 2, 1, 4>>(stream, a);
+    if (small <= cus) return launch_tiled<T, Small>(stream, a);
+    if (half <= cus) return launch_tiled<T, Half>(stream, a);
+    if (medium <= cus) return launch_tiled<T, Tile<128, 128, 2, 2, 1, 3>>(stream, a);
   }
+  auto rounds = [&](int64_t tiles, double whole, double last) {  // two tiles per CU and round
+    const int64_t rest = tiles % (2 * cus);
+    return static_cast<double>(tiles / (2 * cus)) * whole + (rest > cus ? whole : rest > 0 ? last : 0.0);
+  };
+  const double m = rounds(medium, 1.0, 0.65), h = rounds(half, 0.7, 0.5);
+  if constexpr (!wide) {
+    using Large = Tile<128, 256, 2, 2, 1>;
+    const double l = 0.95 * static_cast<double>((tiles_of<Large>(a) + cus - 1) / cus);
+    if (l <= m && l <= h) return launch_tiled<T, Large>(stream, a);
+  }
+  if (h < m) return launch_tiled<T, Half>(stream, a);
   launch_tiled<T, Medium>(stream, a);
 }
 

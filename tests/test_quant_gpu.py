@@ -209,7 +209,10 @@ Q8_SHAPES = [(1, 16, 1), (1, 1536, 7680), (7, 1536, 512), (16, 64, 100), (17, 80
              (65, 144, 64), (128, 128, 128), (129, 1536, 255), (257, 1040, 513), (300, 6144, 320), (1000, 512, 1536),
              # several tiles a workgroup, of 128 x 128 and 128 x 256, one and several steps of K, odd features
              (1300, 272, 1600), (2600, 144, 2570), (5000, 128, 2600), (2048, 144, 5120), (4100, 640, 2817),
-             (8200, 64, 8197), (16500, 128, 4104)]  # outputs past 128 MB
+             (8200, 64, 8197), (16500, 128, 4104),  # outputs past 128 MB
+             # 64 x 64, 128 x 64 and 128 x 128 tiles with three or four stages: fewer steps than stages, and more
+             (40, 48, 200), (100, 1296, 70), (1300, 112, 1000), (1290, 256, 1030), (1000, 896, 1500), (2000, 96, 2000),
+             (1990, 272, 1990), (2040, 1168, 1537), (1290, 272, 3060), (1300, 80, 6100)]
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
