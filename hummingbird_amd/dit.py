@@ -190,9 +190,9 @@ def quantize_params(params: dict) -> dict:
     """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
     rows (`elementwise.quantize_rows`, a scale per output feature) and the timestep and global conditioning layers as
     4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q8"` and `"q4"` of each layer, and the GLU's
-    bias in fp32 under `"q8_bias"`. The other
-    tensors are shared, not copied. Done once per model, on the weights' device; `prepare_static` then takes the result
-    as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
+    bias in fp32 under `"q8_bias"`. The other tensors are shared, not copied. Done once per model, on the weights'
+    device; `prepare_static` then takes the result as its `params`. The layers' input widths must be multiples of 16
+    (8-bit) and 32 (4-bit)."""
     def sequence(seq):
         return {k: {**layer, "q4": (*projection.quantize_q4(layer["weight"]),
                                     None if layer.get("bias") is None else layer["bias"].float())}
