@@ -118,8 +118,10 @@ __device__ __forceinline__ f32x4 mfma_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
 
 // A wave's sums over the chunks wave, wave + waves, ... for FT tiles of 16 features and CT tiles of 16 columns (rows of x
 // times pieces), from feature 16 FT blockIdx.x and row `rows` blockIdx.y on. x is read once for the FT tiles.
-// Waves of a workgroup: the sums of all its waves, 1 KB for each of a wave's tiles, take at most 128 KB.
-constexpr int max_waves(int tiles) { return 128 / tiles < kMaxWaves ? 128 / tiles : kMaxWaves; }
+// Waves of a workgroup: four per SIMD, and three or two where a wave has more tiles, whose registers then hold the loads of
+// a whole chunk (bf16, 33 x 6144 -> 12288, nine tiles: 24.9 us with 12 waves, 27.4 with 8, 29.1 with 14; 64 x 4096 -> 6144,
+// eight: 21.2, 21.5 and, with 16, 25.2). The sums of all waves, 1 KB for each tile of a wave, take at most 128 KB.
+constexpr int max_waves(int tiles) { return tiles >= 12 ? 8 : tiles >= 6 ? 12 : kMaxWaves; }
 
 template <typename T, int CT, int FT>
 __global__ __launch_bounds__(64 * max_waves(CT * FT)) void q4_kernel(const Args a) {
@@ -259,7 +261,7 @@ void launch_rows(hipStream_t stream, const Args& a) {
 // Tiles of features per wave: as few as let every workgroup run at once, one per CU, and four where none do. Fewer read x
 // more often and leave a second, mostly empty round of workgroups; more leave CUs without work (bf16, kernel times with one,
 // two, three and four: 1 x 6144 -> 12288 15.8, 17.8, 13.3 and 16.3 us, 1 x 1536 -> 9216 5.8, 6.1, 5.5 and 6.0,
-// 33 x 6144 -> 12288 51, 41, 28 and 28; with one to three, 1 x 12288 -> 6144 18.8, 16.6 and 21.1). The conversions do not
+// 33 x 6144 -> 12288, as many waves as 128 KB of sums allow, 51, 41, 28 and 28; with one to three, 1 x 12288 -> 6144 18.8, 16.6 and 21.1). The conversions do not
 // show: without them the kernel is no faster.
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
