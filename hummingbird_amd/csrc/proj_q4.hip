@@ -259,10 +259,10 @@ void launch_rows(hipStream_t stream, const Args& a) {
 }
 
 // Tiles of features per wave: as few as let every workgroup run at once, one per CU, and four where none do. Fewer read x
-// more often and leave a second, mostly empty round of workgroups; more leave CUs without work (bf16, kernel times with one,
-// two, three and four: 1 x 6144 -> 12288 15.8, 17.8, 13.3 and 16.3 us, 1 x 1536 -> 9216 5.8, 6.1, 5.5 and 6.0,
-// 33 x 6144 -> 12288, as many waves as 128 KB of sums allow, 51, 41, 28 and 28; with one to three, 1 x 12288 -> 6144 18.8, 16.6 and 21.1). The conversions do not
-// show: without them the kernel is no faster.
+// more often and leave a second, mostly empty round of workgroups; more leave CUs without work (bf16, kernel times with
+// one, two, three and four: 1 x 6144 -> 12288 15.8, 17.8, 13.3 and 16.3 us, 1 x 1536 -> 9216 5.8, 6.1, 5.5 and 6.0,
+// 33 x 6144 -> 12288, with as many waves as 128 KB of sums allow, 51, 41, 28 and 28; with one to three, 1 x 12288 -> 6144
+// 18.8, 16.6 and 21.1). The conversions do not show: without them the kernel is no faster.
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
   constexpr int R = 16 / Pieces<T>::P;

@@ -408,7 +408,7 @@ def dit_forward(params: dict, x: torch.Tensor, t: torch.Tensor, static: dict, cf
     adaln = static["adaln"][:, None, :] + gcond[None] if "adaln" in static else None  # every block's, one launch
     blocks = static.get("blocks", net["blocks"])
     if q8:
-        if not blocks or "q8" not in blocks[0]["ff"]["proj_out"]:
+        if not blocks or adaln is None or "q8" not in blocks[0]["ff"]["proj_out"]:
             raise ValueError('projections="q8" needs prepare_static to be given the params of quantize_params')
         h = _blocks_q8(h, blocks, static, adaln, cfg)
     elif adaln is not None and blocks and use_hip(cfg, h) and ew.residual_rms_supported(h.dtype, cfg.embed_dim):
