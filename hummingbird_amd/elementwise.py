@@ -235,11 +235,15 @@ def _layout(t: torch.Tensor, name: str) -> tuple[int, int, int]:
 
 
 def _batch_rows(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tensor, name: str) -> tuple[int, int]:
-    """`_per_batch` of a tensor on `x`'s device, with a quick way out for None."""
+    """`_per_batch` of a tensor on `x`'s device, with a quick way out for None and for what is as it should be."""
     if t is None:
         return 0, 0
     if t.device != x.device:
         raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    if t.dtype is x.dtype and t.shape == (batch, channels):
+        step, unit = t.stride()
+        if unit == 1:
+            return t.data_ptr(), (step if batch > 1 else channels)
     return _per_batch(t, batch, channels, x.dtype, name)
 
 
@@ -258,6 +262,8 @@ def _f32_channels(t: torch.Tensor, channels: int, device: torch.device, name: st
     """`t` as `channels` fp32 values on `device`, where it must live (converted where it is not fp32)."""
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.dtype is torch.float32 and t.shape == (channels,) and t.is_contiguous():
+        return t
     t = _f32_vector(t, device)
     if t.numel() != channels:
         raise ValueError(f"{name} must have {channels} elements")
@@ -326,7 +332,7 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
     if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
         raise ValueError(f"h and x must be (B, L, C) of one shape, dtype and device, got {tuple(h.shape)} {h.dtype} "
                          f"{h.device}, {tuple(x.shape)} {x.dtype} {x.device}")
-    _, xs, _ = _layout(x, "x")
+    xs = channels if x.is_contiguous() else _layout(x, "x")[1]
     code = dtype_code(h.dtype)
     batch, length, _ = h.shape
     gp, gs = _batch_rows(gate, batch, channels, h, "gate")
@@ -341,8 +347,8 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
     out_h = _new((batch, length, channels), h.dtype, h.device)
     q, s = _q8_out(h, channels)
     _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs,
-                bp, gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels, q.data_ptr(),
-                channels, s.data_ptr(), rows, channels)
+                bp, gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels,
+                q.data_ptr(), channels, s.data_ptr(), rows, channels)
     return out_h, q, s
 
 
