@@ -55,7 +55,7 @@ int check_common(int dtype, int64_t row_stride, int B, int N, int H, int D, int 
   if (B < 1 || N < 1 || H < 1) return fail(HB_ERR_SHAPE, "need B, N, H >= 1 (B=%d, N=%d, H=%d)", B, N, H);
   if (B > 65535 || H > 65535 || N > (1 << 28))
     return fail(HB_ERR_SHAPE, "shape out of range (B=%d <= 65535, H=%d <= 65535, N=%d <= 2^28)", B, H, N);
-  if (static_cast<int64_t>(B) * N * H * D > (int64_t(1) << 40))
+  if (static_cast<int64_t>(B) * N > (int64_t(1) << 40) / (static_cast<int64_t>(H) * D))  // (the product passes 2^64)
     return fail(HB_ERR_SHAPE, "B*N*H*D exceeds 2^40 elements");
   if (half < 0 || 2 * half > D) return fail(HB_ERR_HALF, "half %d outside [0, D/2=%d]", half, D / 2);
   if (row_stride < static_cast<int64_t>(5) * H * D || row_stride % 8 != 0)

@@ -37,7 +37,7 @@ int check_shape(int dtype, int B, int L, int Nk, int H, int D, float eps) {
     return fail(HB_ERR_SHAPE, "need B, L, Nk, H >= 1 (B=%d, L=%d, Nk=%d, H=%d)", B, L, Nk, H);
   if (B > 65535 || H > 65535 || L > (1 << 28) || Nk > (1 << 28))
     return fail(HB_ERR_SHAPE, "shape out of range (B=%d, H=%d <= 65535; L=%d, Nk=%d <= 2^28)", B, H, L, Nk);
-  if (static_cast<int64_t>(B) * (L > Nk ? L : Nk) * H * D > (int64_t(1) << 40))
+  if (static_cast<int64_t>(B) * (L > Nk ? L : Nk) > (int64_t(1) << 40) / (static_cast<int64_t>(H) * D))
     return fail(HB_ERR_SHAPE, "B*max(L,Nk)*H*D exceeds 2^40 elements");
   if (!(eps >= 0.0f) || !isfinite(eps)) return fail(HB_ERR_EPS, "eps %g must be finite and >= 0", eps);
   return HB_OK;

@@ -143,6 +143,16 @@ def test_validators_follow_the_contract(lib, dtype, D, B, N, H, half, stride_mul
         _expected_status(dtype, row_stride, B, N, H, D, half, 0 if window >= 0 else 6)
 
 
+@pytest.mark.parametrize("B,N,H,D", [(65535, 1 << 28, 65535, 64), (32768, 1 << 28, 32768, 64), (65535, 1 << 28, 1024, 128)])
+def test_element_counts_past_64_bits_are_refused(lib, B, N, H, D):
+    """B N H D of 2^64 and more is past 2^40, whatever its remainder."""
+    stride = 5 * H * D
+    assert lib.hb_dense_validate(0, stride, B, N, H, D, 0, 1e-6) == 2
+    assert lib.hb_band_validate(0, stride, B, N, H, D, 0, 1) == 2
+    assert lib.hb_cross_validate(0, 2 * H * D, 3 * H * D, B, N, 1, H, D, 1e-6) == 2
+    assert lib.hb_cross_validate(0, 2 * H * D, 3 * H * D, B, 1, N, H, D, 1e-6) == 2
+
+
 def test_workspace_size(lib):
     # three (B, H, Lp, D) regions (k, k_diff, v prepared) with L padded to the 128-query block
     assert lib.hb_dense_workspace_size(0, 2, 2584, 24, 64) == 3 * 2 * 24 * 2688 * 64 * 2
