@@ -653,7 +653,9 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
 //   then what takes the least time, in rounds of Medium: a round of Large (one per CU) takes 0.95 of one of Medium (two
 //              per CU; 5168 x 7680: 61.0 against 62.0; 5168 x 1536, K = 6144: 41.1 against 44.6) and one of Half 0.7
 //              (504 tiles of Half, 11.3, against the same product's 264 of Medium, 13.9), and a last round of at most
-//              one workgroup per CU 0.65 and 0.5.
+//              one workgroup per CU 0.65 and 0.5. Tall, three stages and one per CU, takes 0.74 where one round of it
+//              does (4000 x 1536: 12.4 against 14.4 Medium; 700 x 7680: 12.7 against 14.3); beyond one round it gains
+//              in a loop over one product (1292 x 12288: 28.4 against 30.4) and loses in a render (39.7 against 38.9 ms).
 // fp32 outputs are bound by the bf16 cores and the conversions, not by copies: two stages but for Half's and, with a tile
 // per CU and more than 8 steps, K split among 16 waves (400 x 1536, K = 6144: 17.7 against 19.6); Small up to 3/4 Medium
 // tiles per CU (154 x 12288: 13.1 against 14.7 Half); 257 x 12288: 16.3 Half against 21.8 Medium.
@@ -683,7 +685,9 @@ void launch(hipStream_t stream, const Args& a) {
   const double m = rounds(medium, 1.0, 0.65), h = rounds(half, 0.7, 0.5);
   if constexpr (!wide) {
     using Large = Tile<128, 256, 2, 2, 1>;
+    using Tall = Tile<128, 192, 2, 2, 1, 3>;
     const double l = 0.95 * static_cast<double>((tiles_of<Large>(a) + cus - 1) / cus);
+    if (tiles_of<Tall>(a) <= cus && h > 0.74) return launch_tiled<T, Tall>(stream, a);
     if (l <= m && l <= h) return launch_tiled<T, Large>(stream, a);
   }
   if (h < m) return launch_tiled<T, Half>(stream, a);

@@ -212,7 +212,8 @@ Q8_SHAPES = [(1, 16, 1), (1, 1536, 7680), (7, 1536, 512), (16, 64, 100), (17, 80
              (8200, 64, 8197), (16500, 128, 4104),  # outputs past 128 MB
              # 64 x 64, 128 x 64 and 128 x 128 tiles with three or four stages: fewer steps than stages, and more
              (40, 48, 200), (100, 1296, 70), (1300, 112, 1000), (1290, 256, 1030), (1000, 896, 1500), (2000, 96, 2000),
-             (1990, 272, 1990), (2040, 1168, 1537), (1290, 272, 3060), (1300, 80, 6100)]
+             (1990, 272, 1990), (2040, 1168, 1537), (1290, 272, 3060), (1300, 80, 6100),
+             (4000, 208, 1501), (1291, 400, 12200), (700, 128, 7600), (3990, 1040, 1410)]  # 128 x 192 tiles
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
