@@ -429,6 +429,40 @@ def test_linear_q4_scales(code):
     assert torch.equal(pr.linear_q4(x, codes, scales)[0].double(), w[:, 5])
 
 
+def spread(t, stride):
+    """`t`'s rows `stride` elements apart in memory that nothing else is written to."""
+    rows, width = t.shape
+    out = torch.empty((rows - 1) * stride + width, dtype=t.dtype, device=DEV).as_strided((rows, width), (stride, 1))
+    out.copy_(t)
+    return out
+
+
+def test_offsets_past_32_bits():
+    """Rows, weights and outputs that end past 2^32 bytes and elements: equal to those next to each other."""
+    announce("offsets past 32 bits: rows")
+    gen = generator(12)
+    x = rand(gen, 4, 256, dtype=torch.bfloat16)
+    far = spread(x, 3 << 29)
+    for got, ref in zip(ew.quantize_rows(far), ew.quantize_rows(x)):
+        assert torch.equal(got.float(), ref.float())
+    announce("offsets past 32 bits: linear_q4")
+    codes, scales = pr.quantize_q4(rand(gen, 600, 256))
+    ref = pr.linear_q4(x, codes, scales)
+    assert torch.equal(pr.linear_q4(far, spread(codes, 1 << 23), spread(scales, 1 << 23)), ref)
+    del far
+    announce("offsets past 32 bits: linear_q8")
+    for M, F in ((1100, 700), (16, 1100), (2000, 3000)):
+        (q, s), (w, sw) = q8_rows(gen, M, 144), q8_rows(gen, F, 144)
+        ref = pr.linear_q8(q, s, w, sw)
+        far_q = spread(q.view(torch.uint8), 1 << 22).view(torch.float8_e4m3fn)
+        far_w = spread(w.view(torch.uint8), 1 << 22).view(torch.float8_e4m3fn)
+        assert torch.equal(pr.linear_q8(far_q, s, far_w, sw), ref)
+        del far_q, far_w
+    (q, s), (w, sw) = q8_rows(gen, 70000, 64), q8_rows(gen, 32768, 64)
+    out = pr.linear_q8(q, s, w, sw)
+    assert torch.equal(out[69000:], pr.linear_q8(q[69000:], s[69000:].contiguous(), w, sw))
+
+
 def test_refusals_of_devices_types_and_shapes():
     announce("refusals")
     x = torch.zeros(4, 64, device=DEV, dtype=torch.bfloat16)
