@@ -38,7 +38,7 @@ struct Args {
 };
 
 // Rows of x as bf16 rows whose sum they are: P pieces, each the leading 8 bits of what the earlier ones leave (truncated,
-// so that no piece overflows and every remainder is exact). Piece p is x after p times y -= y & 0xffff0000, cut to its
+// so that no piece overflows and every remainder is exact; a bf16 value has no bits below 2^-133). Piece p is x after p times y -= y & 0xffff0000, cut to its
 // upper half: a lane holds the masks of its piece, zero past it. An infinity or NaN leaves NaNs in the later pieces;
 // what counts then is the first one's sum (see the end of the kernel).
 template <typename T>

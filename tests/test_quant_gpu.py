@@ -417,6 +417,19 @@ def test_linear_q4_keeps_all_bits_of_x(name):
     assert torch.isnan(out[5]).all()
 
 
+@pytest.mark.parametrize("exponent", [-100, -115, -125])
+def test_linear_q4_of_small_fp32_rows(exponent):
+    """fp32 rows keep their bits down to 2^-133: off by at most 2^-133 a value beyond the sum's rounding."""
+    announce("linear_q4 small rows", exponent)
+    gen = generator(13)
+    x = rand(gen, 5, 256, std=2.0 ** exponent)
+    codes, scales = pr.quantize_q4(rand(gen, 64, 256, std=2.0 ** 60))
+    w = dequant_q4(codes, scales)
+    got, ref = pr.linear_q4(x, codes, scales).double(), x.double() @ w.t()
+    bound = (256 + 4) * 2.0 ** -24 * (x.double().abs() @ w.abs().t()) + 2.0 ** -133 * w.abs().sum(-1)
+    assert ((got - ref).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("code", [8, 9, 64, 127, 200, 249, 250])
 def test_linear_q4_scales(code):
     announce("linear_q4 scale", code)
