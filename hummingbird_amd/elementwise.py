@@ -114,6 +114,18 @@ def _per_batch(t: torch.Tensor | None, batch: int, channels: int, dtype: torch.d
     return t2.data_ptr(), (t2.stride(0) if batch > 1 else channels)
 
 
+def _channel_vector(t: torch.Tensor | None, channels: int, x: torch.Tensor, name: str) -> int:
+    """The pointer of `channels` values of `x`'s dtype and device next to each other, 0 for None. (A `(C, 1)` slice of a
+    wider tensor has C values and a last stride of 1, but is not that.)"""
+    if t is None:
+        return 0
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    if t.dtype != x.dtype or t.numel() != channels or not t.is_contiguous():
+        raise ValueError(f"{name} must be ({channels},) of {x.dtype} with unit stride")
+    return t.data_ptr()
+
+
 def rms_modulate(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: torch.Tensor | None = None,
                  shift: torch.Tensor | None = None) -> torch.Tensor:
     """The DiT block norm on `(B, L, C)`: `cast(x * rsqrt(mean(x^2) + eps) * weight)` with an fp32 island
@@ -154,18 +166,12 @@ def gated_residual(h: torch.Tensor, x: torch.Tensor, gate: torch.Tensor | None =
     _, hs = _rows(h, "h")
     rows, xs = _rows(x, "x")
     gp, gs = _per_batch(gate, batch, channels, h.dtype, "gate")
-
-    def vec(t, name):
-        if t is None:
-            return 0
-        if t.dtype != h.dtype or t.numel() != channels or t.stride(-1) != 1:
-            raise ValueError(f"{name} must be ({channels},) of {h.dtype} with unit stride")
-        return t.data_ptr()
+    bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
     out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     stream = _lib.current_stream(h.device)
     _lib.check(_lib.load().hb_gated_residual(stream, h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
-                                             vec(x_bias, "x_bias"), gp, gs, vec(local, "local"), int(memory), length,
-                                             out.data_ptr(), channels, rows, channels), "gated_residual")
+                                             bp, gp, gs, lp, int(memory), length, out.data_ptr(), channels, rows,
+                                             channels), "gated_residual")
     return out
 
 
@@ -193,20 +199,14 @@ def residual_rms(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: fl
     w = weight.to(device=h.device, dtype=torch.float32).contiguous().reshape(-1)
     if w.numel() != channels:
         raise ValueError(f"weight must have {channels} elements")
-
-    def vec(t, name):
-        if t is None:
-            return 0
-        if t.dtype != h.dtype or t.numel() != channels or t.stride(-1) != 1:
-            raise ValueError(f"{name} must be ({channels},) of {h.dtype} with unit stride")
-        return t.data_ptr()
+    bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
     out_h = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     out_y = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     stream = _lib.current_stream(h.device)
     _lib.check(_lib.load().hb_residual_rms(stream, h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
-                                           vec(x_bias, "x_bias"), gp, gs, vec(local, "local"), int(memory),
-                                           w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(),
-                                           out_y.data_ptr(), channels, rows, channels), "residual_rms")
+                                           bp, gp, gs, lp, int(memory), w.data_ptr(), float(eps), sp, hp, ms, length,
+                                           out_h.data_ptr(), out_y.data_ptr(), channels, rows, channels),
+               "residual_rms")
     return out_h, out_y
 
 
@@ -245,17 +245,6 @@ def _batch_rows(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tens
         if unit == 1:
             return t.data_ptr(), (step if batch > 1 else channels)
     return _per_batch(t, batch, channels, x.dtype, name)
-
-
-def _channel_vector(t: torch.Tensor | None, channels: int, x: torch.Tensor, name: str) -> int:
-    """The pointer of a `(C,)` vector of `x`'s dtype and device, 0 for None."""
-    if t is None:
-        return 0
-    if t.device != x.device:
-        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
-    if t.dtype != x.dtype or t.numel() != channels or t.stride(-1) != 1:
-        raise ValueError(f"{name} must be ({channels},) of {x.dtype} with unit stride")
-    return t.data_ptr()
 
 
 def _f32_channels(t: torch.Tensor, channels: int, device: torch.device, name: str) -> torch.Tensor:

@@ -1,0 +1,20 @@
+"""What the wrappers of the row operators make of their operands' shapes and strides, on the CPU (no kernel runs)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from hummingbird_amd import elementwise as ew
+
+
+def test_channel_vectors_are_values_next_to_each_other():
+    """A (C, 1) slice of a wider tensor has C values and a last stride of 1, and its values lie apart."""
+    x = torch.zeros(2, 3, 16)
+    wide = torch.arange(16 * 8, dtype=torch.float32).reshape(16, 8)
+    for good in (torch.ones(16), torch.ones(1, 16), torch.ones(1, 1, 16), torch.ones(16, 1), wide[2:4].reshape(16)):
+        assert ew._channel_vector(good, 16, x, "x_bias") == good.data_ptr()
+    assert ew._channel_vector(None, 16, x, "x_bias") == 0
+    for bad in (wide[:, :1], wide[:, 3], torch.ones(32)[::2], torch.ones(()), torch.ones(8), torch.ones(16).double(),
+                torch.ones(16, device="meta")):
+        with pytest.raises(ValueError, match="x_bias"):
+            ew._channel_vector(bad, 16, x, "x_bias")
