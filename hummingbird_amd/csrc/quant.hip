@@ -115,10 +115,25 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, int waves, uint32_t* buf
   return row_reduce(v, waves, buf, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
+// y / s, correctly rounded, for values |y| <= 448 s: y times the rounded reciprocal of s, off by an fp32 unit or two, and a
+// step of the remainder, which is exact while s is at least 2^-90. Without the step one value in 2000 of bf16 rows (they
+// often lie on a border between two codes) gets the wrong code; with the compiler's division instead the row operators
+// take up to a third longer (quantize_rows on 5168 x 1536 bf16: 5.9 us without the step, 6.4 with it, 8.6 divided). The order
+// of the operations keeps the sign of a zero.
+struct Divisor {
+  float s, inv;
+  // (an infinite scale leaves finite values zero, and infinite ones NaN)
+  __device__ explicit Divisor(float scale) : s(__builtin_isinf(scale) ? 0.f : scale), inv(__fdiv_rn(1.f, scale)) {}
+  __device__ float quotient(float y) const {
+    const float q = y * inv;
+    return __fmaf_rn(-__fmaf_rn(q, s, -y), inv, q);
+  }
+};
+
 // The row's scale and its values in 8 bits; y holds zeros past the row, `lane` of the row's `lanes`. Magnitudes are
 // compared as their bits: a NaN's are above every number's, so it reaches the scale.
 template <int V, int CH>
-__device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, float* s, int C, int lane, int lanes,
+__device__ __forceinline__ void store_q8(float (&y)[CH][V], uint8_t* q, float* s, int C, int lane, int lanes,
                                          uint32_t* buf) {
   uint32_t m = 0;
 #pragma unroll
@@ -131,7 +146,15 @@ __device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, fl
   const float amax = __uint_as_float(row_max(m, lanes / 64, buf));
   float sc = __fdiv_rn(amax, 448.f);
   if (sc < kScaleFloor) sc = kScaleFloor;  // not for a NaN
-  const float inv = __fdiv_rn(1.f, sc);
+  float up = 1.f;
+  if (sc < 0x1p-64f) {  // so that no remainder falls below the fp32 range; a branch of the whole row
+    up = 0x1p64f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[k][j] *= up;
+  }
+  const Divisor by(sc * up);
 #pragma unroll
   for (int k = 0; k < CH; ++k) {
     const int c0 = (k * lanes + lane) * V;
@@ -139,7 +162,8 @@ __device__ __forceinline__ void store_q8(const float (&y)[CH][V], uint8_t* q, fl
       uint32_t w[V / 4];
 #pragma unroll
       for (int i = 0; i < V / 4; ++i)
-        w[i] = pack_e4m3x4(y[k][4 * i] * inv, y[k][4 * i + 1] * inv, y[k][4 * i + 2] * inv, y[k][4 * i + 3] * inv);
+        w[i] = pack_e4m3x4(by.quotient(y[k][4 * i]), by.quotient(y[k][4 * i + 1]), by.quotient(y[k][4 * i + 2]),
+                           by.quotient(y[k][4 * i + 3]));
       if constexpr (V == 8) *reinterpret_cast<u32x2*>(q + c0) = u32x2{w[0], w[1]};
       else *reinterpret_cast<uint32_t*>(q + c0) = w[0];
     }
