@@ -3,9 +3,8 @@
 //
 //   out[m, f] = (sum_k x[m, k] w[f, k]) sx[m] sw[f] + bias[f],   x, w e4m3, sx, sw, bias and the sum fp32,
 //
-// rounded once to the output type. The weights' scales come first: a sum with a row's scale alone can pass the largest
-// fp32 value where the result does not (rows of 1e34 and weights of 1e-4), one with a weight's does not. C^T = W x^T as in the 16-bit projections: a lane of a 32x32 MFMA's result holds one
-// row of x and 16 features, four of them consecutive.
+// rounded once to the output type, for any scales (see `scaled`). C^T = W x^T as in the 16-bit projections: a lane of a
+// 32x32 MFMA's result holds one row of x and 16 features, four of them consecutive.
 //
 // The e4m3 matrix cores (v_mfma_f32_32x32x64_f8f6f4, and v_mfma_f32_32x32x16_fp8_fp8 alike) do not add in full fp32:
 // within 16 products, what lies more than 13 bits below the largest is dropped. On rows of normal values that is an
@@ -45,6 +44,22 @@ struct Args {
 // e4m3 x e4m3 without block scales, fp32 accumulation.
 __device__ __forceinline__ f32x16 mfma_32x32x64(i32x8 a, i32x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+}
+
+// acc sw sx + bias for any scales, whatever the range of the products on the way. A sum of e4m3 products is 0 or of a
+// magnitude from 2^-18 to 2^41 (K <= 2^23). With a feature's scale of 2^-100 to 2^86 it stays in the fp32 range, and one
+// FMA does the rest. (The row's scale first would overflow for rows of 1e34 and weights of 1e-4.) Other scales, which
+// weights of 1e30 have, would overflow or lose bits where the result does not (weights of 1e33 and rows of 1e-10): they
+// are multiplied as mantissas and their exponents added.
+__device__ __forceinline__ bool ordinary(float sw) {
+  return __float_as_uint(sw) - __float_as_uint(0x1p-100f) <= __float_as_uint(0x1p86f) - __float_as_uint(0x1p-100f);
+}
+__device__ __forceinline__ float scaled_ordinary(float acc, float sw, float sx, float bias) {
+  return __fmaf_rn(acc * sw, sx, bias);
+}
+__device__ __forceinline__ float scaled_any(float acc, float sw, float sx, float bias) {
+  const float m = acc * __builtin_amdgcn_frexp_mantf(sw) * __builtin_amdgcn_frexp_mantf(sx);
+  return ldexpf(m, __builtin_amdgcn_frexp_expf(sw) + __builtin_amdgcn_frexp_expf(sx)) + bias;
 }
 
 template <typename T>
@@ -239,6 +254,10 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
   float sx[TL::NM];
 #pragma unroll
   for (int t = 0; t < TL::NM; ++t) sx[t] = sx_[32 * t + lr];
+  bool odd = false;  // any scale of the wave's features that is not ordinary: a branch of the whole wave
+#pragma unroll
+  for (int n = 0; n < TL::NF; ++n) odd |= !ordinary(sw_[32 * n + lr]);
+  odd = __any(odd);
 #pragma unroll
   for (int n = 0; n < TL::NF; ++n) {
     const int fn = f0 + 32 * n;
@@ -254,8 +273,13 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
 #pragma unroll
     for (int t = 0; t < TL::NM; ++t) {
       float v[16];
+      if (__builtin_expect(odd, 0)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __fmaf_rn(acc[n][t][i] * sw[i], sx[t], bias[i]);
+        for (int i = 0; i < 16; ++i) v[i] = scaled_any(acc[n][t][i], sw[i], sx[t], bias[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = scaled_ordinary(acc[n][t][i], sw[i], sx[t], bias[i]);
+      }
       if constexpr (sizeof(T) == 4) {
         uint32_t w[4][4];  // [g]: features 8 g + 4 lh .. + 3
 #pragma unroll
@@ -630,7 +654,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(const Args a) 
     if (r >= M || f0 + fo >= a.F) continue;
     float v = 0.f;
     for (int i = 0; i < waves; ++i) v += part[i][r >> 4][r & 15][fo];
-    out[r * a.os + f0 + fo] = cast_out<T>(__fmaf_rn(v * a.sw[f0 + fo], a.sx[r], a.bias ? a.bias[f0 + fo] : 0.f));
+    const float sw = a.sw[f0 + fo], bias = a.bias ? a.bias[f0 + fo] : 0.f;
+    v = ordinary(sw) ? scaled_ordinary(v, sw, a.sx[r], bias) : scaled_any(v, sw, a.sx[r], bias);
+    out[r * a.os + f0 + fo] = cast_out<T>(v);
   }
 }
 
