@@ -277,7 +277,8 @@ def quantize_q4(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
               silu: bool = False) -> torch.Tensor:
     """`act(x @ W^T (+ bias))` for few rows `x` `(..., K)` and 4-bit weights (`hb_proj_q4`): `weight` `(F, K / 2)` and
-    `weight_scale` `(F, K / 32)`, both uint8, as `quantize_q4` gives them; `bias` `(F,)`; act = SiLU with `silu`. x
+    `weight_scale` `(F, K / 32)`, both uint8, as `quantize_q4` gives them (any bytes are taken: under a scale of 253 or 254
+    weights of 2^128 and more are infinite, 255 makes its group NaN); `bias` `(F,)`; act = SiLU with `silu`. x
     keeps all of its bits (bf16, half or fp32, there those above 2^-133), the sum, bias and activation are fp32, rounded
     once to `x.dtype`. It serves the layers that see one row per batch entry; up to 2^16 rows are taken."""
     n, xs, k = _layout(x, "x")

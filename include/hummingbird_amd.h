@@ -327,8 +327,9 @@ int hb_residual_rms(hipStream_t stream, const void* h, int dtype, int64_t h_row_
  *   of 1.5e-5 of the result on normal values); for HB_F32 the sums are full fp32.
  * hb_proj_q4 : out[n, f] = act(sum_k x[n, k] e2m1(w[f, k]) 2^(w_scale[f, k / 32] - 127) + bias[f]) for few rows x
  *   (N, K) of `dtype`: w holds two 4-bit codes per byte (OCP e2m1: sign, 2 exponent bits, 1 mantissa bit; the low
- *   nibble the even column), w_scale one e8m0 byte per 32 columns, in [8, 250] (others give scales that the products
- *   do not hold). x keeps all of its bits (fp32: those above 2^-133); sums in fp32; act = SiLU when `silu` != 0, else none; out of `dtype`.
+ *   nibble the even column), w_scale one e8m0 byte per 32 columns. Every code is exact under the bytes 0 to 252; under
+ *   253 and 254 weights of 2^128 and more are infinite, and the byte 255 makes its 32 weights NaN (as in OCP MX). x keeps
+ *   all of its bits (fp32: those above 2^-133); sums in fp32; act = SiLU when `silu` != 0, else none; out of `dtype`.
  *   K a multiple of 32, any N up to 2^16 and F; w row stride (bytes) a multiple of 16, w and x 16-byte aligned, x row
  *   stride a multiple of 8 (bf16, half) or 4 (fp32). */
 int hb_quant_rows(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, void* q, int64_t q_row_stride,

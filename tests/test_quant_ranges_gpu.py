@@ -1,5 +1,5 @@
-"""The quantised products at the ends of their operands' ranges, on the GPU: any fp32 scales of `linear_q8` against
-fp64."""
+"""The quantised products at the ends of their operands' ranges, on the GPU: any fp32 scales of `linear_q8` and any scale
+bytes of `linear_q4` against fp64."""
 from __future__ import annotations
 
 import pytest
@@ -90,3 +90,31 @@ def test_linear_q8_of_scales_that_are_no_numbers(M, K, F):
     ref = ((x.double() @ w.double().t()) * sw.double() * sx.double()[:, None]).float()
     assert torch.equal(torch.isnan(got), torch.isnan(ref))
     assert torch.equal(got.nan_to_num(0.0, 1.0, -1.0), ref.nan_to_num(0.0, 1.0, -1.0))
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("x", [1.0, 2.0 ** -14, 1.75 * 2.0 ** 14])
+def test_linear_q4_of_every_scale_byte(name, x):
+    """Every code under every byte, picked out by one value of x (both nibbles, first and later groups): the product of
+    a power of two times 1.75 and a code of at most 2 bits is exact, so it comes back rounded once. Weights of 2^128 and
+    more are infinite, a group of byte 255 is NaN whatever x is."""
+    announce("linear_q4 every byte", name, x)
+    dtype = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}[name]
+    levels = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=DEV, dtype=torch.float64)
+    levels = torch.cat([levels, -levels])
+    for column in (0, 1, 32 * 5 + 7, 32 * 5 + 30):
+        codes = torch.zeros(256 * 16, 96, dtype=torch.uint8, device=DEV)
+        codes[:, column // 2] = torch.arange(16, device=DEV, dtype=torch.uint8).repeat(256) << (4 * (column % 2))
+        byte = torch.arange(256, device=DEV).repeat_interleave(16)
+        scales = torch.full((256 * 16, 6), 127, dtype=torch.uint8, device=DEV)
+        scales[:, column // 32] = byte.to(torch.uint8)
+        v = torch.zeros(2, 192, dtype=dtype, device=DEV)
+        v[1, column] = x
+        w = levels.repeat(256) * torch.exp2(byte.double() - 127)
+        held = torch.where(w.abs() >= 2.0 ** 128, torch.sign(w) * float("inf"), w)
+        held[byte == 255] = float("nan")
+        got = pr.linear_q4(v, codes, scales)
+        for row, value in ((0, 0.0), (1, x)):
+            ref = (held * value).float().to(dtype)
+            assert torch.equal(torch.isnan(got[row]), torch.isnan(ref)), (column, row)
+            assert torch.equal(got[row].nan_to_num(0.5), ref.nan_to_num(0.5)), (column, row)
