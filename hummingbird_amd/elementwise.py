@@ -126,6 +126,13 @@ def _channel_vector(t: torch.Tensor | None, channels: int, x: torch.Tensor, name
     return t.data_ptr()
 
 
+def _memory_tokens(memory: int, length: int) -> int:
+    """The first token that takes `local`, of `length`: as a C int, which holds no more than 31 bits."""
+    if memory < 0:
+        raise ValueError(f"memory must be >= 0, got {memory}")
+    return min(int(memory), length)
+
+
 def rms_modulate(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: torch.Tensor | None = None,
                  shift: torch.Tensor | None = None) -> torch.Tensor:
     """The DiT block norm on `(B, L, C)`: `cast(x * rsqrt(mean(x^2) + eps) * weight)` with an fp32 island
@@ -170,8 +177,8 @@ def gated_residual(h: torch.Tensor, x: torch.Tensor, gate: torch.Tensor | None =
     out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     stream = _lib.current_stream(h.device)
     _lib.check(_lib.load().hb_gated_residual(stream, h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
-                                             bp, gp, gs, lp, int(memory), length, out.data_ptr(), channels, rows,
-                                             channels), "gated_residual")
+                                             bp, gp, gs, lp, _memory_tokens(memory, length), length, out.data_ptr(),
+                                             channels, rows, channels), "gated_residual")
     return out
 
 
@@ -204,8 +211,8 @@ def residual_rms(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: fl
     out_y = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     stream = _lib.current_stream(h.device)
     _lib.check(_lib.load().hb_residual_rms(stream, h.data_ptr(), dtype_code(h.dtype), hs, x.data_ptr(), xs,
-                                           bp, gp, gs, lp, int(memory), w.data_ptr(), float(eps), sp, hp, ms, length,
-                                           out_h.data_ptr(), out_y.data_ptr(), channels, rows, channels),
+                                           bp, gp, gs, lp, _memory_tokens(memory, length), w.data_ptr(), float(eps), sp,
+                                           hp, ms, length, out_h.data_ptr(), out_y.data_ptr(), channels, rows, channels),
                "residual_rms")
     return out_h, out_y
 
@@ -336,8 +343,8 @@ def residual_rms_q8(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps:
     out_h = _new((batch, length, channels), h.dtype, h.device)
     q, s = _q8_out(h, channels)
     _lib.launch(_lib.load().hb_residual_rms_q8, "residual_rms_q8", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs,
-                bp, gp, gs, lp, memory, w.data_ptr(), float(eps), sp, hp, ms, length, out_h.data_ptr(), channels,
-                q.data_ptr(), channels, s.data_ptr(), rows, channels)
+                bp, gp, gs, lp, _memory_tokens(memory, length), w.data_ptr(), float(eps), sp, hp, ms, length,
+                out_h.data_ptr(), channels, q.data_ptr(), channels, s.data_ptr(), rows, channels)
     return out_h, q, s
 
 

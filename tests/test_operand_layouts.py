@@ -18,3 +18,12 @@ def test_channel_vectors_are_values_next_to_each_other():
                 torch.ones(16, device="meta")):
         with pytest.raises(ValueError, match="x_bias"):
             ew._channel_vector(bad, 16, x, "x_bias")
+
+
+def test_memory_tokens_keep_their_meaning_past_32_bits():
+    """Cut to the sequence's length, not to the low 32 bits of a C int."""
+    for memory, held in ((0, 0), (3, 3), (4, 4), (5, 4), (1 << 31, 4), (1 << 32, 4), ((1 << 32) + 1, 4), (1 << 70, 4)):
+        assert ew._memory_tokens(memory, 4) == held
+    for memory in (-1, -(1 << 32), -(1 << 31) - 5):
+        with pytest.raises(ValueError, match="memory"):
+            ew._memory_tokens(memory, 4)

@@ -33,3 +33,20 @@ def test_channel_vectors_of_other_strides_are_refused(op, operand):
             call(bad)
     for good in (column.contiguous(), column[:, 0].contiguous(), column[:, 0].contiguous()[None]):
         assert torch.equal(call(good)[0, 1], wide[:, 0])
+
+
+@pytest.mark.parametrize("op", ["gated_residual", "residual_rms", "residual_rms_q8"])
+def test_memory_past_32_bits_is_past_the_end(op):
+    announce("memory past 32 bits", op)
+    h = torch.zeros(2, 4, 64, device=DEV)
+    ones = torch.ones(64, device=DEV)
+
+    def call(memory):
+        if op == "gated_residual":
+            return ew.gated_residual(h, h, local=ones, memory=memory)
+        return getattr(ew, op)(h, h, ones, 1e-5, local=ones, memory=memory)[0]
+    for memory in (4, 5, 1 << 31, 1 << 32, (1 << 32) + 2):
+        assert (call(memory) == 0).all(), memory
+    assert torch.equal(call(3)[:, :, 0], torch.tensor([[0.0, 0, 0, 1]] * 2, device=DEV))
+    with pytest.raises(ValueError):
+        call(-(1 << 32))
