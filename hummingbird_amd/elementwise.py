@@ -236,9 +236,10 @@ def _layout(t: torch.Tensor, name: str) -> tuple[int, int, int]:
     width = t.shape[-1] if t.dim() else 0
     if not 0 < width < 1 << 31:
         raise ValueError(f"{name} must have rows of 1 to 2^31 - 1 values, got {tuple(t.shape)}")
-    if t.is_contiguous():
-        return t.numel() // width, width, width
-    return (*_rows(t, name), width)
+    rows, stride = (t.numel() // width, width) if t.is_contiguous() else _rows(t, name)
+    if rows >= 1 << 31:
+        raise ValueError(f"{name} must have fewer than 2^31 rows, got {tuple(t.shape)}")
+    return rows, stride, width
 
 
 def _batch_rows(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tensor, name: str) -> tuple[int, int]:

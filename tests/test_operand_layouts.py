@@ -27,3 +27,24 @@ def test_memory_tokens_keep_their_meaning_past_32_bits():
     for memory in (-1, -(1 << 32), -(1 << 31) - 5):
         with pytest.raises(ValueError, match="memory"):
             ew._memory_tokens(memory, 4)
+
+
+@pytest.mark.parametrize("rows,refused", [((1 << 31) - 1, False), (1 << 31, True), ((1 << 32) + 5, True)])
+def test_row_counts_past_a_c_int_are_refused(rows, refused):
+    """The features of a product go to the library as a C int: 2^32 + 5 of them would be taken for 5."""
+    class Rows:
+        is_cuda, shape = True, torch.Size((rows, 16))
+
+        def dim(self):
+            return 2
+
+        def is_contiguous(self):
+            return True
+
+        def numel(self):
+            return 16 * rows
+    if refused:
+        with pytest.raises(ValueError, match="2\\^31 rows"):
+            ew._layout(Rows(), "weight")
+    else:
+        assert ew._layout(Rows(), "weight") == (rows, 16, 16)
