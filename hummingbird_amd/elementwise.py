@@ -18,19 +18,16 @@ from hummingbird_amd.dense_attention import _f32_vector, _require_gpu, dtype_cod
 
 def _rows(t: torch.Tensor, name: str) -> tuple[int, int]:
     """(rows, row stride in elements) of a tensor whose leading axes flatten onto equally spaced rows: contiguous,
-    or a column slice of a wider contiguous tensor."""
+    a column slice of a wider contiguous tensor, or one token of each of its sequences."""
     if t.dim() < 1 or t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit stride on its last axis")
-    rows = t.numel() // t.shape[-1]
-    if t.dim() == 1:
-        return 1, t.shape[-1]
-    stride = t.stride(-2)
-    step = stride
-    for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size > 1 and st != step:
+    axes = [(size, st) for size, st in zip(t.shape[:-1], t.stride()[:-1]) if size != 1]  # (one row's stride is any)
+    stride = step = axes[-1][1] if axes else t.shape[-1]
+    for size, st in reversed(axes):
+        if st != step:
             raise ValueError(f"{name}'s leading axes must flatten onto rows of one stride")
         step *= size
-    return rows, stride
+    return t.numel() // t.shape[-1], stride
 
 
 def dyt(x: torch.Tensor, norm: dict) -> torch.Tensor:

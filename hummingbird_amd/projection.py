@@ -19,23 +19,9 @@ from hummingbird_amd import _lib
 from hummingbird_amd._derived import f32_vector
 from hummingbird_amd.band_attention import pack_dyt
 from hummingbird_amd.dense_attention import _f32, _f32_vector, _require_gpu, dtype_code
-from hummingbird_amd.elementwise import _f32_channels, _layout, _new
+from hummingbird_amd.elementwise import _f32_channels, _layout, _new, _rows
 
 FUSED_DTYPES = (torch.bfloat16, torch.float16)
-
-
-def _rows(t: torch.Tensor, name: str) -> tuple[int, int]:
-    """(rows, row stride) of a tensor whose leading axes flatten onto rows of one stride with unit stride inside."""
-    if t.stride(-1) != 1:
-        raise ValueError(f"{name} must have unit stride on its last axis")
-    rows = t.numel() // t.shape[-1]
-    stride = t.stride(-2) if t.dim() > 1 else t.shape[-1]
-    step = stride
-    for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if size > 1 and st != step:
-            raise ValueError(f"{name}'s leading axes must flatten onto rows of one stride")
-        step *= size
-    return rows, stride
 
 
 def fused_supported(dtype: torch.dtype, num_heads: int, head_dim: int, embed_dim: int, half: int) -> bool:

@@ -48,3 +48,20 @@ def test_row_counts_past_a_c_int_are_refused(rows, refused):
             ew._layout(Rows(), "weight")
     else:
         assert ew._layout(Rows(), "weight") == (rows, 16, 16)
+
+
+def test_rows_of_one_token_per_sequence():
+    """(B, 1, C) slices are B rows of the sequence's stride; the stride of an axis of one element says nothing."""
+    x = torch.zeros(4, 5, 32)
+    wide = torch.zeros(4, 5, 96)
+    for t, rows, stride in ((x, 20, 32), (x[:, -1:], 4, 160), (x[:, 2], 4, 160), (wide[:, 1:2, 32:64], 4, 480),
+                            (wide[..., 32:64], 20, 96), (wide[1:2, 2:3, :32], 1, 32), (x[0, 0], 1, 32),
+                            (wide[2:3, :, 64:], 5, 96), (x.transpose(0, 1)[:, 1:2], 5, 32),
+                            (torch.zeros(32, 1, 1).permute(1, 2, 0), 1, 32)):
+        got = ew._rows(t, "x")
+        assert got == (rows, stride), (tuple(t.shape), t.stride(), got)
+        flat = torch.as_strided(t, (rows, 32), (stride, 1)) if rows > 1 else t.reshape(1, 32)
+        assert flat.data_ptr() == t.data_ptr() and flat.shape[0] * 32 == t.numel()
+    for t in (x.transpose(0, 1), x[:, ::2], wide[:, :3, :32], x.transpose(1, 2)):
+        with pytest.raises(ValueError, match="x"):
+            ew._rows(t, "x")

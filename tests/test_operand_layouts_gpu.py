@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from hummingbird_amd import elementwise as ew
+from hummingbird_amd import projection as pr
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -50,3 +51,29 @@ def test_memory_past_32_bits_is_past_the_end(op):
     assert torch.equal(call(3)[:, :, 0], torch.tensor([[0.0, 0, 0, 1]] * 2, device=DEV))
     with pytest.raises(ValueError):
         call(-(1 << 32))
+
+
+def test_one_token_of_each_sequence():
+    """(B, 1, C) slices through every row operator and both products: as their contiguous copies."""
+    announce("one token of each sequence")
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    wide = torch.randn(3, 5, 256, device=DEV, generator=gen).to(torch.bfloat16)
+    w = torch.rand(128, device=DEV, generator=gen)
+    x, h = wide[:, -1:, :128], wide[:, 1:2, 128:]
+    xc, hc = x.contiguous(), h.contiguous()
+    codes, scales = pr.quantize_q4(torch.randn(48, 128, device=DEV, generator=gen))
+    weight, ws = ew.quantize_rows(torch.randn(48, 128, device=DEV, generator=gen))
+    q, _ = ew.quantize_rows(wide)
+
+    def equal(got, ref):
+        for a, b in zip(got, ref):
+            assert a.shape == b.shape and torch.equal(a.float(), b.float())
+    equal(ew.quantize_rows(x), ew.quantize_rows(xc))
+    equal(ew.rms_modulate_q8(x, w, 1e-5), ew.rms_modulate_q8(xc, w, 1e-5))
+    equal(ew.residual_rms_q8(h, x, w, 1e-5), ew.residual_rms_q8(hc, xc, w, 1e-5))
+    equal(ew.glu_q8(wide[:, 3:4]), ew.glu_q8(wide[:, 3:4].contiguous()))
+    equal([pr.linear_q4(x, codes, scales)], [pr.linear_q4(xc, codes, scales)])
+    token = q[:, -1:, :128]
+    sx = torch.rand(3, 1, device=DEV, generator=gen)
+    equal([pr.linear_q8(token, sx, weight, ws)], [pr.linear_q8(token.contiguous(), sx, weight, ws)])
+    equal([ew.rms_modulate(x, w, 1e-5), ew.gated_residual(h, x)], [ew.rms_modulate(xc, w, 1e-5), ew.gated_residual(hc, xc)])
