@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void row_kernel(const Args<T> a) {
   store_q8<V, CH>(y, a.q + n * a.qs, a.s + n, C, lane, lanes, max_buf);
 }
 
-// The longest row: 16 waves of 64 lanes of CH chunks.
+// The longest row, in registers of 16 waves of 64 lanes: four chunks of fp32 values a lane, two of 16-bit ones.
 constexpr int kMaxC = 16384;
 
 template <typename T, int KIND, int CH>
@@ -307,8 +307,12 @@ void launch(hipStream_t stream, const Args<T>& a) {
   const int chunks = a.C / Vec<T>::N;
   const int64_t waves = a.N * ((chunks + 63) / 64);
   const bool many = KIND != kGlu && chunks > 64 && waves > 32 * static_cast<int64_t>(device_cus());
-  if (chunks > 3 * 64 * kMaxWaves) launch_ch<T, KIND, 4>(stream, a);
-  else if (many || chunks > 64 * kMaxWaves) launch_ch<T, KIND, 3>(stream, a);
+  constexpr int kLanes = 64 * kMaxWaves, kWidest = kMaxC / Vec<T>::N;
+  static_assert(kWidest <= 4 * kLanes, "the widest row has a kernel that holds it");
+  if constexpr (kWidest > 3 * kLanes) {  // fp32
+    if (chunks > 3 * kLanes) return launch_ch<T, KIND, 4>(stream, a);
+  }
+  if (many || chunks > kLanes) launch_ch<T, KIND, 3>(stream, a);
   else launch_ch<T, KIND, 1>(stream, a);
 }
 
