@@ -78,15 +78,23 @@ def pingpong(params: dict, x0: torch.Tensor, schedule: torch.Tensor, noise: torc
     return x, (torch.stack(vs) if trajectory else None)
 
 
+def _held(tree):
+    """`tree` with its dictionaries, lists and tuples copied and everything else shared, so that no tensor in it goes when
+    the caller's own containers change."""
+    if isinstance(tree, dict):
+        return {k: _held(v) for k, v in tree.items()}
+    return type(tree)(_held(v) for v in tree) if type(tree) in (list, tuple) else tree
+
+
 class PingpongGraph:
     """The whole sampler loop for one clip shape as one HIP graph (`torch.cuda.CUDAGraph` on ROCm).
 
-    Built for fixed `(steps, B, io_channels, T)`, weights and per-clip `static` (the graph reads them where they
-    lie, so they must stay alive and unchanged). `__call__(x0, noise)` copies the inputs into the graph's
-    static buffers, replays the graph on the current stream and returns the final latents in the graph's
-    static output buffer (overwritten by the next call: clone it to keep it). The schedule is fixed at
-    construction. Every launch of `pingpong` is recorded: the denoiser's GEMMs and elementwise work, the
-    attention kernels (their workspaces come from `static`), and the sampler arithmetic.
+    Built for fixed `(steps, B, io_channels, T)`, weights and per-clip `static`. The graph reads them where they lie: it
+    holds them (as `params` and `static`), so that their memory stays theirs, and they must stay unchanged.
+    `__call__(x0, noise)` copies the inputs into the graph's static buffers, replays the graph on the current stream and
+    returns the final latents in the graph's static output buffer (overwritten by the next call: clone it to keep it).
+    The schedule is fixed at construction. Every launch of `pingpong` is recorded: the denoiser's GEMMs and elementwise
+    work, the attention kernels (their workspaces come from `static`), and the sampler arithmetic.
     """
 
     def __init__(self, params: dict, static: dict, cfg: DiTConfig, dtype: Dtype, x0: torch.Tensor,
@@ -97,12 +105,13 @@ class PingpongGraph:
         dev = x0.device
         if schedule is None:
             schedule = build_schedule(steps, device=dev)
+        self.params, self.static = _held(params), _held(static)
         self.x0 = x0.to(latent).clone()
         self.noise = noise.to(latent).clone()
         self.schedule = _per_element(schedule.to(dev), x0.shape[0], latent).contiguous()
 
         def run():
-            out, _ = pingpong(params, self.x0, self.schedule, self.noise, static, cfg, dtype, trajectory=False,
+            out, _ = pingpong(self.params, self.x0, self.schedule, self.noise, self.static, cfg, dtype, trajectory=False,
                               projections=projections)
             return out
 
