@@ -186,14 +186,23 @@ _Q8_LAYERS = (("self_attn", "to_qkv"), ("self_attn", "to_out"), ("cross_attn", "
               ("ff", "glu_proj"), ("ff", "proj_out"))
 
 
-def quantize_params(params: dict) -> dict:
+def quantize_params(params: dict, conditioning: str = "q4") -> dict:
     """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
-    rows (`elementwise.quantize_rows`, a scale per output feature) and the timestep and global conditioning layers as
-    4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q8"` and `"q4"` of each layer, and the GLU's
-    bias in fp32 under `"q8_bias"`. The other tensors are shared, not copied. Done once per model, on the weights'
-    device; `prepare_static` then takes the result as its `params`. The layers' input widths must be multiples of 16
-    (8-bit) and 32 (4-bit)."""
+    rows (`elementwise.quantize_rows`, a scale per output feature), under `"q8"` of each layer, and the GLU's bias in
+    fp32 under `"q8_bias"`; with `conditioning="q4"` also the timestep and global conditioning layers as 4-bit weights
+    (`projection.quantize_q4`, with the bias in fp32), under `"q4"`. `conditioning="keep"` leaves those layers on the
+    weights as they are: they are a few rows of work, but every block reads their result, and their 4 bits make most of
+    the error. (Medium width, random weights: the output is 9 %, 19 % and 26 % of its norm off the 16-bit one's at 2, 12
+    and 24 blocks with "q4", 4 %, 9 % and 12 % with "keep"; a render of 1422 tokens takes 44.7 and 45.0 ms.)
+    The other tensors are shared, not copied, and the 16-bit weights stay beside the 8-bit ones. Done once per model, on
+    the weights' device; `prepare_static` then takes the result as its `params`. The layers' input widths must be
+    multiples of 16 (8-bit) and 32 (4-bit)."""
+    if conditioning not in ("q4", "keep"):
+        raise ValueError(f'conditioning must be "q4" or "keep", got {conditioning!r}')
+
     def sequence(seq):
+        if conditioning == "keep":
+            return {k: {n: t for n, t in layer.items() if n != "q4"} for k, layer in seq.items()}
         return {k: {**layer, "q4": (*projection.quantize_q4(layer["weight"]),
                                     None if layer.get("bias") is None else layer["bias"].float())}
                 for k, layer in seq.items()}
@@ -212,7 +221,9 @@ def quantize_params(params: dict) -> dict:
 
 
 def _sequential_q4(seq: dict, x: torch.Tensor) -> torch.Tensor:
-    """`sequential` on 4-bit weights, the activation in the first product's epilogue."""
+    """`sequential` on 4-bit weights where there are any, the activation in the first product's epilogue."""
+    if "q4" not in seq["in"]:
+        return sequential(seq, x)
     return projection.linear_q4(projection.linear_q4(x, *seq["in"]["q4"], silu=True), *seq["out"]["q4"])
 
 
@@ -386,12 +397,12 @@ def dit_forward(params: dict, x: torch.Tensor, t: torch.Tensor, static: dict, cf
                 projections: str = "torch") -> torch.Tensor:
     """One denoiser evaluation (sa3jax/dit.py:340-361): `(B, io_channels, T)` latents and `(B,)` timesteps -> the
     velocity, same shape, in the compute dtype. `static` comes from `prepare_static`. `projections` is passed to
-    `self_attention`, or "q8": the blocks' projections on 8-bit rows and weights and the conditioning layers on 4-bit
-    weights, with `params` (of `static` too) from `quantize_params`; `attention="hip"` only."""
+    `self_attention`, or "q8": the blocks' projections on 8-bit rows and weights and the conditioning layers on the
+    weights that `quantize_params` gave them, with `params` (of `static` too) from it; `attention="hip"` only."""
     net = params["transformer"]
     compute = dtype.compute
     q8 = projections == "q8"
-    if q8 and "q4" not in net["global_cond_embedder"]["in"]:
+    if q8 and any("q8" not in b["ff"]["proj_out"] for b in net["blocks"]):
         raise ValueError('projections="q8" needs the params of quantize_params')
     h = x.to(compute)
     h = conv1x1(h, params["preprocess_conv"]["weight"]) + h
