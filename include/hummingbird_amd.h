@@ -330,7 +330,8 @@ int hb_residual_rms(hipStream_t stream, const void* h, int dtype, int64_t h_row_
  *   (N, K) of `dtype`: w holds two 4-bit codes per byte (OCP e2m1: sign, 2 exponent bits, 1 mantissa bit; the low
  *   nibble the even column), w_scale one e8m0 byte per 32 columns. Every code is exact under the bytes 0 to 252; under
  *   253 and 254 weights of 2^128 and more are infinite, and the byte 255 makes its 32 weights NaN (as in OCP MX). x keeps
- *   all of its bits (fp32: those above 2^-133); sums in fp32; act = SiLU when `silu` != 0, else none; out of `dtype`.
+ *   all of its bits (fp32: those above 2^-133); sums in fp32; act = SiLU when `silu` != 0 (off by up to
+ *   (1.3 |z| + 6) 2^-24 of itself at negative z, zero below -87.3), else none; out of `dtype`.
  *   K a multiple of 32, any N up to 2^16 and F; w row stride (bytes) a multiple of 16, w and x 16-byte aligned, x row
  *   stride a multiple of 8 (bf16, half) or 4 (fp32). */
 int hb_quant_rows(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, void* q, int64_t q_row_stride,

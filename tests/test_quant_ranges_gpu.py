@@ -118,3 +118,24 @@ def test_linear_q4_of_every_scale_byte(name, x):
             ref = (held * value).float().to(dtype)
             assert torch.equal(torch.isnan(got[row]), torch.isnan(ref)), (column, row)
             assert torch.equal(got[row].nan_to_num(0.5), ref.nan_to_num(0.5)), (column, row)
+
+
+def test_linear_q4_silu_over_its_range():
+    """One weight of 1 per feature hands fp32 values to the activation as they are. The exponent's factor (log2(e) to 2^-26
+    of itself) and its product (2^-24) are rounded, which is |z| (2^-24 + 2^-26) of e^-z; the exponential, the sum, the
+    reciprocal and the product add up to 5 further units and the output's half: (1.3 |z| + 6) 2^-24. Where the sigmoid is
+    below 2^-126 it may be zero."""
+    announce("linear_q4 silu range")
+    K = 256
+    codes = torch.zeros(K, K // 2, dtype=torch.uint8, device=DEV)
+    for f in range(K):
+        codes[f, f // 2] = 2 << (4 * (f % 2))  # e2m1 code 2: 1.0
+    scales = torch.full((K, K // 32), 127, dtype=torch.uint8, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.cat([torch.linspace(-90, 90, 4 * K, device=DEV), 100 * (torch.rand(4 * K, device=DEV, generator=gen) - 0.9),
+                   torch.randn(2 * K, device=DEV, generator=gen)]).reshape(-1, K)
+    got = pr.linear_q4(x, codes, scales, silu=True).double()
+    z = x.double()
+    ref = z * torch.sigmoid(z)
+    bound = (1.3 * torch.clamp(-z, min=0) + 6) * 2.0 ** -24 * ref.abs() + z.abs() * 2.0 ** -126
+    assert ((got - ref).abs() <= bound).all()
