@@ -10,9 +10,9 @@
 // of the same MFMA, whose 16 columns a single row leaves empty anyway. Sums are fp32.
 //
 // A workgroup computes 16 to 64 features for up to 64 columns; its waves take the 128-column chunks of K in turns and
-// their partial sums are added in the waves' order. On v_mfma_f32_16x16x32_bf16 a lane holds 8 consecutive columns of feature
-// (or row) lane % 16; which 8 is free as long as both operands agree, so quarter lane / 16 takes columns 32 q + 8 i of
-// the chunk in MFMA i: a lane's 16 bytes of codes are then one scale group, read in one load.
+// their partial sums are added in the waves' order. On v_mfma_f32_16x16x32_bf16 a lane holds 8 consecutive columns of
+// feature (or row) lane % 16; which 8 is free as long as both operands agree, so quarter lane / 16 takes columns
+// 32 q + 8 i of the chunk in MFMA i: a lane's 16 bytes of codes are then one scale group, read in one load.
 #include "api.h"
 #include "common.h"
 
@@ -38,9 +38,9 @@ struct Args {
 };
 
 // Rows of x as bf16 rows whose sum they are: P pieces, each the leading 8 bits of what the earlier ones leave (truncated,
-// so that no piece overflows and every remainder is exact; a bf16 value has no bits below 2^-133). Piece p is x after p times y -= y & 0xffff0000, cut to its
-// upper half: a lane holds the masks of its piece, zero past it. An infinity or NaN leaves NaNs in the later pieces;
-// what counts then is the first one's sum (see the end of the kernel).
+// so that no piece overflows and every remainder is exact; a bf16 value has no bits below 2^-133). Piece p is x after p
+// times y -= y & 0xffff0000, cut to its upper half: a lane holds the masks of its piece, zero past it. An infinity or NaN
+// leaves NaNs in the later pieces; what counts then is the first one's sum (see the end of the kernel).
 template <typename T>
 struct Pieces;
 template <>
@@ -226,7 +226,8 @@ __global__ __launch_bounds__(64 * max_waves(CT * FT)) void q4_kernel(const Args 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float z = v[j] + bias[t][j];
-        if (a.silu)  // relative error up to (1.3 |z| + 6) 2^-24 for negative z (the exponent is rounded first), zero below -87.3
+        // off by up to (1.3 |z| + 6) 2^-24 of itself for negative z (the exponent is rounded first), zero below -87.3
+        if (a.silu)
           z = z * __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z));
         y[j] = cast_out<T>(z);
       }

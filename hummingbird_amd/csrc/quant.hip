@@ -300,10 +300,10 @@ void launch_ch(hipStream_t stream, const Args<T>& a) {
   hipLaunchKernelGGL((row_kernel<T, KIND, CH>), grid, dim3((lanes + 63) / 64 * 64), 0, stream, a);
 }
 
-// One chunk per lane is quickest while the card holds all waves at once (residual_rms_q8, bf16: 1292 x 1536 6.1 us against
-// 7.6 with three), and for the GLU, whose lanes have two loads each anyway (5168 x 6144: 31.9 against 34.5); beyond that
-// three (5168 x 1536: 13.7 against 14.6, 1000 x 8192: 14.6 against 16.4, fp32 rms_modulate_q8 on 8249 x 1024: 12.2 against
-// 13.8). Wider rows take what holds them.
+// One chunk per lane is quickest while the card holds all waves at once (residual_rms_q8, bf16: 1292 x 1536 5.9 us against
+// 7.4 with three), and for the GLU, whose lanes have two loads each anyway (5168 x 6144: 34.5 against 37.5); beyond that
+// three (5168 x 1536: 14.6 against 15.4, 1000 x 8192: 15.2 against 17.2, fp32 rms_modulate_q8 on 8249 x 1024: 13.2 against
+// 14.6, quantize_rows on 5168 x 1536: 6.5 against 6.9). Wider rows take what holds them.
 template <typename T, int KIND>
 void launch(hipStream_t stream, const Args<T>& a) {
   const int chunks = a.C / Vec<T>::N;
