@@ -60,6 +60,9 @@ def parse() -> argparse.Namespace:
     ap.add_argument("--sampler-only", action="store_true",
                     help="instead of the clip benchmark: the whole 120 s render of the medium DiT (8 pingpong steps "
                          "x 24 blocks, eager and as one HIP graph), one JSON line; for profiling under rocprofv3")
+    ap.add_argument("--q8", choices=("q4", "keep"),
+                    help="with --sampler-only: the render on 8-bit rows and weights, its conditioning layers on 4-bit "
+                         "weights or kept on 16-bit ones")
     ap.add_argument("--decoder-only", action="store_true",
                     help="instead of the clip benchmark: the SAME-L decoder's 12 blocks for a 120 s clip at the "
                          "reference's decoder geometry, chained and block by block, one JSON line; for profiling")
@@ -259,18 +262,21 @@ def extra_shapes(lib, sp, stream, dev) -> dict:
     res["same_l_decoder_120s"] = decoder_shape(dev, gen)
     res["dit_self_attention_120s"] = dit_self_attention_shape(stream, dev, gen)
     res["sampler_120s"] = sampler_shape(dev)
+    res["sampler_120s_q8"] = {c: sampler_shape(dev, conditioning=c) for c in ("q4", "keep")}
     # the matrix cores' data dependence: what the dense kernel's roofline fraction is measured against in practice
     res["mfma_ceiling"] = ceiling_summary(lib, sp, stream, dev)
     return res
 
 
-def sampler_shape(dev, tune: bool = True) -> dict:
+def sampler_shape(dev, tune: bool = True, conditioning: str | None = None) -> dict:
     """The whole denoising of one 120 s clip as the reference renders it: the `medium` DiT (24 blocks, width 1536,
     24 heads; random weights), batch 1, 1358 latents + 64 memory tokens (L = 1422), a 257-token context, 8 pingpong
     steps, bf16, attention="hip" (192 dense self-attention and 192 cross-attention calls). Per-clip state from
     `dit.prepare_static` (not timed); then ms per clip for the eager loop and for the loop captured as one HIP
     graph (median of 3 each), and for the graph again after `sampling.tune_gemms` has let PyTorch's TunableOp pick
-    each GEMM's solution (the tuning itself is not timed; TunableOp is switched off again afterwards)."""
+    each GEMM's solution (the tuning itself is not timed; TunableOp is switched off again afterwards). `conditioning`
+    ("q4" or "keep") times the denoiser on 8-bit rows and weights instead (`dit.quantize_params(params, conditioning)`,
+    `projections="q8"`), which has no GEMMs of the vendor's left to tune in its blocks."""
     import torch
 
     from hummingbird_amd import dit, sampling
@@ -280,6 +286,9 @@ def sampler_shape(dev, tune: bool = True) -> dict:
     cfg, T, steps = MEDIUM_DIT, 1358, SAMPLER_STEPS
     gen = torch.Generator(device=dev).manual_seed(11)
     params = dit.init_params(cfg, BF16, device=dev, seed=11)
+    projections = "torch" if conditioning is None else "q8"
+    if conditioning is not None:
+        params = dit.quantize_params(params, conditioning)
     cond = {"cross_attn_cond": torch.randn((1, 257, cfg.cond_token_dim), device=dev, generator=gen),
             "global_cond": torch.randn((1, cfg.global_cond_dim), device=dev, generator=gen)}
     mask = torch.ones((1, T), dtype=torch.bool, device=dev)
@@ -301,15 +310,16 @@ def sampler_shape(dev, tune: bool = True) -> dict:
             times.append(a.elapsed_time(b))
         return round(float(np.median(times)), 2)
     def eager_clip():
-        return sampling.pingpong(params, x0, schedule, noise, static, cfg, BF16, trajectory=False)
+        return sampling.pingpong(params, x0, schedule, noise, static, cfg, BF16, trajectory=False,
+                                 projections=projections)
     eager = clip_ms(eager_clip)
-    graph = sampling.PingpongGraph(params, static, cfg, BF16, x0, noise)
+    graph = sampling.PingpongGraph(params, static, cfg, BF16, x0, noise, projections=projections)
     replay = clip_ms(lambda: graph(x0, noise))
     del graph
     shape = {"B": 1, "latents": T, "L": T + cfg.num_memory_tokens, "context": 257, "depth": cfg.depth,
              "E": cfg.embed_dim, "H": cfg.num_heads, "steps": steps}
     calls = {"dense": steps * cfg.depth, "cross": steps * cfg.depth}
-    if not tune:
+    if not tune or conditioning is not None:
         return {"shape": shape, "eager_ms_per_clip": eager, "graph_ms_per_clip": replay,
                 "attention_calls_per_clip": calls}
     # GEMM solutions chosen per shape by PyTorch's TunableOp (tuning untimed), then the graph captured again
@@ -696,6 +706,9 @@ def main() -> int:
         ceiling(lib, sp, stream, dev)
         return 0
     if args.sampler_only:
+        if args.q8 is not None:
+            print(json.dumps({"sampler_120s_q8": {args.q8: sampler_shape(dev, conditioning=args.q8)}}), flush=True)
+            return 0
         print(json.dumps({"sampler_120s": sampler_shape(dev, tune=not args.no_tune)}), flush=True)
         return 0
     if args.decoder_only:
