@@ -76,8 +76,8 @@ def residual_dyt(h: torch.Tensor, x: torch.Tensor, bias: torch.Tensor | None = N
     dtype, and with `norm` (DyT params) the DyT of the sum cast back, the next GEMM's input. `x` is the bare
     projection output; `bias` (C values) may be None. Without `norm` the second result is None."""
     _require_gpu(h, "h")
-    if h.shape != x.shape or h.dtype != x.dtype:
-        raise ValueError(f"h {tuple(h.shape)} {h.dtype} and x {tuple(x.shape)} {x.dtype} must match")
+    if h.shape != x.shape or h.dtype != x.dtype or h.device != x.device:
+        raise ValueError(f"h {tuple(h.shape)} {h.dtype} {h.device} and x {tuple(x.shape)} {x.dtype} {x.device} must match")
     channels = h.shape[-1]
     rows, hs = _rows(h, "h")
     _, xs = _rows(x, "x")
@@ -98,13 +98,15 @@ def residual_dyt(h: torch.Tensor, x: torch.Tensor, bias: torch.Tensor | None = N
     return out_h, out_y
 
 
-def _per_batch(t: torch.Tensor | None, batch: int, channels: int, dtype: torch.dtype, name: str):
-    """(pointer, batch stride) of a `(B, C)` (or `(B, 1, C)`) per-batch row tensor in `dtype`, possibly a view into a
-    wider row (the adaLN chunks of `(B, 6 E)`); (0, 0) for None."""
+def _per_batch(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tensor, name: str):
+    """(pointer, batch stride) of a `(B, C)` (or `(B, 1, C)`) per-batch row tensor of `x`'s dtype and device, possibly a
+    view into a wider row (the adaLN chunks of `(B, 6 E)`); (0, 0) for None."""
     if t is None:
         return 0, 0
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on {x.device}, got {t.device}")
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {x.dtype}")
     t2 = t.reshape(t.shape[0], t.shape[-1]) if t.dim() == 3 and t.shape[1] == 1 else t
     if t2.dim() != 2 or tuple(t2.shape) != (batch, channels) or t2.stride(-1) != 1:
         raise ValueError(f"{name} must be (B, C) = ({batch}, {channels}) with unit stride on C, got {tuple(t.shape)}")
@@ -145,8 +147,8 @@ def rms_modulate(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: torch
         raise ValueError(f"weight must have {channels} elements")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift are given together or not at all")
-    sp, ms = _per_batch(scale, batch, channels, x.dtype, "scale")
-    hp, ms2 = _per_batch(shift, batch, channels, x.dtype, "shift")
+    sp, ms = _per_batch(scale, batch, channels, x, "scale")
+    hp, ms2 = _per_batch(shift, batch, channels, x, "shift")
     if scale is not None and ms != ms2:
         raise ValueError("scale and shift must share their batch stride")
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -164,12 +166,13 @@ def gated_residual(h: torch.Tensor, x: torch.Tensor, gate: torch.Tensor | None =
     `gate`, then `+ local` on the tokens at or past `memory` (sa3jax/dit.py:237-241); each step in `h.dtype`.
     `gate` is `(B, C)`, `x_bias` and `local` `(C,)`. One pass (`hb_gated_residual`)."""
     _require_gpu(h, "h")
-    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype:
-        raise ValueError(f"h and x must be (B, L, C) of one shape and dtype, got {tuple(h.shape)}, {tuple(x.shape)}")
+    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
+        raise ValueError(f"h and x must be (B, L, C) of one shape, dtype and device, got {tuple(h.shape)} {h.dtype} "
+                         f"{h.device}, {tuple(x.shape)} {x.dtype} {x.device}")
     batch, length, channels = h.shape
     _, hs = _rows(h, "h")
     rows, xs = _rows(x, "x")
-    gp, gs = _per_batch(gate, batch, channels, h.dtype, "gate")
+    gp, gs = _per_batch(gate, batch, channels, h, "gate")
     bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
     out = torch.empty(h.shape, dtype=h.dtype, device=h.device)
     stream = _lib.current_stream(h.device)
@@ -188,16 +191,17 @@ def residual_rms(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: fl
     returns `(h', norm(h'))`, the same values as the two calls. A DiT block's residuals each feed the next norm
     (sa3jax/dit.py:234-236, 237-247, 249-251 into the next block's 231-233)."""
     _require_gpu(h, "h")
-    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype:
-        raise ValueError(f"h and x must be (B, L, C) of one shape and dtype, got {tuple(h.shape)}, {tuple(x.shape)}")
+    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
+        raise ValueError(f"h and x must be (B, L, C) of one shape, dtype and device, got {tuple(h.shape)} {h.dtype} "
+                         f"{h.device}, {tuple(x.shape)} {x.dtype} {x.device}")
     batch, length, channels = h.shape
     _, hs = _rows(h, "h")
     rows, xs = _rows(x, "x")
-    gp, gs = _per_batch(gate, batch, channels, h.dtype, "gate")
+    gp, gs = _per_batch(gate, batch, channels, h, "gate")
     if (scale is None) != (shift is None):
         raise ValueError("scale and shift are given together or not at all")
-    sp, ms = _per_batch(scale, batch, channels, h.dtype, "scale")
-    hp, ms2 = _per_batch(shift, batch, channels, h.dtype, "shift")
+    sp, ms = _per_batch(scale, batch, channels, h, "scale")
+    hp, ms2 = _per_batch(shift, batch, channels, h, "shift")
     if scale is not None and ms != ms2:
         raise ValueError("scale and shift must share their batch stride")
     w = weight.to(device=h.device, dtype=torch.float32).contiguous().reshape(-1)
@@ -249,7 +253,7 @@ def _batch_rows(t: torch.Tensor | None, batch: int, channels: int, x: torch.Tens
         step, unit = t.stride()
         if unit == 1:
             return t.data_ptr(), (step if batch > 1 else channels)
-    return _per_batch(t, batch, channels, x.dtype, name)
+    return _per_batch(t, batch, channels, x, name)
 
 
 def _f32_channels(t: torch.Tensor, channels: int, device: torch.device, name: str) -> torch.Tensor:

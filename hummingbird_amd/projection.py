@@ -170,8 +170,9 @@ def residual_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | 
     f, k = w.shape
     if x.shape[-1] != k:
         raise ValueError(f"x has {x.shape[-1]} columns, weight {k}")
-    if h.shape[:-1] != x.shape[:-1] or h.shape[-1] != f or h.dtype != x.dtype:
-        raise ValueError(f"h must be {(*x.shape[:-1], f)} of {x.dtype}, got {tuple(h.shape)} {h.dtype}")
+    if h.shape[:-1] != x.shape[:-1] or h.shape[-1] != f or h.dtype != x.dtype or h.device != x.device:
+        raise ValueError(f"h must be {(*x.shape[:-1], f)} of {x.dtype} on {x.device}, got {tuple(h.shape)} {h.dtype} on "
+                         f"{h.device}")
     _, hs = _rows(h, "h")
     bias_p = 0
     if bias is not None:

@@ -65,3 +65,14 @@ def test_rows_of_one_token_per_sequence():
     for t in (x.transpose(0, 1), x[:, ::2], wide[:, :3, :32], x.transpose(1, 2)):
         with pytest.raises(ValueError, match="x"):
             ew._rows(t, "x")
+
+
+def test_batch_rows_of_another_device_are_refused():
+    x = torch.zeros(2, 3, 16)
+    rows = torch.zeros(2, 96)
+    assert ew._per_batch(rows[:, 16:32], 2, 16, x, "gate") == (rows.data_ptr() + 64, 96)
+    assert ew._per_batch(None, 2, 16, x, "gate") == (0, 0)
+    with pytest.raises(ValueError, match="gate must be on"):
+        ew._per_batch(torch.zeros(2, 16, device="meta"), 2, 16, x, "gate")
+    with pytest.raises(TypeError):
+        ew._per_batch(torch.zeros(2, 16).double(), 2, 16, x, "gate")

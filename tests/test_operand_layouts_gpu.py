@@ -77,3 +77,20 @@ def test_one_token_of_each_sequence():
     sx = torch.rand(3, 1, device=DEV, generator=gen)
     equal([pr.linear_q8(token, sx, weight, ws)], [pr.linear_q8(token.contiguous(), sx, weight, ws)])
     equal([ew.rms_modulate(x, w, 1e-5), ew.gated_residual(h, x)], [ew.rms_modulate(xc, w, 1e-5), ew.gated_residual(hc, xc)])
+
+
+def test_operands_on_the_host_are_refused():
+    """A host tensor's address means nothing to a kernel: every operand that goes to it as it is has to be on the rows'
+    device. (Parameters that the wrappers convert, such as norm weights, are moved.)"""
+    announce("host operands")
+    h = torch.zeros(2, 3, 256, device=DEV, dtype=torch.bfloat16)
+    w, host = torch.ones(256, device=DEV), torch.zeros(2, 256, dtype=torch.bfloat16)
+    for call in (lambda: ew.rms_modulate(h, w, 1e-5, host, host), lambda: ew.gated_residual(h, h, gate=host),
+                 lambda: ew.gated_residual(h, h.cpu()), lambda: ew.residual_rms(h, h.cpu(), w, 1e-5),
+                 lambda: ew.residual_rms(h, h, w, 1e-5, gate=host), lambda: ew.residual_dyt(h, h.cpu()),
+                 lambda: ew.residual_rms(h, h, w, 1e-5, scale=host, shift=host),
+                 lambda: ew.rms_modulate_q8(h, w, 1e-5, host, host), lambda: ew.residual_rms_q8(h, h, w, 1e-5, gate=host),
+                 lambda: ew.residual_rms_q8(h, h.cpu(), w, 1e-5), lambda: ew.residual_rms_q8(h, h, w, 1e-5, local=host[0]),
+                 lambda: pr.residual_linear(h, torch.zeros(256, 256, dtype=torch.bfloat16, device=DEV), None, h.cpu())):
+        with pytest.raises(ValueError):
+            call()
