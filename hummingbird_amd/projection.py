@@ -218,10 +218,11 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weig
     if weight.device != dev or x_scale.device != dev or weight_scale.device != dev:
         raise ValueError(f"weight and the scales must be on {dev}, got {weight.device}, {x_scale.device}, "
                          f"{weight_scale.device}")
-    if x_scale.shape != x.shape[:-1] or not x_scale.is_contiguous():
-        raise ValueError(f"x_scale must be contiguous {tuple(x.shape[:-1])}, got {tuple(x_scale.shape)}")
-    if weight_scale.shape != (f,) or not weight_scale.is_contiguous():
-        raise ValueError(f"weight_scale must be contiguous ({f},), got {tuple(weight_scale.shape)}")
+    if x_scale.shape != x.shape[:-1]:
+        raise ValueError(f"x_scale must be {tuple(x.shape[:-1])}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != (f,):
+        raise ValueError(f"weight_scale must be ({f},), got {tuple(weight_scale.shape)}")
+    x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()  # (a slice's scales: copied)
     bp = 0
     if bias is not None:
         bias = _f32_channels(bias, f, dev, "bias")

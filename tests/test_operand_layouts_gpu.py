@@ -94,3 +94,19 @@ def test_operands_on_the_host_are_refused():
                  lambda: pr.residual_linear(h, torch.zeros(256, 256, dtype=torch.bfloat16, device=DEV), None, h.cpu())):
         with pytest.raises(ValueError):
             call()
+
+
+def test_linear_q8_takes_the_scales_of_a_slice():
+    """The rows, their scales and the features of slices: (B, L) scales' last tokens lie L apart."""
+    announce("scales of slices")
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    q, s = ew.quantize_rows(torch.randn(3, 5, 64, device=DEV, generator=gen))
+    w, ws = ew.quantize_rows(torch.randn(40, 64, device=DEV, generator=gen))
+    whole = pr.linear_q8(q, s, w, ws)
+    assert torch.equal(pr.linear_q8(q[:, -1:], s[:, -1:], w, ws), whole[:, -1:])
+    assert torch.equal(pr.linear_q8(q[:, 2], s[:, 2], w, ws), whole[:, 2])
+    assert torch.equal(pr.linear_q8(q, s, w[::2], ws[::2]), whole[..., ::2])
+    assert torch.equal(pr.linear_q8(q[:1], s[:1, 0, None].expand(1, 5) * 0 + s[:1], w, ws), whole[:1])
+    for bad in (s[:, :, None], s[:, 1:], s[0]):
+        with pytest.raises(ValueError, match="x_scale"):
+            pr.linear_q8(q, bad, w, ws)
