@@ -194,9 +194,10 @@ def quantize_params(params: dict, conditioning: str = "q4") -> dict:
     weights as they are: they are a few rows of work, but every block reads their result, and their 4 bits make most of
     the error. (Medium width, random weights: the output is 9 %, 19 % and 26 % of its norm off the 16-bit one's at 2, 12
     and 24 blocks with "q4", 4 %, 9 % and 12 % with "keep"; a render of 1422 tokens takes 44.7 and 45.0 ms.)
-    The other tensors are shared, not copied, and the 16-bit weights stay beside the 8-bit ones. Done once per model, on
-    the weights' device; `prepare_static` then takes the result as its `params`. The layers' input widths must be
-    multiples of 16 (8-bit) and 32 (4-bit)."""
+    The other tensors are shared, not copied. The 16-bit weights stay beside the 8-bit ones (2.4 and 1.2 GB of the medium
+    model), so that the other `projections` still run; where only "q8" does, the `"weight"` entries of the layers that
+    have a `"q8"` may be deleted before `prepare_static`. Done once per model, on the weights' device; `prepare_static`
+    then takes the result as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
     if conditioning not in ("q4", "keep"):
         raise ValueError(f'conditioning must be "q4" or "keep", got {conditioning!r}')
 

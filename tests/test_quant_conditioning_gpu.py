@@ -159,3 +159,26 @@ def test_kept_conditioning_in_a_graph_and_refusals():
         dit.quantize_params(params, conditioning="q8")
     with pytest.raises(ValueError, match="quantize_params"):
         dit.dit_forward(params, x, torch.tensor([0.5], device=DEV), static, MEDIUM2, BF16, projections="q8")
+
+
+@pytest.mark.parametrize("conditioning", ["q4", "keep"])
+def test_16_bit_weights_can_be_let_go(conditioning):
+    """The "q8" path reads no `weight` of a layer that has a `q8`: without them it gives the same bits."""
+    announce("denoiser without the 16-bit weights", conditioning)
+    params, cond, mask, x = case(MEDIUM2, BF16, 1, 100, seed=43, ctx_tokens=257)
+    quantized = dit.quantize_params(params, conditioning=conditioning)
+    t = torch.tensor([0.5], device=DEV)
+    ref = dit.dit_forward(quantized, x, t, dit.prepare_static(quantized, cond, mask, MEDIUM2, BF16), MEDIUM2, BF16,
+                          projections="q8")
+    deleted = 0
+    for block in quantized["transformer"]["blocks"]:
+        for part in block.values():
+            for layer in part.values() if isinstance(part, dict) else ():
+                if isinstance(layer, dict) and "q8" in layer:
+                    del layer["weight"]
+                    deleted += 1
+    assert deleted == 6 * MEDIUM2.depth
+    assert "weight" in params["transformer"]["blocks"][0]["ff"]["proj_out"]  # the caller's own stay
+    got = dit.dit_forward(quantized, x, t, dit.prepare_static(quantized, cond, mask, MEDIUM2, BF16), MEDIUM2, BF16,
+                          projections="q8")
+    assert torch.equal(got, ref)
