@@ -94,7 +94,8 @@ class PingpongGraph:
     `__call__(x0, noise)` copies the inputs into the graph's static buffers, replays the graph on the current stream and
     returns the final latents in the graph's static output buffer (overwritten by the next call: clone it to keep it).
     The schedule is fixed at construction. Every launch of `pingpong` is recorded: the denoiser's GEMMs and elementwise
-    work, the attention kernels (their workspaces come from `static`), and the sampler arithmetic.
+    work, the attention kernels (their workspaces come from `static`: graphs of one `static` may not run at once), and
+    the sampler arithmetic.
     """
 
     def __init__(self, params: dict, static: dict, cfg: DiTConfig, dtype: Dtype, x0: torch.Tensor,
