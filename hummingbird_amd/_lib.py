@@ -86,6 +86,21 @@ SIGNATURES = {
                            c_int, c_int64, c_int64, c_int, c_int]),
     "hb_proj_q4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
                            c_void_p, c_int64, c_int, c_int, c_int]),
+    "hb_quant_rows_mx4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                  c_int]),
+    "hb_rms_modulate_mx4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p, c_void_p, c_int64,
+                                    c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int]),
+    "hb_residual_rms_mx4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                    c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                    c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int]),
+    "hb_glu_mx4": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                           c_int]),
+    "hb_proj_mx4": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                            c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int]),
+    "hb_packed_workspace_size": (c_size_t, [c_int, c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    "hb_packed_attention": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                                    c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_float, c_void_p, c_int64,
+                                    c_int64, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_size_t]),
 }
 
 _lib: ctypes.CDLL | None = None

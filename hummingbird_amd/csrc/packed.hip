@@ -1,0 +1,651 @@
+// Attention over packed sequences for gfx950 (MI355X): queries of N sequences one after the other in q, the keys of each in
+// k and v, H heads of queries to G of keys.
+//
+//   out[t, h] = sum_b softmax_b(scale q[t, h] . k[b, h / gs]) v[b, h / gs],   gs = H / G,
+//
+// over the keys b of t's sequence, those at or before t's place at the end of them when `causal`. A row with no key is zero.
+//
+// A workgroup computes a tile of rows of one sequence for one head of keys; a row is one query's one head, the gs heads that
+// share the keys next to each other, so that a tile reads its keys once whatever gs is and one new token fills gs rows.
+// Keys pass through LDS in tiles of KT, two stages, by global_load_lds; a wave holds 32 NCT rows as MFMA columns:
+//   S^T = K Q^T, P = exp2(c S^T - m) with the running maximum m, O^T += V^T P^T,
+// so that the probabilities go from the accumulators of S^T into the operands of O^T as they are (attn_tile.h), and
+// statistics are a lane's own but for the exchange with its other half. 16-bit inputs multiply on their own type's cores,
+// with P rounded to it (its sum is of the rounded values); fp32 on the fp32 cores with P in fp32. Statistics and sums are fp32.
+//
+// The lengths are read on the device: the grid has a slot for every tile that the rows could need (a sequence wastes less
+// than one), and each workgroup finds its sequence in the offsets; no launch waits for the host to know them.
+#include <cmath>
+#include <type_traits>
+
+#include "api.h"
+#include "attn_tile.h"
+#include "common.h"
+#include "tiles.h"
+
+namespace hb {
+namespace packed {
+
+struct Args {
+  const uint8_t *q, *k, *v;                    // strides in bytes, of tokens and of heads
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  uint8_t* out;
+  int64_t o_ts, o_hs;
+  const int *off, *koff, *klen;                // N + 1 offsets of queries and of keys; N lengths of keys, or null
+  int causal, zero_rest;
+  float c;                                     // scale log2(e)
+  int T, Tk, N, H, G, gs;
+  int slots, splits;                           // tiles of rows, parts of the keys
+  float* part_o;                               // splits > 1: (splits, T, H, D) sums, not yet divided
+  float* part_ml;                              // and (splits, T, H, 2) maxima and totals
+};
+
+// The element type's arithmetic. KT: keys per LDS tile.
+template <class IO>
+struct E16 {
+  static constexpr int ES = 2, KT = 64;
+  using Io = IO;
+};
+struct E32 {
+  static constexpr int ES = 4, KT = 32;
+};
+
+__device__ __forceinline__ int clamp_to(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+struct Tile {
+  bool found;
+  int index;       // of the sequence's tiles, or of the slots without one
+  int idle;        // slots without a tile
+  int q0, lq;      // the sequence's first query and queries
+  int k0, lk;      // and keys
+};
+
+// Slot u's tile of R rows. Lane i of a wave looks at sequence 64 n + i.
+__device__ __forceinline__ Tile find_tile(const Args& a, int u, int R) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int i0 = 0; i0 < a.N; i0 += 64) {
+    const int i = i0 + lane;
+    int q0 = 0, lq = 0;
+    if (i < a.N) {
+      q0 = clamp_to(a.off[i], 0, a.T);
+      lq = clamp_to(a.off[i + 1], q0, a.T) - q0;
+    }
+    const int tiles = static_cast<int>((static_cast<int64_t>(lq) * a.gs + R - 1) / R);
+    int upto = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(upto, d, kWave);
+      if (lane >= d) upto += x;
+    }
+    const uint64_t past = __ballot(before + upto > u);
+    if (past) {
+      const int who = __ffsll(static_cast<unsigned long long>(past)) - 1;
+      Tile t;
+      t.found = true;
+      const int seq = __builtin_amdgcn_readfirstlane(i0 + who);
+      t.q0 = __builtin_amdgcn_readfirstlane(__shfl(q0, who, kWave));
+      t.lq = __builtin_amdgcn_readfirstlane(__shfl(lq, who, kWave));
+      const int n = __builtin_amdgcn_readfirstlane(__shfl(tiles, who, kWave));
+      t.index = u - before - (__builtin_amdgcn_readfirstlane(__shfl(upto, who, kWave)) - n);
+      if (a.causal) t.index = n - 1 - t.index;  // the longest first
+      t.k0 = clamp_to(a.koff[seq], 0, a.Tk);
+      t.lk = clamp_to(a.koff[seq + 1], t.k0, a.Tk) - t.k0;
+      if (a.klen) t.lk = clamp_to(a.klen[seq], 0, t.lk);
+      t.idle = 0;
+      return t;
+    }
+    before += __builtin_amdgcn_readfirstlane(__shfl(upto, 63, kWave));
+  }
+  return Tile{false, u - before, a.slots - before, 0, 0, 0, 0};
+}
+
+// Byte of logical 16-byte chunk `chunk` of row `row` of a K or V tile, such that the reads spread over the banks: K's of one
+// chunk of 32 consecutive rows; V's, transposing ones of 64 bytes of 8 rows or (fp32) of 128 bytes of rows 4 apart.
+template <class E, int D>
+__device__ __forceinline__ int k_byte(int row, int chunk) {
+  constexpr int RB = D * E::ES;
+  if constexpr (RB == 128) return row * RB + 16 * (chunk ^ (row & 7) ^ ((row >> 3) & 1));
+  else return row * RB + 16 * (chunk ^ (row & 15));
+}
+template <class E, int D>
+__device__ __forceinline__ int v_chunk(int row, int chunk) {
+  if constexpr (E::ES == 4) return chunk ^ (8 * ((row >> 2) & 1));
+  else if constexpr (D == 64) return chunk ^ (4 * ((row >> 1) & 1));
+  else return chunk ^ (4 * (row & 3));
+}
+
+template <class E, int D>
+struct Lds {
+  static constexpr int kTile = E::KT * D * E::ES;  // bytes of a K or a V tile
+  static constexpr int kStage = 2 * kTile;
+};
+
+// The copies of a key tile by one of NW waves: 1 KB blocks wv, wv + NW, ... of K, then of V.
+template <class E, int D, int NW>
+struct KeyCopy {
+  static constexpr int RB = D * E::ES, kRows = 1024 / RB, kBlocks = E::KT * RB / 1024 / NW;
+  static constexpr int kCopies = 2 * kBlocks;
+  const uint8_t *k, *v;
+  uint32_t koff[kBlocks], voff[kBlocks];
+  int lk;
+  int64_t k_ts, v_ts;
+
+  __device__ __forceinline__ int row(int u) const {
+    return kRows * (wave_id() % NW + NW * u) + (threadIdx.x & 63) / (64 / kRows);
+  }
+  __device__ __forceinline__ void offsets(int u, int r, uint32_t& ko, uint32_t& vo) const {
+    const int chunk = threadIdx.x & (64 / kRows - 1), at = row(u);
+    ko = static_cast<uint32_t>(r * k_ts) + (k_byte<E, D>(at, chunk) - at * RB);
+    vo = static_cast<uint32_t>(r * v_ts) + 16 * v_chunk<E, D>(at, chunk);
+  }
+  __device__ __forceinline__ KeyCopy(const Args& a, const Tile& t, int g)
+      : k(a.k + t.k0 * a.k_ts + g * a.k_hs), v(a.v + t.k0 * a.v_ts + g * a.v_hs), lk(t.lk), k_ts(a.k_ts), v_ts(a.v_ts) {
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) offsets(u, row(u), koff[u], voff[u]);
+  }
+  // The keys from k0 on into the stage at LDS byte address `stage`; past the last key, that one again (it is masked).
+  __device__ __forceinline__ void operator()(int k0, uint32_t stage) const {
+    const uint8_t *kb = k + k0 * k_ts, *vb = v + k0 * v_ts;
+    const int wv = wave_id() % NW;
+    const bool whole = k0 + E::KT <= lk;
+#pragma unroll
+    for (int u = 0; u < kBlocks; ++u) {
+      uint32_t ko = koff[u], vo = voff[u];
+      if (!whole) {
+        const int r = row(u), last = lk - 1 - k0;
+        offsets(u, r < last ? r : last, ko, vo);
+      }
+      lds_dma16(kb, ko, stage + (wv + NW * u) * 1024);
+      lds_dma16(vb, vo, stage + Lds<E, D>::kTile + (wv + NW * u) * 1024);
+    }
+  }
+};
+
+template <class IO>
+__device__ __forceinline__ float add_pair(uint32_t p, float acc);
+template <>
+__device__ __forceinline__ float add_pair<Bf16Io>(uint32_t p, float acc) { return add_bf16_pair(p, acc); }
+template <>
+__device__ __forceinline__ float add_pair<F16Io>(uint32_t p, float acc) {
+  const uint32_t ones = 0x3c003c00u;
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, ones), acc, false);
+}
+
+// V^T for dims 32 dt + lr and keys {16 g + 8 (j / 4) + 4 lh + j % 4 : j < 8}, by transposing reads (attn_tile.h's v_frag on
+// swizzled rows).
+template <class E, int D>
+__device__ __forceinline__ u32x4 v_operand(const uint8_t* sV, int dt, int g) {
+  const int lane = threadIdx.x & 63, grp = lane >> 4, m = lane & 15;
+  const int row = 16 * g + 4 * (grp >> 1) + (m >> 2), chunk = 4 * dt + 2 * (grp & 1) + ((m & 3) >> 1);
+  const uint8_t* p = sV + row * (2 * D) + 8 * (m & 1);
+  lds_i16x4* p0 = (lds_i16x4*)(p + 16 * v_chunk<E, D>(row, chunk));
+  lds_i16x4* p1 = (lds_i16x4*)(p + 8 * (2 * D) + 16 * v_chunk<E, D>(row + 8, chunk));
+  const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p0);
+  const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p1);
+  const u32x2 ux = __builtin_bit_cast(u32x2, x), uy = __builtin_bit_cast(u32x2, y);
+  return u32x4{ux[0], ux[1], uy[0], uy[1]};
+}
+
+// The rows of a wave: what it holds between key tiles.
+template <class E, int D, int NCT>
+struct Rows {
+  static constexpr int RT = E::KT / 32, kQ = D * E::ES / 32;  // 16-byte pieces of a query per lane
+  u32x4 q[NCT][kQ];
+  f32x16 o[NCT][D / 32];
+  float m[NCT], l[NCT];
+  int lim[NCT];  // keys that this lane's row sees
+
+  // One key tile; `masked`: some row does not see all of its KT keys from k0 on.
+  // `apart`: V's NaNs and infinities reach only the rows that see their keys.
+  __device__ __forceinline__ void step(const uint8_t* sK, const uint8_t* sV, int k0, float c, bool masked, bool apart) {
+    const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
+    f32x16 sc[NCT][RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int ct = 0; ct < NCT; ++ct) sc[ct][rt] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(sK + k_byte<E, D>(32 * rt + lr, 2 * i + lh));
+#pragma unroll
+        for (int ct = 0; ct < NCT; ++ct) {
+          if constexpr (E::ES == 2) {
+            sc[ct][rt] = mfma_io_32x32x16<typename E::Io>(kf, q[ct][i], sc[ct][rt]);
+          } else {
+            const f32x4 x = __builtin_bit_cast(f32x4, kf), y = __builtin_bit_cast(f32x4, q[ct][i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[ct][rt] = mfma_f32_32x32x2(x[j], y[j], sc[ct][rt]);
+          }
+        }
+      }
+    }
+    u32x4 p[NCT][RT][2];  // 16-bit probabilities; fp32 ones stay in sc
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      if (masked) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            sc[ct][rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[ct][rt][r] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[ct][rt][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c;
+      const float mn = fmaxf(m[ct], top);
+      const float base = mn == -INFINITY ? 0.f : mn;  // every key so far masked: nothing to add up
+      const float alpha = fast_exp2(m[ct] - base);
+      m[ct] = mn;
+      l[ct] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] *= alpha;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float e0 = fast_exp2(__fmaf_rn(sc[ct][rt][r], c, -base));
+          const float e1 = fast_exp2(__fmaf_rn(sc[ct][rt][r + 1], c, -base));
+          if constexpr (E::ES == 2) {
+            const uint32_t w = E::Io::pack2(e0, e1);
+            p[ct][rt][r >> 3][(r & 7) >> 1] = w;
+            l[ct] = add_pair<typename E::Io>(w, l[ct]);
+          } else {
+            sc[ct][rt][r] = e0, sc[ct][rt][r + 1] = e1;
+            l[ct] += e0 + e1;
+          }
+        }
+    }
+    if (__builtin_expect(masked && apart, 0)) return add_apart(sV, k0, sc, p);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      if constexpr (E::ES == 2) {
+#pragma unroll
+        for (int g = 0; g < 2 * RT; ++g) {
+          const u32x4 vf = v_operand<E, D>(sV, dt, g);
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct)
+            o[ct][dt] = mfma_io_32x32x16<typename E::Io>(vf, p[ct][g >> 1][g & 1], o[ct][dt]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float vf = v_value(sV, dt, r);
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) o[ct][dt] = mfma_f32_32x32x2(vf, sc[ct][0][r], o[ct][dt]);
+        }
+      }
+    }
+  }
+
+  // fp32: V of key acc_key(0, r, lh), dim 32 dt + lr.
+  __device__ __forceinline__ float v_value(const uint8_t* sV, int dt, int r) const {
+    const int lane = threadIdx.x & 63, lr = lane & 31, key = acc_key(0, r, lane >> 5);
+    return *reinterpret_cast<const float*>(sV + key * (D * 4) + 16 * v_chunk<E, D>(key, 8 * dt + (lr >> 2)) + 4 * (lr & 3));
+  }
+
+  // The same sums from V's finite values, in the same order, and then those of its NaNs and infinities, one key at a time,
+  // added to the rows that see it.
+  __device__ __forceinline__ void add_apart(const uint8_t* sV, int k0, const f32x16 (&sc)[NCT][RT],
+                                            const u32x4 (&p)[NCT][RT][2]) {
+    const int lh = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      auto add = [&](int key, int ct, const f32x16& x) {
+        const bool seen = k0 + key < lim[ct];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[ct][dt][i] = seen ? o[ct][dt][i] + x[i] : o[ct][dt][i];
+      };
+      if constexpr (E::ES == 2) {
+        u32x4 wild[2 * RT];
+        bool any = false;
+#pragma unroll
+        for (int g = 0; g < 2 * RT; ++g) {
+          u32x4 vf = v_operand<E, D>(sV, dt, g);
+          constexpr uint32_t kExp = std::is_same<typename E::Io, Bf16Io>::value ? 0x7f80u : 0x7c00u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t at = ((vf[i] & kExp) == kExp ? 0xffffu : 0u) |
+                                ((vf[i] & (kExp << 16)) == kExp << 16 ? 0xffff0000u : 0u);
+            wild[g][i] = vf[i] & at;
+            vf[i] &= ~at;
+            any |= at != 0;
+          }
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct)
+            o[ct][dt] = mfma_io_32x32x16<typename E::Io>(vf, p[ct][g >> 1][g & 1], o[ct][dt]);
+        }
+        if (!__any(any)) continue;
+#pragma unroll
+        for (int g = 0; g < 2 * RT; ++g) {
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {  // key 16 g + j: element 4 (j / 8) + j % 4 of lane half (j / 4) % 2
+            u32x4 one;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              one[i] = lh == ((j >> 2) & 1) && i == 2 * (j >> 3) + ((j & 3) >> 1)
+                           ? wild[g][i] & (j & 1 ? 0xffff0000u : 0xffffu)
+                           : 0u;
+#pragma unroll
+            for (int ct = 0; ct < NCT; ++ct)
+              add(16 * g + j, ct, mfma_io_32x32x16<typename E::Io>(one, p[ct][g >> 1][g & 1], f32x16{}));
+          }
+        }
+      } else {
+        auto is_wild = [](float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; };
+        bool any = false;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float vf = v_value(sV, dt, r);
+          any |= is_wild(vf);
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) o[ct][dt] = mfma_f32_32x32x2(is_wild(vf) ? 0.f : vf, sc[ct][0][r], o[ct][dt]);
+        }
+        if (!__any(any)) continue;
+#pragma unroll 1
+        for (int n = 0; n < 32; ++n) {  // register n / 2 of lane half n % 2
+          const int r = n >> 1;
+          const float vf = v_value(sV, dt, r), wild = lh == (n & 1) && is_wild(vf) ? vf : 0.f;
+#pragma unroll
+          for (int ct = 0; ct < NCT; ++ct) {
+            float one = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) one = r == i ? sc[ct][0][i] : one;
+            add(acc_key(0, r, n & 1), ct, mfma_f32_32x32x2(wild, one, f32x16{}));
+          }
+        }
+      }
+    }
+  }
+};
+
+// A NaN or an infinity in the values of a key that a row does not see meets a probability of zero, and their product is NaN.
+// Values are seldom so: the sums are taken as they come, and a workgroup that finds a NaN in them repeats its tile with
+// such values of masked tiles apart. The other rows get the same sums as without them, bit for bit.
+template <class E, int D, int NCT, int NW, int WAVES>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) void attend_kernel(const Args a) {
+  using L = Lds<E, D>;
+  constexpr int R = 32 * NCT * NW;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[2 * L::kStage];
+  const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, wv = wave_id();
+  // consecutive workgroups: the parts of one tile's keys, then the heads of keys, then the slots
+  const int part = blockIdx.x % a.splits, rest = blockIdx.x / a.splits, g = rest % a.G, u = rest / a.G;
+  const Tile t = find_tile(a, u, R);
+  const int row_bytes = D * E::ES;
+  if (!t.found) {
+    if (!a.zero_rest || part) return;
+    // the rows of no sequence, shared by the slots without a tile (one at least: every sequence fills the most of its last)
+    const int first = clamp_to(a.off[0], 0, a.T), end = clamp_to(a.off[a.N], first, a.T), spare = a.T - (end - first);
+    const int pieces = a.gs * row_bytes / 16;  // 16-byte ones of this head's rows of a token
+    for (int i = t.index; i < spare; i += t.idle) {
+      uint8_t* row = a.out + static_cast<int64_t>(i < first ? i : end + i - first) * a.o_ts;
+      for (int j = threadIdx.x; j < pieces; j += 64 * NW)
+        st16(row + (g * a.gs + j / (row_bytes / 16)) * a.o_hs + 16 * (j % (row_bytes / 16)), u32x4{0, 0, 0, 0});
+    }
+    return;
+  }
+  const int rows = t.lq * a.gs, r0 = t.index * R + wv * 32 * NCT;
+  // the keys that row r sees; rows past the last as that one
+  auto sees = [&](int r) {
+    const int at = (r < rows ? r : rows - 1) / a.gs;
+    return a.causal ? clamp_to(at + 1 + t.lk - t.lq, 0, t.lk) : t.lk;
+  };
+  const int all = __builtin_amdgcn_readfirstlane(sees(t.index * R + R - 1));  // of the workgroup's rows
+  const int most = r0 < rows ? __builtin_amdgcn_readfirstlane(sees(r0 + 32 * NCT - 1)) : 0;  // of the wave's: the last
+  const int least = __builtin_amdgcn_readfirstlane(sees(r0));                               // and the first one
+  const int each = ((all + a.splits - 1) / a.splits + E::KT - 1) / E::KT * E::KT;
+  const int begin = part * each, end = begin + each < all ? begin + each : all;
+
+  Rows<E, D, NCT> w;
+  int64_t row_of[NCT];  // token, head
+  int head[NCT];
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const int r = r0 + 32 * ct + lr, rc = r < rows ? r : rows - 1, at = rc / a.gs;
+    row_of[ct] = t.q0 + at;
+    head[ct] = g * a.gs + rc - at * a.gs;
+    w.lim[ct] = sees(r);
+    const uint8_t* p = a.q + row_of[ct] * a.q_ts + head[ct] * a.q_hs;
+#pragma unroll
+    for (int i = 0; i < Rows<E, D, NCT>::kQ; ++i) w.q[ct][i] = ld16(p + 32 * i + 16 * lh);
+  }
+  const uint32_t lds0 = lds_addr(smem);
+  for (bool apart = false;; apart = true) {
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      w.m[ct] = -INFINITY, w.l[ct] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) w.o[ct][dt] = f32x16{};
+    }
+    if (begin < end) {
+      const KeyCopy<E, D, NW> copy(a, t, g);
+      copy(begin, lds0);
+      int stage = 0;
+      for (int k0 = begin; k0 < end; k0 += E::KT, stage ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies of the tile
+        __syncthreads();                                  // everybody's, and the other stage is free
+        if (k0 + E::KT < end) copy(k0 + E::KT, lds0 + (stage ^ 1) * L::kStage);
+        const uint8_t* s = smem + stage * L::kStage;
+        if (k0 < most) w.step(s, s + L::kTile, k0, a.c, k0 + E::KT > least, apart);
+      }
+    }
+    if (apart) break;
+    bool nan = false;
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) nan |= w.o[ct][dt][i] != w.o[ct][dt][i];
+    if (!__syncthreads_or(nan)) break;  // (and the stages are free)
+  }
+
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) {
+    const float total = w.l[ct] + __shfl_xor(w.l[ct], 32, kWave);
+    if (r0 + 32 * ct + lr >= rows) continue;
+    if (a.splits > 1) {
+      const int64_t n = (static_cast<int64_t>(part) * a.T + row_of[ct]) * a.H + head[ct];
+      float* po = a.part_o + n * D;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * i + 4 * lh) =
+              f32x4{w.o[ct][dt][4 * i], w.o[ct][dt][4 * i + 1], w.o[ct][dt][4 * i + 2], w.o[ct][dt][4 * i + 3]};
+      if (lh == 0) a.part_ml[2 * n] = w.m[ct], a.part_ml[2 * n + 1] = total;
+      continue;
+    }
+    const float inv = total == 0.f ? 0.f : __frcp_rn(total);
+    uint8_t* orow = a.out + row_of[ct] * a.o_ts + head[ct] * a.o_hs;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = w.o[ct][dt][4 * i + j] * inv;
+        uint8_t* p = orow + (32 * dt + 8 * i + 4 * lh) * E::ES;
+        if constexpr (E::ES == 2)
+          *reinterpret_cast<u32x2*>(p) = u32x2{E::Io::pack2(x[0], x[1]), E::Io::pack2(x[2], x[3])};
+        else
+          *reinterpret_cast<f32x4*>(p) = f32x4{x[0], x[1], x[2], x[3]};
+      }
+  }
+}
+
+// The parts of each row's keys joined, in their order: a wave per row.
+template <class E, int D>
+__global__ __launch_bounds__(256) void join_kernel(const Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 4 + wave_id(), all = static_cast<int64_t>(a.T) * a.H;
+  if (n >= all) return;
+  const int token = static_cast<int>(n / a.H), head = static_cast<int>(n - static_cast<int64_t>(token) * a.H);
+  const int first = clamp_to(a.off[0], 0, a.T);
+  if (token < first || token >= clamp_to(a.off[a.N], first, a.T)) return;  // of no sequence
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + n)]);
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int N = D / 64;
+  float sum[N] = {}, total = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = s * all + n;
+    const float f = fast_exp2(a.part_ml[2 * at] - base);
+    total = __fmaf_rn(f, a.part_ml[2 * at + 1], total);
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[j] = __fmaf_rn(f, a.part_o[at * D + N * lane + j], sum[j]);
+  }
+  const float inv = total == 0.f ? 0.f : __frcp_rn(total);
+  uint8_t* p = a.out + token * a.o_ts + head * a.o_hs + N * lane * E::ES;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if constexpr (E::ES == 4) reinterpret_cast<float*>(p)[j] = sum[j] * inv;
+    else reinterpret_cast<uint16_t*>(p)[j] = static_cast<uint16_t>(E::Io::pack2(sum[j] * inv, 0.f));
+  }
+}
+
+constexpr int kWaves = 4, kColumns = 1, kTileRows = 32 * kColumns * kWaves;
+
+// Slots: a sequence of n rows takes at most (n + kTileRows - 1) / kTileRows tiles.
+int64_t slots_of(int64_t T, int N, int gs) { return (T * gs + kTileRows - 1) / kTileRows + N; }
+
+// Parts of the keys: where the tiles do not fill the card twice, as many as do, of 256 keys in the mean at least.
+int splits_of(int64_t T, int64_t Tk, int N, int H, int G) {
+  const int64_t tiles = slots_of(T, N, H / G) * G, want = 2 * device_cus();
+  int64_t s = want / tiles;
+  const int64_t most = Tk / N / 256;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+size_t workspace_of(int64_t T, int64_t Tk, int N, int H, int G, int D) {
+  const int s = splits_of(T, Tk, N, H, G);
+  return s == 1 ? 0 : static_cast<size_t>(s) * static_cast<size_t>(T) * H * (D + 2) * 4;
+}
+
+template <class E, int D>
+void launch(hipStream_t stream, const Args& a) {
+  constexpr int kPerSimd = E::ES == 2 && D == 64 ? 3 : 2;
+  hipLaunchKernelGGL((attend_kernel<E, D, kColumns, kWaves, kPerSimd>), dim3(static_cast<unsigned>(a.slots) * a.G * a.splits),
+                     dim3(64 * kWaves), 0, stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((join_kernel<E, D>), dim3(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.H + 3) / 4)),
+                       dim3(256), 0, stream, a);
+}
+
+int check_sizes(const char* what, int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D) {
+  if (dtype != HB_BF16 && dtype != HB_F32 && dtype != HB_F16)
+    return fail(HB_ERR_DTYPE, "%s: dtype %d is not HB_BF16 (0), HB_F32 (1) or HB_F16 (2)", what, dtype);
+  if (D != 64 && D != 128) return fail(HB_ERR_HEAD_DIM, "%s: head_dim %d is not 64 or 128", what, D);
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (T < 1 || Tk < 0 || N < 1 || H < 1 || G < 1 || H % G || H > 65535 || N > (1 << 20) || T > kMost || Tk > kMost ||
+      T * (H / G) > kMost || slots_of(T, N, H / G) * G >= (int64_t(1) << 24))
+    return fail(HB_ERR_SHAPE, "%s: T=%lld, Tk=%lld, N=%d, H=%d, G=%d out of range", what, static_cast<long long>(T),
+                static_cast<long long>(Tk), N, H, G);
+  return HB_OK;
+}
+
+}  // namespace packed
+}  // namespace hb
+
+using namespace hb;
+
+extern "C" {
+
+size_t hb_packed_workspace_size(int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D) {
+  clear_error();
+  if (packed::check_sizes("packed_workspace_size", dtype, T, Tk, N, H, G, D)) return 0;
+  return packed::workspace_of(T, Tk, N, H, G, D);
+}
+
+int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, int dtype, const int* offsets, const int* key_offsets,
+                        const int* key_lengths, int causal, float scale, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, int zero_rest, int64_t T, int64_t Tk, int N, int H, int G, int D,
+                        void* workspace, size_t workspace_bytes) {
+  clear_error();
+  const char* what = "packed_attention";
+  int st = packed::check_sizes(what, dtype, T, Tk, N, H, G, D);
+  if (st) return st;
+  if (!q || !offsets || !key_offsets || !out || (Tk > 0 && (!k || !v)))
+    return fail(HB_ERR_NULL, "%s: q, k, v, offsets, key_offsets and out must be non-NULL", what);
+  if (!(scale > 0.0f) || !std::isfinite(scale) || !std::isfinite(scale * kLog2e))
+    return fail(HB_ERR_EPS, "%s: scale %g must be finite and > 0", what, scale);
+  const int es = dtype == HB_F32 ? 4 : 2, vec = 16 / es;
+  struct Operand {
+    const char* name;
+    const void* p;
+    int64_t ts, hs, tokens;
+    int heads;
+    int64_t bytes;
+  } ops[] = {{"out", out, out_token_stride, out_head_stride, T, H, 0}, {"q", q, q_token_stride, q_head_stride, T, H, 0},
+             {"k", k, k_token_stride, k_head_stride, Tk, G, 0},       {"v", v, v_token_stride, v_head_stride, Tk, G, 0}};
+  for (Operand& o : ops) {
+    if (!o.tokens) continue;
+    if (reinterpret_cast<uintptr_t>(o.p) % 16 || o.ts % vec || o.hs % vec || o.ts < 0 || o.hs < 0)
+      return fail(HB_ERR_STRIDE, "%s: %s must be 16-byte aligned with strides that are multiples of %d, not negative", what,
+                  o.name, vec);
+    // a key tile's rows are addressed by 32-bit offsets from its first
+    if ((o.name[0] == 'k' || o.name[0] == 'v') && o.ts > (1 << 23))
+      return fail(HB_ERR_STRIDE, "%s: %s token stride must be at most 2^23", what, o.name);
+    if ((st = check_extent(what, o.name, o.tokens, o.ts, D)) || (st = check_extent(what, o.name, o.heads, o.hs, D)))
+      return st;
+    o.bytes = ((o.tokens - 1) * o.ts + (o.heads - 1) * o.hs + D) * es;
+  }
+  // the output's rows share no element: heads within tokens or tokens within heads
+  const bool inside = H == 1 || out_head_stride >= D, outside = T == 1 || out_token_stride >= D;
+  if (!inside || !outside ||
+      !(T == 1 || H == 1 || out_token_stride >= (H - 1) * out_head_stride + D ||
+        out_head_stride >= (T - 1) * out_token_stride + D))
+    return fail(HB_ERR_STRIDE, "%s: the rows of out overlap", what);
+  const int64_t ob = ops[0].bytes, table = (static_cast<int64_t>(N) + 1) * 4;
+  const size_t need = packed::workspace_of(T, Tk, N, H, G, D);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(HB_ERR_WORKSPACE, "%s needs %zu bytes of workspace, 16-byte aligned", what, need);
+  auto misaligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; };
+  if (misaligned(offsets) || misaligned(key_offsets) || misaligned(key_lengths))
+    return fail(HB_ERR_STRIDE, "%s: offsets, key_offsets and key_lengths must be 4-byte aligned", what);
+  const int64_t wb = static_cast<int64_t>(need);
+  for (const Operand& o : ops)
+    if ((o.name[0] != 'o' && (st = check_disjoint(what, "out", out, ob, o.name, o.p, o.bytes))) ||
+        (st = check_disjoint(what, "workspace", workspace, wb, o.name, o.p, o.bytes)))
+      return st;
+  const struct {
+    const char* name;
+    const void* p;
+    int64_t bytes;
+  } tables[] = {{"offsets", offsets, table}, {"key_offsets", key_offsets, table}, {"key_lengths", key_lengths, table - 4}};
+  for (const auto& o : tables)
+    if ((st = check_disjoint(what, "out", out, ob, o.name, o.p, o.bytes)) ||
+        (st = check_disjoint(what, "workspace", workspace, wb, o.name, o.p, o.bytes)))
+      return st;
+  packed::Args a = {};
+  a.q = static_cast<const uint8_t*>(q), a.q_ts = q_token_stride * es, a.q_hs = q_head_stride * es;
+  a.k = static_cast<const uint8_t*>(k), a.k_ts = k_token_stride * es, a.k_hs = k_head_stride * es;
+  a.v = static_cast<const uint8_t*>(v), a.v_ts = v_token_stride * es, a.v_hs = v_head_stride * es;
+  a.out = static_cast<uint8_t*>(out), a.o_ts = out_token_stride * es, a.o_hs = out_head_stride * es;
+  a.off = offsets, a.koff = key_offsets, a.klen = key_lengths;
+  a.causal = causal != 0, a.zero_rest = zero_rest != 0, a.c = scale * kLog2e;
+  a.T = static_cast<int>(T), a.Tk = static_cast<int>(Tk), a.N = N, a.H = H, a.G = G, a.gs = H / G;
+  a.slots = static_cast<int>(packed::slots_of(T, N, H / G)), a.splits = packed::splits_of(T, Tk, N, H, G);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o ? a.part_o + static_cast<int64_t>(a.splits) * T * H * D : nullptr;
+  auto run = [&](auto e) {
+    using E = decltype(e);
+    if (D == 64) packed::launch<E, 64>(stream, a);
+    else packed::launch<E, 128>(stream, a);
+  };
+  if (dtype == HB_BF16) run(packed::E16<Bf16Io>{});
+  else if (dtype == HB_F16) run(packed::E16<F16Io>{});
+  else run(packed::E32{});
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(HB_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return HB_OK;
+}
+
+}  // extern "C"

@@ -16,17 +16,11 @@
 
 #include "api.h"
 #include "common.h"
+#include "rows_tile.h"
 #include "tiles.h"
 
 namespace hb {
 namespace q8 {
-
-// Outputs of more bytes than half of the last cache (256 MB) are stored past it: what reads them next would not find
-// them there, and they would drive the operands out (8249 x 1536 -> 12288, 203 MB: 172 -> 160 us). Smaller ones stay:
-// without, the denoiser's 120 s render, whose norms read them at once, takes 40.6 ms instead of 40.0.
-constexpr int64_t kStreamBytes = int64_t(128) << 20;
-
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct Args {
   const uint8_t* x;  // (M, K), row stride x_rs bytes
@@ -63,15 +57,6 @@ __device__ __forceinline__ float scaled_any(float acc, float sw, float sx, float
   return ldexpf(m, __builtin_amdgcn_frexp_expf(sw) + __builtin_amdgcn_frexp_expf(sx)) + bias;
 }
 
-template <typename T>
-__device__ __forceinline__ T cast_out(float v);
-template <>
-__device__ __forceinline__ uint16_t cast_out<uint16_t>(float v) { return f2bf(v); }
-template <>
-__device__ __forceinline__ _Float16 cast_out<_Float16>(float v) { return static_cast<_Float16>(v); }
-template <>
-__device__ __forceinline__ float cast_out<float>(float v) { return v; }
-
 // 8 e4m3 codes as bf16, exact.
 __device__ __forceinline__ u32x4 widen8(u32x2 c) {
   u32x4 v;
@@ -89,8 +74,6 @@ __device__ __forceinline__ u32x4 widen8(u32x2 c) {
 // multiplies NF x NM tiles of 32 x 32. Two stages suffice where a CU has two workgroups or a step takes longer than a
 // copy; a workgroup that has its CU to itself waits for its copies with two (0.5 us a step, whatever the tile) and gains
 // from three or four (2584 x 6144 -> 1536, Medium, 27.5 -> 25.3 us; 400 x 6144 -> 1536, Small, 14.5 -> 12.3).
-constexpr int kStep = 128;  // bytes (columns) of K per stage
-
 template <int FT_, int MT_, int WF_, int WM_, int WAVES_, int STAGES_ = 2>
 struct Tile {
   static constexpr int FT = FT_, MT = MT_, WF = WF_, WM = WM_;
@@ -102,37 +85,9 @@ struct Tile {
   static_assert(FT % (8 * NW) == 0 && MT % (8 * NW) == 0 && NF >= 1 && NM >= 1, "whole copies and tiles per wave");
 };
 
-// As lds_dma16 with 4 bytes per lane: 256 bytes at LDS byte address `lds`.
-__device__ __forceinline__ void lds_dma4(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(sbase) : "m0");
-}
-
-// As lds_dma16 with an address per lane.
-__device__ __forceinline__ void lds_dma16_any(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "m0");
-}
-
-// Byte of logical 16-byte chunk `chunk` of row `row` in a stage: the reads of a fragment (one chunk of consecutive
-// rows) then spread over the banks.
-__device__ __forceinline__ int swz_byte(int row, int chunk) {
-  return row * kStep + 16 * (chunk ^ (row & 7) ^ ((row >> 3) & 1));
-}
-
-// All but the newest N of this wave's copies have landed (older loads and stores too).
-template <int N>
-__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-// This wave's LDS reads and writes are done.
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // The copies of a stage by one wave: blocks wv, wv + NW, ... of the A rows (features), then of the B rows. Lane i's 16
 // bytes land at byte 16 i of a block, row i / 8, position i % 8, so it fetches the chunk that the swizzle puts there.
 // RAGGED: K may end inside a stage; chunks from column K on come from `zeros`.
-__device__ __attribute__((aligned(16))) const uint8_t zeros[16] = {};
 
 template <class TL, bool RAGGED>
 struct StageCopy {
@@ -204,54 +159,12 @@ __device__ __forceinline__ f32x16 multiply(const u32x4 (&a)[2], const u32x4 (&b)
   return c;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<uint16_t>(float lo, float hi) { return pack_bf16x2(lo, hi); }
-template <>
-__device__ __forceinline__ uint32_t pack2<_Float16>(float lo, float hi) { return F16Io::pack2(lo, hi); }
-
-// A lane half's registers exchanged: `x`'s upper half of the wave (or of each 32 lanes) against `y`'s lower one.
-__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {
-  const u32x2 r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
-  x = r[0], y = r[1];
-}
-__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {
-  const u32x2 r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
-  x = r[0], y = r[1];
-}
-
-// 16 bytes of consecutive results from feature f of a row on, those past the last feature left out. Rows of any stride and
-// width: the 16-byte store takes any alignment of its elements.
-// STREAM: past the caches (see kStreamBytes).
-typedef u32x4 u32x4_align2 __attribute__((aligned(2)));
-template <bool STREAM, typename T>
-__device__ __forceinline__ void store16(T* row, int f, int F, u32x4 v) {
-  constexpr int N = 16 / static_cast<int>(sizeof(T));
-  if (f + N <= F) {
-    u32x4_align2* p = reinterpret_cast<u32x4_align2*>(row + f);
-    if constexpr (STREAM) __builtin_nontemporal_store(v, p);
-    else *p = v;
-  } else if (f < F) {
-#pragma unroll
-    for (int j = 0; j < N - 1; ++j) {
-      if (f + j >= F) continue;
-      if constexpr (sizeof(T) == 4) row[f + j] = __uint_as_float(v[j]);
-      else row[f + j] = __builtin_bit_cast(T, static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1))));
-    }
-  }
-}
-
-// A wave's results. Lane (lr, lh) holds, in registers 4 g .. 4 g + 3 of a 32 x 32 tile, features 8 g + 4 lh .. + 3 of row
-// lr. The results of a tile leave in stores of 16 rows of 64 bytes: for 16-bit types the wave's halves exchange so that
-// a lane holds eight consecutive features, and then its 16-lane rows so that four lanes hold 64 bytes of a row (through
-// LDS a tile waits for its own round trip: 5168 x 6144 -> 1536 54 against 43 us). `sw`, `bias`, `sx`: the scales of this
-// wave's features and rows, in LDS.
+// A wave's results, scaled and stored (see `store_32x32`). `sw`, `bias`, `sx`: the scales of this wave's features and
+// rows, in LDS.
 template <typename T, class TL, bool STREAM>
 __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL::NF][TL::NM], int f0, int64_t m0,
                                            const float* sw_, const float* bias_, const float* sx_) {
   const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
-  T* const out = static_cast<T*>(a.out);
   float sx[TL::NM];
 #pragma unroll
   for (int t = 0; t < TL::NM; ++t) sx[t] = sx_[32 * t + lr];
@@ -281,46 +194,7 @@ __device__ __forceinline__ void store_tile(const Args& a, const f32x16 (&acc)[TL
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = scaled_ordinary(acc[n][t][i], sw[i], sx[t], bias[i]);
       }
-      if constexpr (sizeof(T) == 4) {
-        uint32_t w[4][4];  // [g]: features 8 g + 4 lh .. + 3
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[g][j] = __float_as_uint(v[4 * g + j]);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)  // 64 bytes of a row: groups 2 p and 2 p + 1
-#pragma unroll
-          for (int j = 0; j < 4; ++j) swap16(w[2 * p][j], w[2 * p + 1][j]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {  // rows 16 (q % 2) .. of the tile
-          const int64_t m = m0 + 32 * t + 16 * (q & 1) + (lr & 15);
-          const int f = fn + 16 * (q >> 1) + 8 * (lr >> 4) + 4 * lh;
-          if (m < a.M) store16<STREAM>(out + m * a.os, f, a.F, u32x4{w[q][0], w[q][1], w[q][2], w[q][3]});
-        }
-      } else {
-        uint32_t w[4][2];  // [g]: features 8 g + 4 lh .. + 3
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          w[g][0] = pack2<T>(v[4 * g], v[4 * g + 1]);
-          w[g][1] = pack2<T>(v[4 * g + 2], v[4 * g + 3]);
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p)  // lane half lh: the eight features of group 2 p + lh
-#pragma unroll
-          for (int j = 0; j < 2; ++j) swap32(w[2 * p][j], w[2 * p + 1][j]);
-#pragma unroll
-        for (int p = 0; p < 2; ++p)  // rows 16 p .. of the tile, 16 lanes of groups 0, 1 and 16 of 2, 3 in each half
-#pragma unroll
-          for (int j = 0; j < 2; ++j) swap16(w[p][j], w[2 + p][j]);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int64_t m = m0 + 32 * t + 16 * p + (lr & 15);
-          const int f = fn + 16 * (lr >> 4) + 8 * lh;
-          if (m < a.M)
-            store16<STREAM>(out + m * a.os, f, a.F,
-                            u32x4{w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]});
-        }
-      }
+      store_32x32<T, STREAM>(static_cast<T*>(a.out), a.os, a.M, a.F, m0 + 32 * t, fn, v);
     }
   }
 }

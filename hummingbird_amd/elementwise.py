@@ -3,8 +3,9 @@
 the compute dtype (sa3jax/same_l.py:58-69, 191-192), of the GLU gate of `same_l._feed_forward`
 (sa3jax/same_l.py:172-183; the DiT's SwiGLU, sa3jax/dit.py:218-221, is the same gate), and of the DiT block's
 norms, adaLN modulations and residuals (sa3jax/dit.py:224-251). The `_q8` forms of the latter (`quantize_rows`,
-`rms_modulate_q8`, `residual_rms_q8`, `glu_q8`) end in 8-bit rows, the inputs of `projection.linear_q8`. Tensors are
-torch tensors on a ROCm device; work is enqueued on torch's current stream.
+`rms_modulate_q8`, `residual_rms_q8`, `glu_q8`) end in 8-bit rows, the inputs of `projection.linear_q8`, and the `_mx4`
+forms in microscaled 4-bit rows, those of `projection.linear_mx4`. Tensors are torch tensors on a ROCm device; work is
+enqueued on torch's current stream.
 """
 from __future__ import annotations
 
@@ -366,4 +367,107 @@ def glu_q8(proj: torch.Tensor, bias: torch.Tensor | None = None) -> tuple[torch.
     q, s = _q8_out(proj, inner)
     _lib.launch(_lib.load().hb_glu_q8, "glu_q8", proj.device, proj.data_ptr(), code, stride, bp, q.data_ptr(), inner,
                 s.data_ptr(), rows, inner)
+    return q, s
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Microscaled 4-bit rows: e2m1 codes `q`, two per byte (the low nibble the even column), with one e8m0 scale byte `s` per
+# 32 columns, standing for the code's value times 2^(s - 127): the form of `projection.quantize_q4`'s weights.
+
+MX4_GROUP = 32  # columns that share a scale
+
+
+def _mx4_out(like: torch.Tensor, width: int, what: str) -> tuple[torch.Tensor, torch.Tensor]:
+    """Contiguous 4-bit rows of `width` values and their scale bytes, for the rows of `like`."""
+    if width % MX4_GROUP:
+        raise ValueError(f"{what}: rows must be a multiple of {MX4_GROUP} values, got {width}")
+    rows = tuple(like.shape[:-1])
+    return (_new((*rows, width // 2), torch.uint8, like.device),
+            _new((*rows, width // MX4_GROUP), torch.uint8, like.device))
+
+
+def quantize_rows_mx4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`x` `(..., C)` as 4-bit rows `(q, s)`, q `(..., C / 2)` and s `(..., C / 32)`, both uint8, in one pass
+    (`hb_quant_rows_mx4`): per group of 32 columns the least s, from 8 on, that brings the largest magnitude to 6 or below
+    (127 for a group of zeros), and e2m1(x 2^(127 - s)), to nearest, ties to the even code. A group with a NaN or an
+    infinity stands for NaNs (s = 255). C a multiple of 32."""
+    rows, stride, channels = _layout(x, "x")
+    code = dtype_code(x.dtype)
+    q, s = _mx4_out(x, channels, "quantize_rows_mx4")
+    _lib.launch(_lib.load().hb_quant_rows_mx4, "quantize_rows_mx4", x.device, x.data_ptr(), code, stride, q.data_ptr(),
+                channels // 2, s.data_ptr(), channels // MX4_GROUP, rows, channels)
+    return q, s
+
+
+def rms_modulate_mx4(x: torch.Tensor, weight: torch.Tensor, eps: float, scale: torch.Tensor | None = None,
+                     shift: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`rms_modulate(x, weight, eps, scale, shift)` on `(B, L, C)` in fp32 throughout, as 4-bit rows `(q, s)` (see
+    `quantize_rows_mx4`), in one pass (`hb_rms_modulate_mx4`). C a multiple of 32, at most `Q8_MAX_WIDTH`."""
+    rows, stride, channels = _layout(x, "x")
+    if x.dim() != 3:
+        raise ValueError(f"x must be (B, L, C), got {tuple(x.shape)}")
+    code = dtype_code(x.dtype)
+    batch, length, _ = x.shape
+    w = _f32_channels(weight, channels, x.device, "weight")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift are given together or not at all")
+    sp, ms = _batch_rows(scale, batch, channels, x, "scale")
+    hp, ms2 = _batch_rows(shift, batch, channels, x, "shift")
+    if ms != ms2:
+        raise ValueError("scale and shift must share their batch stride")
+    q, s = _mx4_out(x, channels, "rms_modulate_mx4")
+    _lib.launch(_lib.load().hb_rms_modulate_mx4, "rms_modulate_mx4", x.device, x.data_ptr(), code, stride, w.data_ptr(),
+                float(eps), sp, hp, ms, length, q.data_ptr(), channels // 2, s.data_ptr(), channels // MX4_GROUP, rows,
+                channels)
+    return q, s
+
+
+def residual_rms_mx4(h: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
+                     gate: torch.Tensor | None = None, x_bias: torch.Tensor | None = None,
+                     local: torch.Tensor | None = None, memory: int = 0, scale: torch.Tensor | None = None,
+                     shift: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`residual_rms(h, x, weight, eps, gate, x_bias, local, memory, scale, shift)` with the norm as 4-bit rows, in one
+    pass (`hb_residual_rms_mx4`): `(h', q, s)`, h' in `h.dtype`, `(q, s)` as `quantize_rows_mx4` gives them. Both are
+    rounded once, from fp32: the norm reads h' before its rounding. C a multiple of 32, at most `Q8_MAX_WIDTH`."""
+    rows, hs, channels = _layout(h, "h")
+    if h.dim() != 3 or x.shape != h.shape or x.dtype != h.dtype or x.device != h.device:
+        raise ValueError(f"h and x must be (B, L, C) of one shape, dtype and device, got {tuple(h.shape)} {h.dtype} "
+                         f"{h.device}, {tuple(x.shape)} {x.dtype} {x.device}")
+    xs = channels if x.is_contiguous() else _layout(x, "x")[1]
+    code = dtype_code(h.dtype)
+    batch, length, _ = h.shape
+    gp, gs = _batch_rows(gate, batch, channels, h, "gate")
+    if (scale is None) != (shift is None):
+        raise ValueError("scale and shift are given together or not at all")
+    sp, ms = _batch_rows(scale, batch, channels, h, "scale")
+    hp, ms2 = _batch_rows(shift, batch, channels, h, "shift")
+    if ms != ms2:
+        raise ValueError("scale and shift must share their batch stride")
+    w = _f32_channels(weight, channels, h.device, "weight")
+    bp, lp = _channel_vector(x_bias, channels, h, "x_bias"), _channel_vector(local, channels, h, "local")
+    q, s = _mx4_out(h, channels, "residual_rms_mx4")
+    out_h = _new((batch, length, channels), h.dtype, h.device)
+    _lib.launch(_lib.load().hb_residual_rms_mx4, "residual_rms_mx4", h.device, h.data_ptr(), code, hs, x.data_ptr(), xs,
+                bp, gp, gs, lp, _memory_tokens(memory, length), w.data_ptr(), float(eps), sp, hp, ms, length,
+                out_h.data_ptr(), channels, q.data_ptr(), channels // 2, s.data_ptr(), channels // MX4_GROUP, rows,
+                channels)
+    return out_h, q, s
+
+
+def glu_mx4(proj: torch.Tensor, bias: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`value * silu(gate)` for `[value | gate]` = the two halves of the last axis of `proj (+ bias)`, in fp32, as
+    4-bit rows `(q, s)` (see `quantize_rows_mx4`), in one pass (`hb_glu_mx4`): the DiT's SwiGLU
+    (sa3jax/dit.py:218-221). `bias` `(2F,)` is the glu_proj layer's where `proj` is the bare product. F a multiple of 32."""
+    rows, stride, width = _layout(proj, "proj")
+    code = dtype_code(proj.dtype)
+    if width % 2:
+        raise ValueError(f"the glu_proj output width {width} is not even")
+    inner = width // 2
+    bp = 0
+    if bias is not None:
+        bias = _f32_channels(bias, width, proj.device, "bias")
+        bp = bias.data_ptr()
+    q, s = _mx4_out(proj, inner, "glu_mx4")
+    _lib.launch(_lib.load().hb_glu_mx4, "glu_mx4", proj.device, proj.data_ptr(), code, stride, bp, q.data_ptr(),
+                inner // 2, s.data_ptr(), inner // MX4_GROUP, rows, inner)
     return q, s

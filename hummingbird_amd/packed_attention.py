@@ -1,0 +1,88 @@
+"""Attention over packed sequences on MI355X (`hb_packed_attention`): prompts or clips of different lengths one after the
+other in one tensor, causal or not, with heads of queries that share heads of keys, and new tokens over the keys of their
+sequences. It is the plain softmax attention of the non-differential model (`DiTConfig.differential = False`,
+sa3jax/dit.py:150-176) and of transformers beside the denoiser; `dense_attention`, `band_attention` and
+`cross_attention` are the differential ones. Tensors are torch tensors on a ROCm device; work is enqueued on torch's
+current stream.
+"""
+from __future__ import annotations
+
+import torch
+
+from hummingbird_amd import _lib
+from hummingbird_amd.dense_attention import _require_gpu, dtype_code
+
+SUPPORTED_HEAD_DIMS = (64, 128)
+
+
+def _heads(t: torch.Tensor, name: str) -> None:
+    if t.dim() != 3 or t.stride(2) != 1:
+        raise ValueError(f"{name} must be (tokens, heads, head_dim) with unit stride on its last axis, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+
+
+def _table(t: torch.Tensor, name: str, entries: int, device: torch.device) -> torch.Tensor:
+    """A table of int32 entries on `device`."""
+    if t.device != device or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32 on {device}, got {t.dtype} on {t.device}")
+    if t.dim() != 1 or t.shape[0] != entries or not t.is_contiguous():
+        raise ValueError(f"{name} must have {entries} entries next to each other, got {tuple(t.shape)}")
+    return t
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor,
+                     key_offsets: torch.Tensor | None = None, key_lengths: torch.Tensor | None = None, *,
+                     causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`q` `(T, H, D)`, `k` and `v` `(Tk, G, D)` -> `(T, H, D)` in `q.dtype`: softmax attention of N sequences, query head
+    h over key head `h // (H // G)`.
+
+    Sequence i has the queries `offsets[i]` to `offsets[i + 1]` and the keys `key_offsets[i]` to `key_offsets[i + 1]`
+    (`offsets` where not given), the first `key_lengths[i]` of them where that is given: the keys of a cache whose slots
+    have room behind them. `offsets` and `key_offsets` are `(N + 1,)` ascending, `key_lengths` `(N,)`, int32 on the device;
+    they are read there, so nothing waits for them and a captured call follows their contents. With `causal` query a of
+    lq sees the keys b <= a + lk - lq of lk: the queries are the last of the keys' tokens (one new token: lq = 1).
+    A query that sees no key gives zeros; keys that a query does not see take no part in it, whatever their values.
+    `scale` (default `D ** -0.5`) is positive.
+
+    `out`, if given, is written and returned, its tokens of no sequence (before `offsets[0]`, from `offsets[N]` on) left as
+    they are; a new output has zeros there. D 64 or 128; bf16, half or fp32 (fp32 throughout); any strides of tokens and
+    heads that are multiples of 16 bytes (of k's and v's tokens up to 2^23 values), every tensor 16-byte aligned."""
+    _require_gpu(q, "q")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _heads(t, name)
+        if t.dtype != q.dtype or t.device != q.device:
+            raise TypeError(f"{name} must be {q.dtype} on {q.device} as q, got {t.dtype} on {t.device}")
+    code, dev = dtype_code(q.dtype), q.device
+    tokens, heads, dim = q.shape
+    keys, kv_heads, _ = k.shape
+    if dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"packed_attention needs head_dim in {SUPPORTED_HEAD_DIMS} (head_dim={dim})")
+    if k.shape != v.shape or k.shape[2] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"k and v must be (Tk, G, D) with H a multiple of G, got q {tuple(q.shape)}, k {tuple(k.shape)}, "
+                         f"v {tuple(v.shape)}")
+    if offsets.dim() != 1 or offsets.shape[0] < 1:
+        raise ValueError(f"offsets must be (N + 1,), got {tuple(offsets.shape)}")
+    count = offsets.shape[0] - 1
+    _table(offsets, "offsets", count + 1, dev)
+    key_offsets = offsets if key_offsets is None else _table(key_offsets, "key_offsets", count + 1, dev)
+    if key_lengths is not None:
+        _table(key_lengths, "key_lengths", count, dev)
+    fresh = out is None
+    if fresh:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _heads(out, "out")
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            raise ValueError(f"out must be {tuple(q.shape)} of {q.dtype} on {dev}, got {tuple(out.shape)} {out.dtype} on "
+                             f"{out.device}")
+    if tokens == 0 or count == 0:
+        return out.zero_() if fresh else out
+    lib = _lib.load()
+    need = int(lib.hb_packed_workspace_size(code, tokens, keys, count, heads, kv_heads, dim))
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.launch(lib.hb_packed_attention, "packed_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
+                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), code, offsets.data_ptr(),
+                key_offsets.data_ptr(), 0 if key_lengths is None else key_lengths.data_ptr(), int(bool(causal)),
+                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), out.stride(0), out.stride(1), int(fresh),
+                tokens, keys, count, heads, kv_heads, dim, workspace.data_ptr() if need else 0, need)
+    return out

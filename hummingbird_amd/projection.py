@@ -9,7 +9,8 @@ workspace. `attend_projected` runs the attention against them (`hb_dense_attend_
 (`hb_proj`). Together they compute what `h @ W_qkv^T -> dense_attention -> @ W_o^T` computes, in the same cast points.
 
 `linear_q8` multiplies 8-bit rows (`elementwise.quantize_rows` and its kin) with 8-bit weights (`hb_proj_q8`), and
-`linear_q4` a few rows with 4-bit weights (`quantize_q4`, `hb_proj_q4`).
+`linear_q4` a few rows with 4-bit weights (`quantize_q4`, `hb_proj_q4`); `linear_mx4` multiplies microscaled 4-bit rows
+(`elementwise.quantize_rows_mx4` and its kin) with the same weights (`hb_proj_mx4`).
 """
 from __future__ import annotations
 
@@ -291,4 +292,40 @@ def linear_q4(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
     out = _new((*x.shape[:-1], f), x.dtype, dev)
     _lib.launch(_lib.load().hb_proj_q4, "linear_q4", dev, x.data_ptr(), code, xs, weight.data_ptr(), ws,
                 weight_scale.data_ptr(), ss, bp, int(bool(silu)), out.data_ptr(), f, n, k, f)
+    return out
+
+
+def linear_mx4(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+               bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """`x @ W^T (+ bias)` of microscaled 4-bit rows on the 4-bit matrix cores (`hb_proj_mx4`): `x` `(..., K / 2)` and
+    `x_scale` `(..., K / 32)` as `elementwise.quantize_rows_mx4` gives them, `weight` `(F, K / 2)` and `weight_scale`
+    `(F, K / 32)` as `quantize_q4` (or `quantize_rows_mx4`) does, all uint8, `bias` `(F,)`; products exact, sums and bias in
+    fp32, one rounding to `dtype` (bf16, half or fp32). A scale byte of 255 makes the outputs that its group enters NaN. K a
+    multiple of 32; up to 2^21 rows and 2^21 features."""
+    n, xs, half = _layout(x, "x")
+    dev, k = x.device, 2 * half
+    if any(t.dtype != torch.uint8 for t in (x, x_scale, weight, weight_scale)):
+        raise TypeError(f"linear_mx4 takes uint8 codes and scales, got {x.dtype}, {x_scale.dtype}, {weight.dtype} and "
+                        f"{weight_scale.dtype}")
+    if weight.dim() != 2 or weight.shape[1] != half or k % Q4_GROUP:
+        raise ValueError(f"x must be (..., K / 2) and weight (F, K / 2), K a multiple of {Q4_GROUP}, got "
+                         f"{tuple(x.shape)} and {tuple(weight.shape)}")
+    code, groups = dtype_code(dtype), k // Q4_GROUP
+    if weight.device != dev or x_scale.device != dev or weight_scale.device != dev:
+        raise ValueError(f"weight and the scales must be on {dev}, got {weight.device}, {x_scale.device}, "
+                         f"{weight_scale.device}")
+    f, ws, _ = _layout(weight, "weight")
+    if x_scale.shape != (*x.shape[:-1], groups):
+        raise ValueError(f"x_scale must be {(*x.shape[:-1], groups)}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != (f, groups):
+        raise ValueError(f"weight_scale must be ({f}, {groups}), got {tuple(weight_scale.shape)}")
+    xss = groups if x_scale.is_contiguous() else _layout(x_scale, "x_scale")[1]
+    wss = groups if weight_scale.is_contiguous() else _layout(weight_scale, "weight_scale")[1]
+    bp = 0
+    if bias is not None:
+        bias = _f32_channels(bias, f, dev, "bias")
+        bp = bias.data_ptr()
+    out = _new((*x.shape[:-1], f), dtype, dev)
+    _lib.launch(_lib.load().hb_proj_mx4, "linear_mx4", dev, x.data_ptr(), xs, x_scale.data_ptr(), xss,
+                weight.data_ptr(), ws, weight_scale.data_ptr(), wss, bp, out.data_ptr(), code, f, n, k, f)
     return out

@@ -353,6 +353,68 @@ int hb_proj_q4(hipStream_t stream, const void* x, int dtype, int64_t x_row_strid
                int64_t w_row_stride, const void* w_scale, int64_t w_scale_row_stride, const float* bias, int silu,
                void* out, int64_t out_row_stride, int N, int K, int F);
 
+/* ---- Microscaled 4-bit rows --------------------------------------------------------------------------------
+ * A 4-bit row (OCP MX) holds e2m1 codes (sign, 2 exponent bits, 1 mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two per byte
+ * (the low nibble the even column), and one e8m0 scale byte s, 2^(s - 127), per 32 columns; it stands for the products.
+ * The form of hb_proj_q4's weights. No counterpart in the reference.
+ *   hb_quant_rows_mx4, hb_rms_modulate_mx4, hb_residual_rms_mx4, hb_glu_mx4 : hb_quant_rows, hb_rms_modulate_q8,
+ *   hb_residual_rms_q8 and hb_glu_q8 with 4-bit rows for 8-bit ones: y as there, in fp32, then per group of 32 columns the
+ *   least s, from 8 to 253, that brings the group's largest magnitude to 6 or below (127 for a group of zeros), and
+ *   e2m1(y 2^(127 - s)), round to nearest, ties to the even code. A group with a NaN or an infinity gets the byte 255,
+ *   which makes its 32 values NaN; the others of its row are as they would be (the norms spread a NaN or an infinity over
+ *   the row).
+ *   Operands as for the 8-bit forms; C, F multiples of 32, up to 16384 for the norms and 2^24 for the others; q: rows of
+ *   C / 2 bytes, 16-byte aligned with a stride that is a multiple of 16; q_scale: rows of C / 32 bytes, any stride.
+ * hb_proj_mx4 : out[m, f] = sum_k x[m, k] w[f, k] + bias[f], x (M, K) and w (F, K) 4-bit rows, on the 4-bit matrix cores:
+ *   products exact, sums and bias fp32, one rounding to out_dtype; bias: F floats or NULL. A scale byte 255 makes every
+ *   output that its group enters NaN. K a multiple of 32, M and F up to 2^21; code strides in bytes, multiples of 16 up to
+ *   2^22, 16-byte aligned; scale rows with any stride and alignment; out row stride >= F. */
+int hb_quant_rows_mx4(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, void* q,
+                      int64_t q_row_stride, void* q_scale, int64_t q_scale_row_stride, int64_t N, int C);
+int hb_rms_modulate_mx4(hipStream_t stream, const void* x, int dtype, int64_t x_row_stride, const float* weight,
+                        float eps, const void* scale, const void* shift, int64_t mod_batch_stride, int rows_per_batch,
+                        void* q, int64_t q_row_stride, void* q_scale, int64_t q_scale_row_stride, int64_t N, int C);
+int hb_residual_rms_mx4(hipStream_t stream, const void* h, int dtype, int64_t h_row_stride, const void* x,
+                        int64_t x_row_stride, const void* x_bias, const void* gate, int64_t gate_batch_stride,
+                        const void* local, int memory, const float* weight, float eps, const void* scale,
+                        const void* shift, int64_t mod_batch_stride, int rows_per_batch, void* out_h,
+                        int64_t out_h_row_stride, void* q, int64_t q_row_stride, void* q_scale,
+                        int64_t q_scale_row_stride, int64_t N, int C);
+int hb_glu_mx4(hipStream_t stream, const void* proj, int dtype, int64_t proj_row_stride, const float* bias, void* q,
+               int64_t q_row_stride, void* q_scale, int64_t q_scale_row_stride, int64_t N, int F);
+int hb_proj_mx4(hipStream_t stream, const void* x, int64_t x_row_stride, const void* x_scale,
+                int64_t x_scale_row_stride, const void* w, int64_t w_row_stride, const void* w_scale,
+                int64_t w_scale_row_stride, const float* bias, void* out, int out_dtype, int64_t out_row_stride,
+                int64_t M, int K, int F);
+
+/* ---- Attention over packed sequences -----------------------------------------------------------------------
+ * Plain (one-branch) softmax attention of N sequences of different lengths: prompts, clips of one batch, new tokens over
+ * the keys of their sequences. Sequence i has the queries offsets[i] .. offsets[i + 1] of q's T tokens and the keys
+ * key_offsets[i] .. key_offsets[i + 1] of k's and v's Tk, the first key_lengths[i] of them where key_lengths is given
+ * (slots of a cache with room behind). H heads of queries share G heads of keys (H a multiple of G): head h reads key
+ * head h / (H / G).
+ *   out[t, h] = sum_b softmax_b(scale q[t, h] . k[b]) v[b]
+ * over the keys of t's sequence; with `causal` != 0 over those up to t's place when the queries are the last of them:
+ * query a of lq sees keys b <= a + lk - lq. A row that sees no key is zero. A key that a row does not see takes no part in
+ * it, whatever its values are. Tokens of no sequence (before offsets[0], from offsets[N] on) are left as they were in out,
+ * or zeroed with `zero_rest` != 0.
+ *   offsets, key_offsets : N + 1 ascending ints on the device; key_lengths: N ints or NULL. They are read by the kernel, so a
+ *                          captured call follows their contents. Entries outside [0, T] ([0, Tk]) are taken as the nearest
+ *                          one inside; where they do not ascend, which values are written is not specified.
+ *   q, out (T, H, D), k, v (Tk, G, D) of `dtype`: strides in elements of tokens and heads, multiples of 8 (bf16, half) or 4
+ *                          (fp32), 16-byte aligned; k's and v's token strides up to 2^23.
+ *   dtype HB_BF16, HB_F16 (matrix products on operands of that type, probabilities rounded to it) or HB_F32 (fp32
+ *   throughout); statistics and sums fp32. D 64 or 128; scale > 0; T (H / G) up to 2^30, Tk up to 2^30, N up to 2^20.
+ *   workspace : >= hb_packed_workspace_size(...) bytes, 16-byte aligned; 0 (and NULL allowed) where the rows fill the card
+ *               by themselves, else the keys are split and the parts joined from it. One call's at a time. */
+size_t hb_packed_workspace_size(int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D);
+int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                        int64_t v_head_stride, int dtype, const int* offsets, const int* key_offsets,
+                        const int* key_lengths, int causal, float scale, void* out, int64_t out_token_stride,
+                        int64_t out_head_stride, int zero_rest, int64_t T, int64_t Tk, int N, int H, int G, int D,
+                        void* workspace, size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif
