@@ -125,7 +125,6 @@ struct Lds {
 template <class E, int D, int NW>
 struct KeyCopy {
   static constexpr int RB = D * E::ES, kRows = 1024 / RB, kBlocks = E::KT * RB / 1024 / NW;
-  static constexpr int kCopies = 2 * kBlocks;
   const uint8_t *k, *v;
   uint32_t koff[kBlocks], voff[kBlocks];
   int lk;
@@ -187,7 +186,7 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* sV, int dt, int g) {
   return u32x4{ux[0], ux[1], uy[0], uy[1]};
 }
 
-// The rows of a wave: what it holds between key tiles.
+// The rows of a wave, NCT times 32 of them, MFMA columns: what it holds between key tiles.
 template <class E, int D, int NCT>
 struct Rows {
   static constexpr int RT = E::KT / 32, kQ = D * E::ES / 32;  // 16-byte pieces of a query per lane
@@ -196,11 +195,31 @@ struct Rows {
   float m[NCT], l[NCT];
   int lim[NCT];  // keys that this lane's row sees
 
-  // One key tile; `masked`: some row does not see all of its KT keys from k0 on.
-  // `apart`: V's NaNs and infinities reach only the rows that see their keys.
-  __device__ __forceinline__ void step(const uint8_t* sK, const uint8_t* sV, int k0, float c, bool masked, bool apart) {
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      m[ct] = -INFINITY, l[ct] = 0.f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] = f32x16{};
+    }
+  }
+  // A total or a sum that is NaN or infinite.
+  __device__ __forceinline__ bool wild() const {
+    bool found = false;
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      found |= !(l[ct] < INFINITY);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) found |= !(fabsf(o[ct][dt][i]) < INFINITY);
+    }
+    return found;
+  }
+
+  // The scores of 32 RT keys.
+  __device__ __forceinline__ void scores(const uint8_t* sK, f32x16 (&sc)[NCT][RT]) const {
     const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
-    f32x16 sc[NCT][RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -220,46 +239,68 @@ struct Rows {
         }
       }
     }
-    u32x4 p[NCT][RT][2];  // 16-bit probabilities; fp32 ones stay in sc
+  }
+
+  // The scores' probabilities: 16-bit ones in p, fp32 ones in the scores' place. The reference m is a row's maximum over the
+  // first tile, and follows the maximum only where that has passed it by 2^kSlack: larger probabilities lose nothing while
+  // they are in range, and o is seldom multiplied. bf16 ones are to 2^127: the maximum of the tiles after the first is not
+  // looked at (causal, 8192 tokens, 24 heads of 64: 246 -> 233 us) unless `careful`. No row's sums depend on its neighbours.
+  static constexpr bool kWide = std::is_same<E, E16<Bf16Io>>::value;
+  static constexpr float kSlack = kWide ? 100.f : 8.f;
+  __device__ __forceinline__ void softmax(int ct, f32x16 (&sc)[RT], u32x4 (&p)[RT][2], int k0, float c, bool masked,
+                                          bool look) {
+    const int lh = (threadIdx.x & 63) >> 5;
+    if (masked) {
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      if (masked) {
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            sc[ct][rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[ct][rt][r] : -INFINITY;
-      }
+        for (int r = 0; r < 16; ++r) sc[rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[rt][r] : -INFINITY;
+    }
+    if (look) {
       float top = -INFINITY;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[ct][rt][r]);
-      top = fmaxf(top, __shfl_xor(top, 32, kWave)) * c;
-      const float mn = fmaxf(m[ct], top);
-      const float base = mn == -INFINITY ? 0.f : mn;  // every key so far masked: nothing to add up
-      const float alpha = fast_exp2(m[ct] - base);
-      m[ct] = mn;
-      l[ct] *= alpha;
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[rt][r]);
+      const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
+      const bool passed = top > m[ct] + kSlack;
+      if (__any(passed)) {
+        const float alpha = passed ? fast_exp2(m[ct] - top) : 1.f;
+        m[ct] = passed ? top : m[ct];
+        l[ct] *= alpha;
 #pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] *= alpha;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float e0 = fast_exp2(__fmaf_rn(sc[ct][rt][r], c, -base));
-          const float e1 = fast_exp2(__fmaf_rn(sc[ct][rt][r + 1], c, -base));
-          if constexpr (E::ES == 2) {
-            const uint32_t w = E::Io::pack2(e0, e1);
-            p[ct][rt][r >> 3][(r & 7) >> 1] = w;
-            l[ct] = add_pair<typename E::Io>(w, l[ct]);
-          } else {
-            sc[ct][rt][r] = e0, sc[ct][rt][r + 1] = e1;
-            l[ct] += e0 + e1;
-          }
-        }
+        for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] *= alpha;
+      }
     }
-    if (__builtin_expect(masked && apart, 0)) return add_apart(sV, k0, sc, p);
+    const float base = m[ct] == -INFINITY ? 0.f : m[ct];  // every key so far masked: nothing to add up
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float e0 = fast_exp2(__fmaf_rn(sc[rt][r], c, -base));
+        const float e1 = fast_exp2(__fmaf_rn(sc[rt][r + 1], c, -base));
+        if constexpr (E::ES == 2) {
+          const uint32_t w = E::Io::pack2(e0, e1);
+          p[rt][r >> 3][(r & 7) >> 1] = w;
+          l[ct] = add_pair<typename E::Io>(w, l[ct]);
+        } else {
+          sc[rt][r] = e0, sc[rt][r + 1] = e1;
+          l[ct] += e0 + e1;
+        }
+      }
+  }
+
+  // One key tile; `masked`: some row does not see all of its keys from k0 on. `careful`: every maximum is looked at, and V's
+  // NaNs and infinities reach only the rows that see their keys.
+  __device__ __forceinline__ void step(const uint8_t* sK, const uint8_t* sV, int k0, float c, bool masked, bool first,
+                                       bool careful) {
+    f32x16 sc[NCT][RT];
+    u32x4 p[NCT][RT][2];
+    scores(sK, sc);
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) softmax(ct, sc[ct], p[ct], k0, c, masked, !kWide || first || careful);
+    if (__builtin_expect(masked && careful, 0)) return add_apart(sV, k0, sc, p);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
       if constexpr (E::ES == 2) {
@@ -362,9 +403,9 @@ struct Rows {
   }
 };
 
-// A NaN or an infinity in the values of a key that a row does not see meets a probability of zero, and their product is NaN.
-// Values are seldom so: the sums are taken as they come, and a workgroup that finds a NaN in them repeats its tile with
-// such values of masked tiles apart. The other rows get the same sums as without them, bit for bit.
+// A NaN or an infinity in the values of a key that a row does not see meets a probability of zero, and their product is NaN;
+// a score 2^127 above the reference gives an infinity. Both are rare: the sums are taken as they come, and a workgroup that
+// finds a NaN or an infinity in them repeats its tile with care. The other rows get the same sums as before, bit for bit.
 template <class E, int D, int NCT, int NW, int WAVES>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) void attend_kernel(const Args a) {
   using L = Lds<E, D>;
@@ -400,47 +441,36 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
   const int begin = part * each, end = begin + each < all ? begin + each : all;
 
   Rows<E, D, NCT> w;
-  int64_t row_of[NCT];  // token, head
+  int64_t token[NCT];
   int head[NCT];
 #pragma unroll
   for (int ct = 0; ct < NCT; ++ct) {
     const int r = r0 + 32 * ct + lr, rc = r < rows ? r : rows - 1, at = rc / a.gs;
-    row_of[ct] = t.q0 + at;
+    token[ct] = t.q0 + at;
     head[ct] = g * a.gs + rc - at * a.gs;
     w.lim[ct] = sees(r);
-    const uint8_t* p = a.q + row_of[ct] * a.q_ts + head[ct] * a.q_hs;
+    const uint8_t* p = a.q + token[ct] * a.q_ts + head[ct] * a.q_hs;
 #pragma unroll
     for (int i = 0; i < Rows<E, D, NCT>::kQ; ++i) w.q[ct][i] = ld16(p + 32 * i + 16 * lh);
   }
   const uint32_t lds0 = lds_addr(smem);
-  for (bool apart = false;; apart = true) {
-#pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      w.m[ct] = -INFINITY, w.l[ct] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) w.o[ct][dt] = f32x16{};
-    }
+  for (bool careful = false;; careful = true) {
+    w.clear();
     if (begin < end) {
       const KeyCopy<E, D, NW> copy(a, t, g);
       copy(begin, lds0);
       int stage = 0;
       for (int k0 = begin; k0 < end; k0 += E::KT, stage ^= 1) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies of the tile
-        __syncthreads();                                  // everybody's, and the other stage is free
+        // vmcnt(0): this wave's copies of the tile. As the builtin, which the compiler counts: after assembly it would wait for
+        // the queries' loads inside the loop, and with them for the copies of the next tile (one token 89 -> 65 us).
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+        __syncthreads();  // everybody's, and the other stage is free
         if (k0 + E::KT < end) copy(k0 + E::KT, lds0 + (stage ^ 1) * L::kStage);
         const uint8_t* s = smem + stage * L::kStage;
-        if (k0 < most) w.step(s, s + L::kTile, k0, a.c, k0 + E::KT > least, apart);
+        if (k0 < most) w.step(s, s + L::kTile, k0, a.c, k0 + E::KT > least, k0 == begin, careful);
       }
     }
-    if (apart) break;
-    bool nan = false;
-#pragma unroll
-    for (int ct = 0; ct < NCT; ++ct)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) nan |= w.o[ct][dt][i] != w.o[ct][dt][i];
-    if (!__syncthreads_or(nan)) break;  // (and the stages are free)
+    if (careful || !__syncthreads_or(w.wild())) break;  // (and the stages are free)
   }
 
 #pragma unroll
@@ -448,19 +478,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
     const float total = w.l[ct] + __shfl_xor(w.l[ct], 32, kWave);
     if (r0 + 32 * ct + lr >= rows) continue;
     if (a.splits > 1) {
-      const int64_t n = (static_cast<int64_t>(part) * a.T + row_of[ct]) * a.H + head[ct];
-      float* po = a.part_o + n * D;
+      const int64_t at = (static_cast<int64_t>(part) * a.T + token[ct]) * a.H + head[ct];
+      float* po = a.part_o + at * D;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * i + 4 * lh) =
               f32x4{w.o[ct][dt][4 * i], w.o[ct][dt][4 * i + 1], w.o[ct][dt][4 * i + 2], w.o[ct][dt][4 * i + 3]};
-      if (lh == 0) a.part_ml[2 * n] = w.m[ct], a.part_ml[2 * n + 1] = total;
+      if (lh == 0) a.part_ml[2 * at] = w.m[ct], a.part_ml[2 * at + 1] = total;
       continue;
     }
     const float inv = total == 0.f ? 0.f : __frcp_rn(total);
-    uint8_t* orow = a.out + row_of[ct] * a.o_ts + head[ct] * a.o_hs;
+    uint8_t* orow = a.out + token[ct] * a.o_ts + head[ct] * a.o_hs;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll

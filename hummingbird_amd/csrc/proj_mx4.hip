@@ -52,18 +52,21 @@ __device__ __forceinline__ f32x4 mfma_16x16x128(u32x4 a, u32x4 b, f32x4 c, uint3
                                                           static_cast<int>(sb));
 }
 
-// As lds_dma4 with an address per lane.
-__device__ __forceinline__ void lds_dma4_any(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "m0");
+// A pointer that is the same in every lane, in scalar registers.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uintptr_t>(p);
+  const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+  const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)));
+  return reinterpret_cast<const uint8_t*>(hi << 32 | lo);
 }
 
 // ---- Tiled product ------------------------------------------------------------------------------------------
 // A workgroup of WF x WM waves computes FT features x MT rows in steps of 256 columns, which stream through kStages LDS
 // stages: code rows of 128 bytes whose 16-byte chunks are XOR-swizzled, then the rows' scales. A wave multiplies NF x NM
-// tiles of 32 x 32.
-// RAGGED: K ends inside a stage, or scale rows that are not whole dwords. A row's eight scales of a stage then lie in two
-// or three dwords, the first with up to three bytes of what is before them: the dwords are copied whole (each holds at
-// least a byte of the row), 16 bytes a row, and shifted when they are used.
+// tiles of 32 x 32, of one 64-column block after the other, and reads the next block's operands meanwhile.
+// The scales are copied for kChunk steps at once, 32 bytes a row, into kBufs buffers of their own.
+// RAGGED: K ends inside two steps, or scale rows that are not aligned to 16 bytes. The scales of two steps then lie in two
+// 16-byte pieces, which are copied whole (each holds at least a byte of the row) and read from where they start.
 template <int FT_, int MT_, int WF_, int WM_, int WAVES_, int STAGES_ = 2>
 struct Tile {
   static constexpr int FT = FT_, MT = MT_, WF = WF_, WM = WM_;
@@ -76,12 +79,15 @@ struct Tile {
 };
 template <class TL, bool RAGGED>
 struct Stage {
-  static constexpr int kRows = TL::FT + TL::MT;
-  static constexpr int kScaleRow = RAGGED ? 16 : 8;  // bytes
-  static constexpr int kScales = kRows * kStep;      // where the scales start
-  static constexpr int kBytes = kRows * (kStep + kScaleRow);
-  static constexpr int kScaleBlocks = kRows * kScaleRow / 256;  // copies of 256 bytes; a wave's past the last repeat it
+  static constexpr int kRows = TL::FT + TL::MT, kBytes = kRows * kStep;
+  static constexpr int kChunk = RAGGED ? 2 : 4;  // steps whose scales are copied together
+  static constexpr int kScaleRow = 32, kScaleBytes = kRows * kScaleRow;
+  // A chunk's copies start kStages steps before it, when the last reads of the chunk whose buffer it takes are over:
+  // kBufs - 1 chunks, of two steps or (RAGGED) one where they are K's last, are kStages - 1 steps at least.
+  static constexpr int kBufs = RAGGED ? TL::kStages : (TL::kStages + 2) / 2;
+  static constexpr int kScaleBlocks = kScaleBytes / 1024;  // copies; a wave's past the last repeat it
   static constexpr int kBlocksS = (kScaleBlocks + TL::NW - 1) / TL::NW;
+  static constexpr int kLds = TL::kStages * kBytes + kBufs * kScaleBytes;
 };
 
 // The copies of a stage by one wave: of the codes, blocks wv, wv + NW, ... of the A rows (features), then of the B rows,
@@ -93,14 +99,14 @@ struct StageCopy {
   const uint8_t* w0;
   const uint8_t* x0;
   uint32_t aoff[TL::kBlocksA], boff[TL::kBlocksB];
-  const uint8_t* sp[St::kBlocksS];  // this lane's dword of step 0
+  const uint8_t* sp[St::kBlocksS];  // this lane's 16 bytes of the first chunk
   int srem[St::kBlocksS];           // bytes from it to its row's end
   const int wv = wave_id() % TL::NW, r8 = (threadIdx.x & 63) >> 3, chunk = (threadIdx.x & 7) ^ r8 ^ (wv & 1);
 
   // Aims the copies at the tile of feature f0 and row m0. Rows past an end read the last one; their results are not stored.
   __device__ __forceinline__ void aim(const Args& a, int f0, int64_t m0) {
-    w0 = a.w + f0 * a.w_rs;
-    x0 = a.x + m0 * a.x_rs;
+    w0 = uniform(a.w + f0 * a.w_rs);
+    x0 = uniform(a.x + m0 * a.x_rs);
     const int lastf = a.F - 1 - f0;
     const int64_t lastm = a.M - 1 - m0;
 #pragma unroll
@@ -113,91 +119,91 @@ struct StageCopy {
       const int r = 8 * (wv + TL::NW * u) + r8;
       boff[u] = static_cast<uint32_t>((r < lastm ? r : lastm) * a.x_rs) + 16 * chunk;
     }
-    constexpr int kDwords = St::kScaleRow / 4, kPer = 64 / kDwords;  // dwords a row, rows a block
-    const int lane = threadIdx.x & 63, d = lane % kDwords;
+    constexpr int kPieces = 2, kPer = 64 / kPieces;  // 16-byte pieces a row, rows a block
+    const int lane = threadIdx.x & 63, piece = lane % kPieces;
 #pragma unroll
     for (int u = 0; u < St::kBlocksS; ++u) {
-      int block = wv + TL::NW * u;
-      if (block > St::kScaleBlocks - 1) block = St::kScaleBlocks - 1;
+      const int block = scale_block(u);
       const bool isa = block * kPer < TL::FT;
-      const int r = block * kPer + lane / kDwords - (isa ? 0 : TL::FT);
+      const int r = block * kPer + lane / kPieces - (isa ? 0 : TL::FT);
       const int64_t last = isa ? lastf : lastm, rr = r < last ? r : last;
       const uint8_t* row = isa ? a.sw + (f0 + rr) * a.sw_rs : a.sx + (m0 + rr) * a.sx_rs;
-      const int ahead = RAGGED ? static_cast<int>(reinterpret_cast<uintptr_t>(row) & 3) : 0;
-      sp[u] = row - ahead + 4 * d;
-      srem[u] = 4 * d < ahead + 8 ? a.K / kGroup + ahead - 4 * d : 0;
+      const int ahead = RAGGED ? static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) : 0;
+      sp[u] = row - ahead + 16 * piece;
+      srem[u] = a.K / kGroup + ahead - 16 * piece;
     }
   }
-  // Copy u of step s, to the stage at LDS byte address `stage`.
+  __device__ __forceinline__ int scale_block(int u) const {
+    const int block = wv + TL::NW * u;
+    return block < St::kScaleBlocks ? block : St::kScaleBlocks - 1;
+  }
+  // Copy u of step s's codes, to the stage at LDS byte address `stage`.
   __device__ __forceinline__ void one(int u, int s, int K, uint32_t stage) const {
     const int k = s * kStep;  // byte of the rows
-    if (u < TL::kBlocksA + TL::kBlocksB) {
-      const bool a = u < TL::kBlocksA;
-      const uint8_t* base = (a ? w0 : x0) + k;
-      const uint32_t off = a ? aoff[a ? u : 0] : boff[a ? 0 : u - TL::kBlocksA];
-      const uint32_t to = stage + (a ? 0 : TL::FT * kStep) + (wv + TL::NW * (a ? u : u - TL::kBlocksA)) * 1024;
-      if constexpr (RAGGED) lds_dma16_any(k + 16 * chunk < K / 2 ? base + off : zeros, to);
-      else lds_dma16(base, off, to);
-    } else {
-      const int i = u - TL::kBlocksA - TL::kBlocksB;
-      int block = wv + TL::NW * i;
-      if (block > St::kScaleBlocks - 1) block = St::kScaleBlocks - 1;
-      const uint32_t to = stage + St::kScales + 256 * block;
-      if constexpr (RAGGED) lds_dma4_any(8 * s < srem[i] ? sp[i] + 8 * s : zeros, to);
-      else lds_dma4_any(sp[i] + 8 * s, to);
-    }
+    const bool a = u < TL::kBlocksA;
+    const uint8_t* base = (a ? w0 : x0) + k;
+    const uint32_t off = a ? aoff[a ? u : 0] : boff[a ? 0 : u - TL::kBlocksA];
+    const uint32_t to = stage + (a ? 0 : TL::FT * kStep) + (wv + TL::NW * (a ? u : u - TL::kBlocksA)) * 1024;
+    if constexpr (RAGGED) lds_dma16_any(k + 16 * chunk < K / 2 ? base + off : zeros, to);
+    else lds_dma16(base, off, to);
   }
-  static constexpr int kCopies = TL::kBlocksA + TL::kBlocksB + St::kBlocksS;
-};
-
-// Half a stage of a wave's operands: two blocks of 32 columns of each of its rows, lane half lh the blocks
-// 4 lh + 2 kk + 0, 1, and the scales of lane half lh's four.
-template <class TL, bool RAGGED>
-struct Frags {
-  using St = Stage<TL, RAGGED>;
-  u32x4 a[TL::NF][2], b[TL::NM][2];
-  uint32_t sa[TL::NF][RAGGED ? 2 : 1], sb[TL::NM][RAGGED ? 2 : 1];
-  static constexpr int kTwo = 2 * (TL::NF + TL::NM), kReads = kTwo + TL::NF + TL::NM;
-  __device__ __forceinline__ void read(int i, const uint8_t* st, int fw, int mw, int kk) {
-    const int lr = threadIdx.x & 31, lh = (threadIdx.x & 63) >> 5;
-    if (i < kTwo) {
-      const int c = 4 * lh + 2 * kk + (i & 1), t = i >> 1;
-      if (t < TL::NF) a[t][i & 1] = *reinterpret_cast<const u32x4*>(st + swz_byte(fw + 32 * t + lr, c));
-      else
-        b[t - TL::NF][i & 1] =
-            *reinterpret_cast<const u32x4*>(st + TL::FT * kStep + swz_byte(mw + 32 * (t - TL::NF) + lr, c));
-      return;
-    }
-    const int t = i - kTwo;
-    const int row = t < TL::NF ? fw + 32 * t + lr : TL::FT + mw + 32 * (t - TL::NF) + lr;
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(st + St::kScales + St::kScaleRow * row + 4 * lh);
+  // The scales of the chunk that starts at step s to the buffer at LDS byte address `buf`. Pieces past a row's end come from
+  // `zeros` (without RAGGED K is a multiple of 512: a piece lies before the end or past it).
+  __device__ __forceinline__ void scales(int s, uint32_t buf) const {
 #pragma unroll
-    for (int j = 0; j < (RAGGED ? 2 : 1); ++j) {
-      if (t < TL::NF) sa[t][j] = p[j];
-      else sb[t - TL::NF][j] = p[j];
-    }
+    for (int u = 0; u < St::kBlocksS; ++u)
+      lds_dma16_any(8 * s < srem[u] ? sp[u] + 8 * s : zeros, buf + 1024 * scale_block(u));
+  }
+  static constexpr int kCopies = TL::kBlocksA + TL::kBlocksB;
+};
+
+// A wave's operands of block J of a stage: lane half lh's 32 columns of each of its rows, chunk 4 lh + J.
+template <class TL>
+struct Block {
+  u32x4 a[TL::NF], b[TL::NM];
+  static constexpr int kReads = TL::NF + TL::NM;
+  __device__ __forceinline__ void read(int t, const uint8_t* st, int fw, int mw, int j) {
+    const int lr = threadIdx.x & 31, lh = (threadIdx.x & 63) >> 5, c = 4 * lh + j;
+    if (t < TL::NF) a[t] = *reinterpret_cast<const u32x4*>(st + swz_byte(fw + 32 * t + lr, c));
+    else b[t - TL::NF] = *reinterpret_cast<const u32x4*>(st + TL::FT * kStep + swz_byte(mw + 32 * (t - TL::NF) + lr, c));
   }
 };
 
-// The scales of a lane half's four blocks out of the dwords that hold them: `shift` bytes in, those past K left out.
-__device__ __forceinline__ uint32_t scale_of(const uint32_t (&d)[1], uint32_t, uint32_t) { return d[0]; }
-__device__ __forceinline__ uint32_t scale_of(const uint32_t (&d)[2], uint32_t shift, uint32_t mask) {
-  return __builtin_amdgcn_alignbyte(d[1], d[0], shift) & mask;
-}
+// The scales of a step: of lane half lh's four blocks, a byte each.
+template <class TL, bool RAGGED>
+struct Scales {
+  using St = Stage<TL, RAGGED>;
+  static constexpr int kDwords = RAGGED ? 2 : 1;
+  uint32_t raw[TL::NF + TL::NM][kDwords];
+  // From the buffer `buf`, of the chunk's step `at`; `ahead`: where in its first piece the row starts.
+  __device__ __forceinline__ void read(int t, const uint8_t* buf, int at, int fw, int mw, uint32_t ahead) {
+    const int lr = threadIdx.x & 31, lh = (threadIdx.x & 63) >> 5;
+    const int row = t < TL::NF ? fw + 32 * t + lr : TL::FT + mw + 32 * (t - TL::NF) + lr;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(buf + St::kScaleRow * row + 8 * at + 4 * lh + (ahead & ~3u));
+#pragma unroll
+    for (int j = 0; j < kDwords; ++j) raw[t][j] = p[j];
+  }
+  // Out of the dwords that hold them, those past K (`mask`) left out.
+  __device__ __forceinline__ uint32_t get(int t, uint32_t ahead, uint32_t mask) const {
+    if constexpr (RAGGED) return __builtin_amdgcn_alignbyte(raw[t][1], raw[t][0], ahead & 3) & mask;
+    else return raw[t][0];
+  }
+};
 
 template <class TL>
 int64_t tiles_of(const Args& a) {
   return static_cast<int64_t>((a.F + TL::FT - 1) / TL::FT) * ((a.M + TL::MT - 1) / TL::MT);
 }
 
-// The loop of the 8-bit product (proj_q8.hip), with steps of 256 columns: workgroups stay and their copies run kStages
-// steps ahead across the tiles' ends.
+// Workgroups stay: each takes every gridDim.x-th tile, and its copies run kStages steps ahead of the products across
+// the tiles' ends, so that a tile's first steps land while the one before it is finished and stored. Past the last tile they
+// copy that tile's columns again, for nothing: the loop has no branch around a copy, and the kernel waits for them
+// before it ends.
 template <typename T, class TL, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL::kWaves, TL::kWaves))) void tiled_kernel(
     const Args a) {
   using St = Stage<TL, RAGGED>;
-  __shared__ __attribute__((aligned(16))) uint8_t smem[TL::kStages * St::kBytes];
-  __shared__ __attribute__((aligned(16))) float bias[2][TL::FT];  // of a tile and of the next
+  __shared__ __attribute__((aligned(16))) uint8_t smem[St::kLds];
   const int nf = (a.F + TL::FT - 1) / TL::FT, nm = static_cast<int>((a.M + TL::MT - 1) / TL::MT), tiles = nf * nm;
   // Groups of eight feature tiles walk the row tiles together, and the workgroups of an XCD take consecutive tiles, so
   // that both operands are read from its L2.
@@ -211,11 +217,14 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5;
   const int wv = wave_id(), fw = wv % TL::WF * (32 * TL::NF), mw = wv / TL::WF * (32 * TL::NM);
   const uint32_t lds0 = lds_addr(smem);
+  constexpr uint32_t kScales0 = TL::kStages * St::kBytes, kScalesEnd = St::kLds;
   const int nk = (a.K + kCols - 1) / kCols;
 
-  // What is copied next: step `cs` of tile `ct` (in the order of p).
+  // What is copied next: step `cs` of tile `ct` (in the order of p), its scales to the buffer at `cbuf`.
   StageCopy<TL, RAGGED> copy;
   int ct = blockIdx.x, cs = 0;
+  uint32_t cbuf = kScales0;
+  auto next_buf = [](uint32_t x) { return x + St::kScaleBytes == kScalesEnd ? kScales0 : x + St::kScaleBytes; };
   auto aim = [&]() {
     int f0;
     int64_t m0;
@@ -223,128 +232,142 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     copy.aim(a, f0, m0);
   };
   auto advance = [&]() {
-    if (++cs < nk) return;
+    if (++cs < nk) {
+      if (cs % St::kChunk == 0) cbuf = next_buf(cbuf);
+      return;
+    }
     cs = 0;
+    cbuf = next_buf(cbuf);
     if (ct + static_cast<int>(gridDim.x) >= tiles) return;
     ct += gridDim.x;
     aim();
   };
-  using Fr = Frags<TL, RAGGED>;
-  constexpr int kTiles = TL::NF * TL::NM, kReads = Fr::kReads, kCopies = StageCopy<TL, RAGGED>::kCopies;
-  auto copy_bias = [&](int f0, int set) {  // 64 features by a wave, copied while the tile's first step runs
-    if (!a.bias || 64 * wv >= TL::FT) return;
-    const int i = 64 * wv + lane, f = i < a.F - 1 - f0 ? i : a.F - 1 - f0;
-    lds_dma4(a.bias + f0, 4 * f, lds_addr(bias[set]) + 256 * wv);
+  constexpr int kTiles = TL::NF * TL::NM, kReads = Block<TL>::kReads, kCopies = StageCopy<TL, RAGGED>::kCopies;
+  // A step has four blocks of kTiles products. When its last block is in registers everywhere and the next step's copies
+  // have landed (the one barrier of a step, before the last block's products), the stage is free: the step kStages on is
+  // copied into it, kFirst copies among the last block's products and the others among the next step's first.
+  constexpr int kFirst = kCopies / 2;
+  auto chunk = [&]() {
+    if (cs % St::kChunk == 0) copy.scales(cs, __builtin_amdgcn_readfirstlane(lds0 + cbuf));
   };
-  if (!a.bias && threadIdx.x < TL::FT) bias[0][threadIdx.x] = bias[1][threadIdx.x] = 0.f;
   aim();
 #pragma unroll
   for (int i = 0; i < TL::kStages; ++i) {
 #pragma unroll
-    for (int u = 0; u < kCopies; ++u) copy.one(u, cs, a.K, lds0 + i * St::kBytes);
-    advance();
+    for (int u = 0; u < (i == TL::kStages - 1 ? kFirst : kCopies); ++u) {
+      if (u == 0 && i < TL::kStages - 1) chunk();
+      copy.one(u, cs, a.K, lds0 + i * St::kBytes);
+    }
+    if (i < TL::kStages - 1) advance();
   }
-  wait_copies<(TL::kStages - 1) * kCopies>();
+  wait_copies<(TL::kStages - 2) * kCopies + kFirst>();
   wait_lds();
   barrier();
-  Fr lo, hi;
+  uint32_t ahead[kReads] = {};  // where in its first piece a row's scales start, of the tile whose scales are read next
+  auto find_ahead = [&](int tile) {
+    if constexpr (RAGGED) {
+      int f0;
+      int64_t m0;
+      origin(tile, f0, m0);
 #pragma unroll
-  for (int i = 0; i < kReads; ++i) lo.read(i, smem, fw, mw, 0);
+      for (int t = 0; t < kReads; ++t) {
+        const int f = f0 + fw + 32 * t + lr;
+        const int64_t m = m0 + mw + 32 * (t - TL::NF) + lr;
+        const uint64_t at = t < TL::NF
+                                ? reinterpret_cast<uintptr_t>(a.sw) + static_cast<int64_t>(f < a.F ? f : a.F - 1) * a.sw_rs
+                                : reinterpret_cast<uintptr_t>(a.sx) + (m < a.M ? m : a.M - 1) * a.sx_rs;
+        ahead[t] = static_cast<uint32_t>(at) & 15;
+      }
+    }
+  };
+  find_ahead(blockIdx.x);
+  uint32_t sbuf = kScales0;  // the buffer of the next scales
+  Block<TL> blk[2];
+  Scales<TL, RAGGED> next;
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) blk[0].read(i, smem, fw, mw, 0), next.read(i, smem + sbuf, 0, fw, mw, ahead[i]);
 
-  // A step of a wave is 2 kTiles pairs of products, lo's and hi's. In the first kFree the operands of hi are read; then
-  // every wave has the whole stage in registers (barrier) and the step kStages on is copied into it, over kTiles pairs.
-  // Before hi's products the next step's copies, issued kStages - 1 steps ago, have landed (barrier), and its lo is read
-  // during them.
-  constexpr int kFree = kTiles / 2;                            // 0: one barrier does for both
-  constexpr int kEarly = (kTiles - kFree) * kCopies / kTiles;  // copies issued before the second barrier
-  constexpr int kLater = (TL::kStages - 2) * kCopies;          // copies of the steps between the next and that one
-  uint32_t b = 0;                                              // byte offset of the step's stage
-  int set = 0;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, set ^= 1) {
+  uint32_t b = 0;                                                                     // byte offset of the step's stage
+  uint32_t late = __builtin_amdgcn_readfirstlane(lds0 + (TL::kStages - 1) * St::kBytes);  // the stage whose copies go on
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     int f0;
     int64_t m0;
     origin(tile, f0, m0);
-    copy_bias(f0, set);
-    uint32_t sha[TL::NF] = {}, shb[TL::NM] = {};  // where in its first dword a row's scales start
-    if constexpr (RAGGED) {
-#pragma unroll
-      for (int t = 0; t < TL::NF; ++t) {
-        const int f = f0 + fw + 32 * t + lr;
-        sha[t] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.sw) + (f < a.F ? f : a.F - 1) * a.sw_rs) & 3;
-      }
-#pragma unroll
-      for (int t = 0; t < TL::NM; ++t) {
-        const int64_t m = m0 + mw + 32 * t + lr;
-        shb[t] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.sx) + (m < a.M ? m : a.M - 1) * a.sx_rs) & 3;
-      }
-    }
     f32x16 acc[TL::NF][TL::NM];
 #pragma unroll
     for (int i = 0; i < TL::NF; ++i)
 #pragma unroll
       for (int j = 0; j < TL::NM; ++j) acc[i][j] = f32x16{};
+#pragma unroll 1
     for (int s = 0; s < nk; ++s) {
-      const uint32_t stage = __builtin_amdgcn_readfirstlane(lds0 + b);
-      const int step = cs;
+      chunk();  // with the copies that go on among the first block's products
       uint32_t mask = ~0u;  // the bytes of a lane half's scales that lie before K
       if constexpr (RAGGED) {
         const int n = a.K / kGroup - 8 * s - 4 * lh;
         mask = n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1;
       }
-      auto copies = [&](int j) {  // those of product j past the barrier
+      uint32_t sc[kReads];
 #pragma unroll
-        for (int u = j * kCopies / kTiles; u < (j + 1) * kCopies / kTiles; ++u) copy.one(u, step, a.K, stage);
-      };
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        if (kFree == 0 || i < kFree) {
-          constexpr int n = kFree == 0 ? kTiles : kFree;
-#pragma unroll
-          for (int r = i * kReads / n; r < (i + 1) * kReads / n; ++r) hi.read(r, smem + b, fw, mw, 1);
-        }
-        if (kFree > 0 && i == kFree) {
+      for (int t = 0; t < kReads; ++t) sc[t] = next.get(t, ahead[t], mask);
+      // the next step's scales: the chunk's next ones, or a new chunk's first
+      const bool over = s + 1 == nk;
+      const int at = over ? 0 : (s + 1) % St::kChunk;
+      if (!at) sbuf = next_buf(sbuf);
+      if (RAGGED && over) find_ahead(tile + gridDim.x < static_cast<unsigned>(tiles) ? tile + gridDim.x : tile);
+      const uint8_t* const here = smem + b;
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + b);
+      b = b == (TL::kStages - 1) * St::kBytes ? 0 : b + St::kBytes;
+      auto block = [&](auto which) {
+        constexpr int J = decltype(which)::value;
+        if constexpr (J == 3) {
+          wait_copies<(TL::kStages - 2) * kCopies>();
           wait_lds();
           barrier();
         }
-        if (kFree > 0 && i >= kFree) copies(i - kFree);
-        const int ti = i / TL::NM, tj = i % TL::NM;
-        const uint32_t sa = scale_of(lo.sa[ti], sha[ti], mask), sb = scale_of(lo.sb[tj], shb[tj], mask);
-        acc[ti][tj] = mfma_32x32x64<0>(lo.a[ti][0], lo.b[tj][0], acc[ti][tj], sa, sb);
-        acc[ti][tj] = mfma_32x32x64<1>(lo.a[ti][1], lo.b[tj][1], acc[ti][tj], sa, sb);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      wait_copies<kLater + (kFree == 0 ? 0 : kEarly)>();
-      if (kFree == 0) wait_lds();
-      barrier();
-      b = b == (TL::kStages - 1) * St::kBytes ? 0 : b + St::kBytes;
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        if (kFree == 0) copies(i);
-        else if (i < kFree) copies(kTiles - kFree + i);
-        // (after the very last step, of a stage that nothing needs)
+        for (int i = 0; i < kTiles; ++i) {
 #pragma unroll
-        for (int r = i * kReads / kTiles; r < (i + 1) * kReads / kTiles; ++r) lo.read(r, smem + b, fw, mw, 0);
-        const int ti = i / TL::NM, tj = i % TL::NM;
-        const uint32_t sa = scale_of(hi.sa[ti], sha[ti], mask), sb = scale_of(hi.sb[tj], shb[tj], mask);
-        acc[ti][tj] = mfma_32x32x64<2>(hi.a[ti][0], hi.b[tj][0], acc[ti][tj], sa, sb);
-        acc[ti][tj] = mfma_32x32x64<3>(hi.a[ti][1], hi.b[tj][1], acc[ti][tj], sa, sb);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      advance();
-    }
-    if (nk < TL::kStages - 1) {  // the bias's copy is among those that the last wait left
-      wait_copies<0>();
-      barrier();
+          for (int r = i * kReads / kTiles; r < (i + 1) * kReads / kTiles; ++r) {
+            // (after the very last step, of a stage that nothing needs)
+            blk[(J + 1) & 1].read(r, J == 3 ? smem + b : here, fw, mw, (J + 1) & 3);
+            if constexpr (J == 3) next.read(r, smem + sbuf, at, fw, mw, ahead[r]);
+          }
+          if constexpr (J == 0 || J == 3) {
+            constexpr int kFrom = J == 3 ? 0 : kFirst, kNum = J == 3 ? kFirst : kCopies - kFirst;
+#pragma unroll
+            for (int u = i * kNum / kTiles; u < (i + 1) * kNum / kTiles; ++u)
+              copy.one(kFrom + u, cs, a.K, J == 3 ? to : late);
+          }
+          const int ti = i / TL::NM, tj = i % TL::NM;
+          acc[ti][tj] = mfma_32x32x64<J>(blk[J & 1].a[ti], blk[J & 1].b[tj], acc[ti][tj], sc[ti], sc[TL::NF + tj]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (J == 0) advance();
+      };
+      block(std::integral_constant<int, 0>{});
+      block(std::integral_constant<int, 1>{});
+      block(std::integral_constant<int, 2>{});
+      block(std::integral_constant<int, 3>{});
+      late = to;
     }
 #pragma unroll
     for (int n = 0; n < TL::NF; ++n) {
       __builtin_amdgcn_sched_barrier(0);  // the biases of one n at a time: registers
-      float bs[16];
+      float bs[16] = {};
+      if (a.bias) {
+        const int fn = f0 + fw + 32 * n;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 b4 = *reinterpret_cast<const f32x4*>(bias[set] + fw + 32 * n + 8 * g + 4 * lh);
+        for (int g = 0; g < 4; ++g) {
+          const int f = fn + 8 * g + 4 * lh;
+          if (fn + 32 <= a.F) {
+            const f32x4 b4 = *reinterpret_cast<const f32x4_align4*>(a.bias + f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bs[4 * g + j] = b4[j];
+            for (int j = 0; j < 4; ++j) bs[4 * g + j] = b4[j];
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bs[4 * g + j] = a.bias[f + j < a.F ? f + j : a.F - 1];
+          }
+        }
       }
 #pragma unroll
       for (int t = 0; t < TL::NM; ++t) {
@@ -358,10 +381,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   wait_copies<0>();
 }
 
-// Whether the scale rows are whole dwords and K whole stages.
+// Whether K ends inside two stages, or the scale rows are not 16-byte aligned.
 bool is_ragged(const Args& a) {
-  auto odd = [](const uint8_t* p, int64_t rs) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(rs)) & 3; };
-  return a.K % kCols || odd(a.sx, a.sx_rs) || odd(a.sw, a.sw_rs);
+  auto odd = [](const uint8_t* p, int64_t rs) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(rs)) & 15; };
+  return a.K % (2 * kCols) || odd(a.sx, a.sx_rs) || odd(a.sw, a.sw_rs);
 }
 
 template <typename T, class TL>

@@ -139,6 +139,21 @@ def test_large_scores(name):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+def test_scores_far_above_the_first_ones(name):
+    """Later keys whose scores pass the first tile's by more than any type's exponent range holds, in steps."""
+    announce("packed far scores", name)
+    D, n = 64, 330
+    q, k, v = make(name, n, n, 2, 1, D, 17)
+    q[..., 0] = 4.0
+    for step in (30.0, 90.0, 126.0, 400.0):
+        kk = (k * 0.1).contiguous()
+        kk[..., 0] = torch.div(torch.arange(n, device=DEV), 64, rounding_mode="floor")[:, None] * step
+        for causal in (False, True):
+            got = pa.packed_attention(q, kk, v, offsets([n]), causal=causal, scale=0.25)
+            check(got, q, kk, v, [n], [n], [0], causal, 0.25, name, (step, causal))
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
 @pytest.mark.parametrize("D", [64, 128])
 def test_values_of_keys_that_are_not_seen(name, D):
     """NaN and infinities in keys and values that a row does not see (later ones of its own sequence, the next sequence's,
