@@ -516,17 +516,30 @@ __global__ __launch_bounds__(256) void join_kernel(const Args a) {
   const int token = static_cast<int>(n / a.H), head = static_cast<int>(n - static_cast<int64_t>(token) * a.H);
   const int first = clamp_to(a.off[0], 0, a.T);
   if (token < first || token >= clamp_to(a.off[a.N], first, a.T)) return;  // of no sequence
-  float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + n)]);
-  const float base = top == -INFINITY ? 0.f : top;
-  constexpr int N = D / 64;
-  float sum[N] = {}, total = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = s * all + n;
-    const float f = fast_exp2(a.part_ml[2 * at] - base);
-    total = __fmaf_rn(f, a.part_ml[2 * at + 1], total);
+  // lane i: part i's maximum and total (64 parts at most)
+  float top = -INFINITY, total = 0.f;
+  if (lane < a.splits) top = a.part_ml[2 * (lane * all + n)], total = a.part_ml[2 * (lane * all + n) + 1];
+  const float best = wave_max(top), f = fast_exp2(top - (best == -INFINITY ? 0.f : best));
+  total *= f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) sum[j] = __fmaf_rn(f, a.part_o[at * D + N * lane + j], sum[j]);
+  for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d, kWave);
+  constexpr int N = D / 64, kAtOnce = 8;
+  float sum[N] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += kAtOnce) {
+    float o[kAtOnce][N];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = (s0 + i < a.splits ? s0 + i : a.splits - 1) * all + n;
+#pragma unroll
+      for (int j = 0; j < N; ++j) o[i][j] = a.part_o[at * D + N * lane + j];
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float fi = __shfl(f, s0 + i, kWave);
+      if (s0 + i < a.splits)
+#pragma unroll
+        for (int j = 0; j < N; ++j) sum[j] = __fmaf_rn(fi, o[i][j], sum[j]);
+    }
   }
   const float inv = total == 0.f ? 0.f : __frcp_rn(total);
   uint8_t* p = a.out + token * a.o_ts + head * a.o_hs + N * lane * E::ES;
@@ -542,9 +555,10 @@ constexpr int kWaves = 4, kColumns = 1, kTileRows = 32 * kColumns * kWaves;
 // Slots: a sequence of n rows takes at most (n + kTileRows - 1) / kTileRows tiles.
 int64_t slots_of(int64_t T, int N, int gs) { return (T * gs + kTileRows - 1) / kTileRows + N; }
 
-// Parts of the keys: where the tiles do not fill the card twice, as many as do, of 256 keys in the mean at least.
+// Parts of the keys: where the tiles do not give every CU three workgroups, as many as do (16 new tokens, 8 heads of keys of
+// 128: 58 us against 63 with two a CU), of 256 keys in the mean at least.
 int splits_of(int64_t T, int64_t Tk, int N, int H, int G) {
-  const int64_t tiles = slots_of(T, N, H / G) * G, want = 2 * device_cus();
+  const int64_t tiles = slots_of(T, N, H / G) * G, want = 3 * device_cus();
   int64_t s = want / tiles;
   const int64_t most = Tk / N / 256;
   if (s > most) s = most;
@@ -559,7 +573,7 @@ size_t workspace_of(int64_t T, int64_t Tk, int N, int H, int G, int D) {
 
 template <class E, int D>
 void launch(hipStream_t stream, const Args& a) {
-  constexpr int kPerSimd = E::ES == 2 && D == 64 ? 3 : 2;
+  constexpr int kPerSimd = D == 64 ? 3 : 2;
   hipLaunchKernelGGL((attend_kernel<E, D, kColumns, kWaves, kPerSimd>), dim3(static_cast<unsigned>(a.slots) * a.G * a.splits),
                      dim3(64 * kWaves), 0, stream, a);
   if (a.splits > 1)
