@@ -246,7 +246,7 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   // A step has four blocks of kTiles products. When its last block is in registers everywhere and the next step's copies
   // have landed (the one barrier of a step, before the last block's products), the stage is free: the step kStages on is
   // copied into it, kFirst copies among the last block's products and the others among the next step's first.
-  constexpr int kFirst = kCopies / 2;
+  constexpr int kFirst = 3 * kCopies / 4;
   auto chunk = [&]() {
     if (cs % St::kChunk == 0) copy.scales(cs, __builtin_amdgcn_readfirstlane(lds0 + cbuf));
   };
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
 // Whether K ends inside two stages, or the scale rows are not 16-byte aligned.
 bool is_ragged(const Args& a) {
   auto odd = [](const uint8_t* p, int64_t rs) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(rs)) & 15; };
-  return a.K % (2 * kCols) || odd(a.sx, a.sx_rs) || odd(a.sw, a.sw_rs);
+  return a.K % 512 || odd(a.sx, a.sx_rs) || odd(a.sw, a.sw_rs);
 }
 
 template <typename T, class TL>
@@ -473,22 +473,28 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
                      dim3(64 * (chunks < kMaxWaves ? chunks : kMaxWaves)), 0, stream, a);
 }
 
-// Which kernel: few rows up to 16 (up to 32 of a narrow product); then tiles by how many the product has for the card's
-// CUs.
+// Which kernel, as measured (us, of which a call's host part is 7.7; K = 1536 unless said). In order:
+//   few rows  up to 16 rows, and up to 32 of a narrow product (24 x 1536, K = 6144: 9.5 against 11.0 Small);
+//   Small     up to 3/4 Medium tiles a CU (1422 x 1536, K = 6144: 18.8 against 21.3; but 2584 x 1536, K = 6144: 30.9 against
+//             23.1), with four stages where a CU has one such tile and more than four steps (400 x 1536, K = 6144: 11.6
+//             against 14.6);
+//   Huge      K of 4096 and more, and 3/4 tiles a CU at least: its products take half as many LDS reads (8249 x 1536,
+//             K = 6144: 51.1 against 56.6; 8192^3: 266 against 316), but one workgroup has the CU and nothing runs beside its
+//             epilogue (8249 x 12288: 128 against 119);
+//   Medium    the rest, two workgroups a CU (against 128 x 256 tiles 2584 x 12288: 42.1 and 47.2, 5168 x 7680: 49.7 and 49.1,
+//             8249 x 12288: 119 and 125; 128 x 64: 48.6, 58.7, 144).
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
   using Small = Tile<64, 64, 2, 2, 3>;
-  using Half = Tile<128, 64, 2, 2, 2, 3>;
   using Medium = Tile<128, 128, 2, 2, 2>;
-  using Large = Tile<128, 256, 2, 2, 1>;
-  const int64_t cus = device_cus(), small = tiles_of<Small>(a), half = tiles_of<Half>(a), medium = tiles_of<Medium>(a);
+  using Huge = Tile<256, 256, 2, 2, 1>;
+  const int64_t cus = device_cus(), small = tiles_of<Small>(a);
   if (a.M <= 16) return launch_few_rows<T, 1>(stream, a);
   if (a.M <= 32 && small <= cus / 4) return launch_few_rows<T, 2>(stream, a);
   if (small <= cus && a.K > 4 * kCols) return launch_tiled<T, Tile<64, 64, 2, 2, 1, 4>>(stream, a);
-  if (small <= cus) return launch_tiled<T, Small>(stream, a);
-  if (half <= cus) return launch_tiled<T, Half>(stream, a);
-  if (medium <= 2 * cus) return launch_tiled<T, Medium>(stream, a);
-  launch_tiled<T, Large>(stream, a);
+  if (tiles_of<Medium>(a) <= cus * 3 / 4) return launch_tiled<T, Small>(stream, a);
+  if (a.K >= 4096 && tiles_of<Huge>(a) >= cus * 3 / 4) return launch_tiled<T, Huge>(stream, a);
+  launch_tiled<T, Medium>(stream, a);
 }
 
 }  // namespace mx4

@@ -7,7 +7,7 @@ neighbour where that magnitude lies within 2^-16 M of the border, and each value
 the nearest of the codes has.
 
 Products. Codes are multiples of 1/2 up to 6, and with scales of 1/2, 1 and 2 for each operand a product is a multiple of
-2^-4 up to 144, so sums of K <= 2^11 terms (and a bias of multiples of 1/4) are below 2^23 of these: every order adds them
+2^-4 up to 144, so sums of K <= 4128 terms (and a bias of multiples of 1/4) are below 2^24 of these: every order adds them
 exactly in fp32 and the result is the correctly rounded one, compared for equality, which an element read or written in the
 wrong place cannot pass.
 """
@@ -212,7 +212,8 @@ def check_exact(x, xs, w, ws, bias, dtype, out):
 # rows, columns, features: few rows; one tile; tiles of each size, whole and partly empty; K inside a stage, over its end
 SHAPES = [(1, 32, 1), (7, 1536, 7680), (16, 96, 17), (17, 64, 15), (31, 1056, 513), (33, 256, 64), (64, 512, 64),
           (65, 288, 65), (100, 2048, 129), (129, 1536, 257), (257, 1024, 1001), (700, 1536, 1536), (700, 1056, 1537),
-          (1422, 1536, 1536), (1300, 512, 4096), (2584, 800, 1536), (2049, 1536, 7680), (1025, 1504, 12288)]
+          (1422, 1536, 1536), (1300, 512, 4096), (2584, 800, 1536), (2049, 1536, 7680), (1025, 1504, 12288), (3900, 4096, 3300), (3841, 4128, 3329),
+          (24, 4096, 1000), (300, 2048, 1000)]
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
