@@ -11,6 +11,7 @@ import torch
 
 from hummingbird_amd import _lib
 from hummingbird_amd.dense_attention import _require_gpu, dtype_code
+from hummingbird_amd.elementwise import _new
 
 SUPPORTED_HEAD_DIMS = (64, 128)
 
@@ -23,9 +24,9 @@ def _heads(t: torch.Tensor, name: str) -> None:
 
 def _table(t: torch.Tensor, name: str, entries: int, device: torch.device) -> torch.Tensor:
     """A table of int32 entries on `device`."""
-    if t.device != device or t.dtype != torch.int32:
+    if t.dtype is not torch.int32 or t.device != device:
         raise TypeError(f"{name} must be int32 on {device}, got {t.dtype} on {t.device}")
-    if t.dim() != 1 or t.shape[0] != entries or not t.is_contiguous():
+    if t.shape != (entries,) or not t.is_contiguous():
         raise ValueError(f"{name} must have {entries} entries next to each other, got {tuple(t.shape)}")
     return t
 
@@ -47,14 +48,19 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     `out`, if given, is written and returned, its tokens of no sequence (before `offsets[0]`, from `offsets[N]` on) left as
     they are; a new output has zeros there. D 64 or 128; bf16, half or fp32 (fp32 throughout); any strides of tokens and
     heads that are multiples of 16 bytes (of k's and v's tokens up to 2^23 values), every tensor 16-byte aligned."""
-    _require_gpu(q, "q")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _heads(t, name)
-        if t.dtype != q.dtype or t.device != q.device:
-            raise TypeError(f"{name} must be {q.dtype} on {q.device} as q, got {t.dtype} on {t.device}")
-    code, dev = dtype_code(q.dtype), q.device
+    if not q.is_cuda:
+        _require_gpu(q, "q")
+    dtype, dev = q.dtype, q.device
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    if k.dtype is not dtype or v.dtype is not dtype or k.device != dev or v.device != dev:
+        raise TypeError(f"k and v must be {dtype} on {dev} as q, got {k.dtype} on {k.device} and {v.dtype} on {v.device}")
+    code = dtype_code(dtype)
     tokens, heads, dim = q.shape
     keys, kv_heads, _ = k.shape
+    (qt, qh, q1), (kt, kh, k1), (vt, vh, v1) = q.stride(), k.stride(), v.stride()
+    if q1 != 1 or k1 != 1 or v1 != 1:
+        _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
     if dim not in SUPPORTED_HEAD_DIMS:
         raise ValueError(f"packed_attention needs head_dim in {SUPPORTED_HEAD_DIMS} (head_dim={dim})")
     if k.shape != v.shape or k.shape[2] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -69,7 +75,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         _table(key_lengths, "key_lengths", count, dev)
     fresh = out is None
     if fresh:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = _new((tokens, heads, dim), dtype, dev)
     else:
         _heads(out, "out")
         if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
@@ -80,9 +86,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     lib = _lib.load()
     need = int(lib.hb_packed_workspace_size(code, tokens, keys, count, heads, kv_heads, dim))
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib.launch(lib.hb_packed_attention, "packed_attention", dev, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(),
-                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), code, offsets.data_ptr(),
-                key_offsets.data_ptr(), 0 if key_lengths is None else key_lengths.data_ptr(), int(bool(causal)),
-                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), out.stride(0), out.stride(1), int(fresh),
-                tokens, keys, count, heads, kv_heads, dim, workspace.data_ptr() if need else 0, need)
+    ot, oh, _ = out.stride()
+    _lib.launch(lib.hb_packed_attention, "packed_attention", dev, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(),
+                vt, vh, code, offsets.data_ptr(), key_offsets.data_ptr(),
+                0 if key_lengths is None else key_lengths.data_ptr(), int(bool(causal)),
+                float(dim ** -0.5 if scale is None else scale), out.data_ptr(), ot, oh, int(fresh), tokens, keys, count,
+                heads, kv_heads, dim, workspace.data_ptr() if need else 0, need)
     return out

@@ -303,20 +303,20 @@ def linear_mx4(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     fp32, one rounding to `dtype` (bf16, half or fp32). A scale byte of 255 makes the outputs that its group enters NaN. K a
     multiple of 32; up to 2^21 rows and 2^21 features."""
     n, xs, half = _layout(x, "x")
-    dev, k = x.device, 2 * half
-    if any(t.dtype != torch.uint8 for t in (x, x_scale, weight, weight_scale)):
+    dev, u8, shape = x.device, torch.uint8, weight.shape
+    if not (x.dtype is u8 and x_scale.dtype is u8 and weight.dtype is u8 and weight_scale.dtype is u8):
         raise TypeError(f"linear_mx4 takes uint8 codes and scales, got {x.dtype}, {x_scale.dtype}, {weight.dtype} and "
                         f"{weight_scale.dtype}")
-    if weight.dim() != 2 or weight.shape[1] != half or k % Q4_GROUP:
+    if len(shape) != 2 or shape[1] != half or half % (Q4_GROUP // 2):
         raise ValueError(f"x must be (..., K / 2) and weight (F, K / 2), K a multiple of {Q4_GROUP}, got "
-                         f"{tuple(x.shape)} and {tuple(weight.shape)}")
-    code, groups = dtype_code(dtype), k // Q4_GROUP
+                         f"{tuple(x.shape)} and {tuple(shape)}")
+    code, f, groups, lead = dtype_code(dtype), shape[0], half // (Q4_GROUP // 2), x.shape[:-1]
     if weight.device != dev or x_scale.device != dev or weight_scale.device != dev:
         raise ValueError(f"weight and the scales must be on {dev}, got {weight.device}, {x_scale.device}, "
                          f"{weight_scale.device}")
-    f, ws, _ = _layout(weight, "weight")
-    if x_scale.shape != (*x.shape[:-1], groups):
-        raise ValueError(f"x_scale must be {(*x.shape[:-1], groups)}, got {tuple(x_scale.shape)}")
+    ws = half if weight.is_contiguous() else _layout(weight, "weight")[1]
+    if x_scale.shape != (*lead, groups):
+        raise ValueError(f"x_scale must be {(*lead, groups)}, got {tuple(x_scale.shape)}")
     if weight_scale.shape != (f, groups):
         raise ValueError(f"weight_scale must be ({f}, {groups}), got {tuple(weight_scale.shape)}")
     xss = groups if x_scale.is_contiguous() else _layout(x_scale, "x_scale")[1]
@@ -325,7 +325,7 @@ def linear_mx4(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wei
     if bias is not None:
         bias = _f32_channels(bias, f, dev, "bias")
         bp = bias.data_ptr()
-    out = _new((*x.shape[:-1], f), dtype, dev)
+    out = _new((*lead, f), dtype, dev)
     _lib.launch(_lib.load().hb_proj_mx4, "linear_mx4", dev, x.data_ptr(), xs, x_scale.data_ptr(), xss,
-                weight.data_ptr(), ws, weight_scale.data_ptr(), wss, bp, out.data_ptr(), code, f, n, k, f)
+                weight.data_ptr(), ws, weight_scale.data_ptr(), wss, bp, out.data_ptr(), code, f, n, 2 * half, f)
     return out
