@@ -631,6 +631,8 @@ int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_strid
              {"k", k, k_token_stride, k_head_stride, Tk, G, 0},       {"v", v, v_token_stride, v_head_stride, Tk, G, 0}};
   for (Operand& o : ops) {
     if (!o.tokens) continue;
+    if (o.tokens == 1) o.ts = 0;  // never stepped by, whatever the caller's tensor has there
+    if (o.heads == 1) o.hs = 0;
     if (reinterpret_cast<uintptr_t>(o.p) % 16 || o.ts % vec || o.hs % vec || o.ts < 0 || o.hs < 0)
       return fail(HB_ERR_STRIDE, "%s: %s must be 16-byte aligned with strides that are multiples of %d, not negative", what,
                   o.name, vec);
@@ -642,12 +644,12 @@ int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_strid
     o.bytes = ((o.tokens - 1) * o.ts + (o.heads - 1) * o.hs + D) * es;
   }
   // the output's rows share no element: heads within tokens or tokens within heads
-  const bool inside = H == 1 || out_head_stride >= D, outside = T == 1 || out_token_stride >= D;
+  const Operand &oo = ops[0], &oq = ops[1], &ok = ops[2], &ov = ops[3];
+  const bool inside = H == 1 || oo.hs >= D, outside = T == 1 || oo.ts >= D;
   if (!inside || !outside ||
-      !(T == 1 || H == 1 || out_token_stride >= (H - 1) * out_head_stride + D ||
-        out_head_stride >= (T - 1) * out_token_stride + D))
+      !(T == 1 || H == 1 || oo.ts >= (H - 1) * oo.hs + D || oo.hs >= (T - 1) * oo.ts + D))
     return fail(HB_ERR_STRIDE, "%s: the rows of out overlap", what);
-  const int64_t ob = ops[0].bytes, table = (static_cast<int64_t>(N) + 1) * 4;
+  const int64_t ob = oo.bytes, table = (static_cast<int64_t>(N) + 1) * 4;
   const size_t need = packed::workspace_of(T, Tk, N, H, G, D);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(HB_ERR_WORKSPACE, "%s needs %zu bytes of workspace, 16-byte aligned", what, need);
@@ -669,10 +671,10 @@ int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_strid
         (st = check_disjoint(what, "workspace", workspace, wb, o.name, o.p, o.bytes)))
       return st;
   packed::Args a = {};
-  a.q = static_cast<const uint8_t*>(q), a.q_ts = q_token_stride * es, a.q_hs = q_head_stride * es;
-  a.k = static_cast<const uint8_t*>(k), a.k_ts = k_token_stride * es, a.k_hs = k_head_stride * es;
-  a.v = static_cast<const uint8_t*>(v), a.v_ts = v_token_stride * es, a.v_hs = v_head_stride * es;
-  a.out = static_cast<uint8_t*>(out), a.o_ts = out_token_stride * es, a.o_hs = out_head_stride * es;
+  a.q = static_cast<const uint8_t*>(q), a.q_ts = oq.ts * es, a.q_hs = oq.hs * es;
+  a.k = static_cast<const uint8_t*>(k), a.k_ts = ok.ts * es, a.k_hs = ok.hs * es;
+  a.v = static_cast<const uint8_t*>(v), a.v_ts = ov.ts * es, a.v_hs = ov.hs * es;
+  a.out = static_cast<uint8_t*>(out), a.o_ts = oo.ts * es, a.o_hs = oo.hs * es;
   a.off = offsets, a.koff = key_offsets, a.klen = key_lengths;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0, a.c = scale * kLog2e;
   a.T = static_cast<int>(T), a.Tk = static_cast<int>(Tk), a.N = N, a.H = H, a.G = G, a.gs = H / G;

@@ -402,7 +402,8 @@ int hb_proj_mx4(hipStream_t stream, const void* x, int64_t x_row_stride, const v
  *                          captured call follows their contents. Entries outside [0, T] ([0, Tk]) are taken as the nearest
  *                          one inside; where they do not ascend, which values are written is not specified.
  *   q, out (T, H, D), k, v (Tk, G, D) of `dtype`: strides in elements of tokens and heads, multiples of 8 (bf16, half) or 4
- *                          (fp32), 16-byte aligned; k's and v's token strides up to 2^23.
+ *                          (fp32), 16-byte aligned; k's and v's token strides up to 2^23; that of an axis of one is
+ *                          not looked at.
  *   dtype HB_BF16, HB_F16 (matrix products on operands of that type, probabilities rounded to it) or HB_F32 (fp32
  *   throughout); statistics and sums fp32. D 64 or 128; scale > 0; T (H / G) up to 2^30, Tk up to 2^30, N up to 2^20.
  *   workspace : >= hb_packed_workspace_size(...) bytes, 16-byte aligned; 0 (and NULL allowed) where the rows fill the card

@@ -65,6 +65,15 @@ def test_workspace(lib):
     assert attend(lib, **few, ws=addr(5) - 64, wb=need) == STRIDE
 
 
+def test_strides_of_one_token_and_one_head_are_not_looked_at(lib):
+    """They step to nothing: each of these calls gets as far as the missing workspace."""
+    one = dict(T=1, N=1, Tk=9000, H=4, G=2)
+    assert attend(lib, **one, qt=3, ot=-5) == WORKSPACE
+    assert attend(lib, **one, qt=1 << 61, ot=0) == WORKSPACE
+    assert attend(lib, T=2, N=1, Tk=9000, H=1, G=1, qh=7, kh=-1, vh=1 << 62, oh=0) == WORKSPACE
+    assert attend(lib, T=1, N=1, Tk=1, H=1, G=1, kt=5, vt=1 << 40, q=addr(0) + 2) == STRIDE
+
+
 def test_wrapper_refuses_cpu_tensors():
     q = torch.zeros(3, 2, 64)
     with pytest.raises(ValueError, match="ROCm device"):

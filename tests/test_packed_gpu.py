@@ -205,6 +205,16 @@ def test_layouts(name):
     assert torch.equal(pa.packed_attention(q, k, v, offsets(lengths), out=by_head), want)
 
 
+def test_strides_of_axes_of_one():
+    announce("packed axes of one")
+    q, k, v = make("bf16", 1, 70, 4, 1, 64, 18)
+    at, koff = offsets([1]), offsets([70])
+    want = pa.packed_attention(q, k, v, at, koff)
+    odd = [q.as_strided(q.shape, (3, 64, 1)), k.as_strided(k.shape, (64, 5, 1)), v.as_strided(v.shape, (64, 1, 1))]
+    out = torch.empty_like(q).as_strided(q.shape, (7, 64, 1))
+    assert torch.equal(pa.packed_attention(*odd, at, koff, out=out), want)
+
+
 def test_tokens_of_no_sequence():
     announce("packed rest")
     for H, G, D, split in ((4, 2, 64, False), (8, 2, 128, True)):
