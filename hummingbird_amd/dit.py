@@ -14,6 +14,7 @@ block norms run in fp32 and cast back, the timestep features are fp32 (sa3jax/di
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -23,6 +24,7 @@ from hummingbird_amd import dense_attention, projection, xla_chain
 from hummingbird_amd import elementwise as ew
 from hummingbird_amd.config import DiTConfig
 from hummingbird_amd.dtypes import Dtype
+from hummingbird_amd.packed_attention import packed_attention
 
 
 def use_hip(cfg: DiTConfig, qkv: torch.Tensor) -> bool:
@@ -34,6 +36,44 @@ def use_hip(cfg: DiTConfig, qkv: torch.Tensor) -> bool:
     if not qkv.is_cuda:
         raise ValueError('attention="hip" needs ROCm device tensors; use attention="xla" on the CPU')
     return True
+
+
+def use_packed(cfg: DiTConfig, x: torch.Tensor) -> bool:
+    """Whether the model's plain attention runs on `packed_attention`: `attention="hip"` and not differential
+    (sa3jax/dit.py:131-176 without the second branch)."""
+    if cfg.attention != "hip" or cfg.differential:
+        return False
+    if not x.is_cuda:
+        raise ValueError('attention="hip" needs ROCm device tensors; use attention="xla" on the CPU')
+    return True
+
+
+class PackedContext(NamedTuple):
+    """A clip's context for the plain cross-attention: normalised keys and the values, `(B * Nk, H, D)` each, and where
+    each batch entry's start, `(B + 1,)`."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    offsets: torch.Tensor
+
+
+def _even_offsets(batch: int, length: int, device: torch.device) -> torch.Tensor:
+    """Where `batch` sequences of `length` tokens start, and the last one ends."""
+    return torch.arange(0, batch * length + 1, max(length, 1), dtype=torch.int32, device=device)[:batch + 1]
+
+
+def _plain_self_attention(qkv: torch.Tensor, attn: dict, static: dict, cfg: DiTConfig) -> torch.Tensor:
+    """The self-attention of the model without the second branch, `qkv` `(B, L, 3 H D)` = [q | k | v]: RMSNorm and RoPE
+    of q and k (sa3jax/dit.py:45-98) in torch, the value mask, then `packed_attention` with a sequence per batch
+    entry."""
+    batch, length, _ = qkv.shape
+    q, k, v = (t.unflatten(-1, (cfg.num_heads, cfg.head_dim)) for t in qkv.chunk(3, dim=-1))
+    cos, sin = (t[:, None, :] for t in (static["cos"], static["sin"]))
+    q, k = (xla_chain.rope(xla_chain.rms(t, attn[n]["weight"], cfg.qk_norm_eps), cos, sin, qkv.dtype)
+            for t, n in ((q, "q_norm"), (k, "k_norm")))
+    v = v * static["valid"].to(qkv.dtype)[:, :, None, None]
+    out = packed_attention(*(t.flatten(0, 1) for t in (q, k, v)), static["offsets"], causal=False)
+    return out.reshape(batch, length, -1)
 
 
 def static_tables(inv_freq: torch.Tensor, valid: torch.Tensor, cfg: DiTConfig,
@@ -48,7 +88,10 @@ def static_tables(inv_freq: torch.Tensor, valid: torch.Tensor, cfg: DiTConfig,
     full = torch.cat([ones, valid.to(torch.bool)], dim=-1)
     length = full.shape[1]
     static = {"inv_freq": inv_freq, "valid": full}
-    if cfg.attention == "hip":
+    if cfg.attention == "hip" and not cfg.differential:
+        static["cos"], static["sin"] = xla_chain.rope_tables(length, inv_freq)
+        static["offsets"] = _even_offsets(batch, length, full.device)
+    elif cfg.attention == "hip":
         static["hip_cos"], static["hip_sin"], static["hip_mask"] = dense_attention.tables(
             length, inv_freq, full, cfg.head_dim, compute)
     return static
@@ -90,6 +133,10 @@ def self_attention(h: torch.Tensor, block: dict, static: dict, cfg: DiTConfig,
                                               static["hip_cos"], static["hip_sin"], static["hip_mask"],
                                               cfg.num_heads, cfg.head_dim, cfg.rope_dim // 2, cfg.qk_norm_eps,
                                               lam=lam, workspace=static.get("hip_workspace"))
+    elif use_packed(cfg, qkv):
+        if lam is not None:
+            raise ValueError("lam weights the second branch, which the plain model has not")
+        out = _plain_self_attention(qkv, attn, static, cfg)
     else:
         if not cfg.differential:
             raise NotImplementedError("only the differential self-attention is on this package's path")
@@ -101,28 +148,46 @@ def self_attention(h: torch.Tensor, block: dict, static: dict, cfg: DiTConfig,
 def cross_context(block: dict, ctx: torch.Tensor, cfg: DiTConfig):
     """The context's K/V for one block, computed once per clip (reference: dit._cross_kv, dit.py:274-284):
     `to_kv` -> split -> k_norm on k and k_diff. With `attention="hip"` the result is a prepared
-    `cross_attention.CrossKV` on the device, otherwise the `(k, k_diff, v)` tensors of the XLA chain.
+    `cross_attention.CrossKV` on the device (of the plain model a `PackedContext`), otherwise the `(k, k_diff, v)`
+    tensors of the XLA chain.
     `block["cross_attn"]` holds `to_kv.weight (3E, C)`, `to_q.weight (2E, E)`, `to_out.weight (E, E)`,
     `q_norm.weight`, `k_norm.weight`."""
     attn = block["cross_attn"]
     kv = ctx @ attn["to_kv"]["weight"].t()
     if use_hip(cfg, kv):
         return xattn.prepare_cross_kv(kv, attn["k_norm"]["weight"], cfg.num_heads, cfg.head_dim, cfg.qk_norm_eps)
+    if use_packed(cfg, kv):
+        k, v = (t.unflatten(-1, (cfg.num_heads, cfg.head_dim)).flatten(0, 1) for t in kv.chunk(2, dim=-1))
+        return PackedContext(xla_chain.rms(k, attn["k_norm"]["weight"], cfg.qk_norm_eps), v,
+                             _even_offsets(kv.shape[0], kv.shape[1], kv.device))
     if not cfg.differential:
         raise NotImplementedError("only the differential cross-attention is on this package's path")
     return xla_chain.cross_kv(kv, attn["k_norm"]["weight"], cfg.num_heads, cfg.head_dim, cfg.qk_norm_eps)
 
 
-def cross_attention(h: torch.Tensor, block: dict, context, cfg: DiTConfig,
-                    lam: torch.Tensor | None = None) -> torch.Tensor:
+def cross_attention(h: torch.Tensor, block: dict, context, cfg: DiTConfig, lam: torch.Tensor | None = None,
+                    offsets: torch.Tensor | None = None) -> torch.Tensor:
     """`to_q` -> differential cross-attention -> `to_out` (reference: dit._cross_attention, dit.py:203-215)
-    against `cross_context(...)` of the same block."""
+    against `cross_context(...)` of the same block. `offsets`: of the plain model's queries, where the caller has them
+    (`static["offsets"]`)."""
     attn = block["cross_attn"]
     q = h @ attn["to_q"]["weight"].t()
     if use_hip(cfg, q):
         if not isinstance(context, xattn.CrossKV):
             raise TypeError('attention="hip" needs the context prepared by cross_context with attention="hip"')
         out = xattn.cross_attention(q, context, attn["q_norm"]["weight"], cfg.qk_norm_eps, lam=lam)
+    elif use_packed(cfg, q):
+        if not isinstance(context, PackedContext):
+            raise TypeError('attention="hip" needs the context prepared by cross_context with attention="hip"')
+        if lam is not None:
+            raise ValueError("lam weights the second branch, which the plain model has not")
+        if context.offsets.shape[0] != q.shape[0] + 1:
+            raise ValueError(f"h has batch {q.shape[0]}, the context {context.offsets.shape[0] - 1}")
+        if offsets is None:
+            offsets = _even_offsets(q.shape[0], q.shape[1], q.device)
+        rows = xla_chain.rms(q.unflatten(-1, (cfg.num_heads, cfg.head_dim)), attn["q_norm"]["weight"], cfg.qk_norm_eps)
+        out = packed_attention(rows.flatten(0, 1), context.k, context.v, offsets, context.offsets,
+                               causal=False).reshape(*q.shape[:2], -1)
     else:
         if not cfg.differential:
             raise NotImplementedError("only the differential cross-attention is on this package's path")
@@ -182,14 +247,16 @@ def local_constants(blocks: list, compute: torch.dtype) -> torch.Tensor:
                                b["to_local_embed"]["out"]["bias"]) for b in blocks])
 
 
-_Q8_LAYERS = (("self_attn", "to_qkv"), ("self_attn", "to_out"), ("cross_attn", "to_q"), ("cross_attn", "to_out"),
-              ("ff", "glu_proj"), ("ff", "proj_out"))
+QUANTIZED = ("q8", "mx4")  # forms of the blocks' projections beside the 16-bit one
+_QUANTIZED_LAYERS = (("self_attn", "to_qkv"), ("self_attn", "to_out"), ("cross_attn", "to_q"), ("cross_attn", "to_out"),
+                     ("ff", "glu_proj"), ("ff", "proj_out"))
 
 
-def quantize_params(params: dict, conditioning: str = "q4") -> dict:
+def quantize_params(params: dict, conditioning: str = "q4", weights: str = "q8") -> dict:
     """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
     rows (`elementwise.quantize_rows`, a scale per output feature), under `"q8"` of each layer, and the GLU's bias in
-    fp32 under `"q8_bias"`; with `conditioning="q4"` also the timestep and global conditioning layers as 4-bit weights
+    fp32 under `"q8_bias"`; with `weights="mx4"` what `dit_forward(projections="mx4")` reads, microscaled 4-bit rows
+    (`projection.quantize_q4`) under `"mx4"` and `"mx4_bias"`; with `conditioning="q4"` also the timestep and global conditioning layers as 4-bit weights
     (`projection.quantize_q4`, with the bias in fp32), under `"q4"`. `conditioning="keep"` leaves those layers on the
     weights as they are: they are a few rows of work, but every block reads their result, and their 4 bits make most of
     the error. (Medium width, random weights: the output is 9 %, 19 % and 26 % of its norm off the 16-bit one's at 2, 12
@@ -200,6 +267,9 @@ def quantize_params(params: dict, conditioning: str = "q4") -> dict:
     then takes the result as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
     if conditioning not in ("q4", "keep"):
         raise ValueError(f'conditioning must be "q4" or "keep", got {conditioning!r}')
+    if weights not in QUANTIZED:
+        raise ValueError(f"weights must be one of {QUANTIZED}, got {weights!r}")
+    quantize = ew.quantize_rows if weights == "q8" else projection.quantize_q4
 
     def sequence(seq):
         if conditioning == "keep":
@@ -210,10 +280,10 @@ def quantize_params(params: dict, conditioning: str = "q4") -> dict:
 
     def block(b):
         out = dict(b)
-        for part, layer in _Q8_LAYERS:
-            out[part] = {**out[part], layer: {**b[part][layer], "q8": ew.quantize_rows(b[part][layer]["weight"])}}
+        for part, layer in _QUANTIZED_LAYERS:
+            out[part] = {**out[part], layer: {**b[part][layer], weights: quantize(b[part][layer]["weight"])}}
         # in fp32 as the GLU reads it: converted at each call it takes a launch of 2.6 us per block and step
-        out["ff"]["glu_proj"]["q8_bias"] = b["ff"]["glu_proj"]["bias"].float()
+        out["ff"]["glu_proj"][f"{weights}_bias"] = b["ff"]["glu_proj"]["bias"].float()
         return out
     net = params["transformer"]
     return {**params, "to_timestep_embed": sequence(params["to_timestep_embed"]),
@@ -228,19 +298,26 @@ def _sequential_q4(seq: dict, x: torch.Tensor) -> torch.Tensor:
     return projection.linear_q4(projection.linear_q4(x, *seq["in"]["q4"], silu=True), *seq["out"]["q4"])
 
 
-def _blocks_q8(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tensor, cfg: DiTConfig) -> torch.Tensor:
-    """`_blocks_fused` on 8-bit rows and weights: each norm, GLU and attention output leaves as the 8-bit rows that the
-    next projection multiplies. `adaln` is `(depth, B, 6 E)`."""
+def _blocks_quantized(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tensor, cfg: DiTConfig,
+                      form: str) -> torch.Tensor:
+    """`_blocks_fused` on rows and weights of 8 ("q8") or 4 ("mx4") bits: each norm, GLU and attention output leaves as
+    the rows that the next projection multiplies. `adaln` is `(depth, B, 6 E)`."""
     eps, E, dt = cfg.norm_eps, h.shape[-1], h.dtype
     depth = len(blocks)
+    if form == "q8":
+        rms_modulate, residual_rms, glu = ew.rms_modulate_q8, ew.residual_rms_q8, ew.glu_q8
+        quantize_rows, multiply = ew.quantize_rows, projection.linear_q8
+    else:
+        rms_modulate, residual_rms, glu = ew.rms_modulate_mx4, ew.residual_rms_mx4, ew.glu_mx4
+        quantize_rows, multiply = ew.quantize_rows_mx4, projection.linear_mx4
 
     def chunks(i):
         return adaln[i].reshape(adaln.shape[1], 6, E).unbind(1)  # (B, E) views: scale, shift, gate x 2
 
     def product(rows, layer):
-        return projection.linear_q8(*rows, *layer["q8"], dtype=dt)
+        return multiply(*rows, *layer[form], dtype=dt)
     s_self, sh_self, g_self, s_ff, sh_ff, g_ff = chunks(0)
-    rows = ew.rms_modulate_q8(h, blocks[0]["pre_norm"]["weight"], eps, s_self, sh_self)
+    rows = rms_modulate(h, blocks[0]["pre_norm"]["weight"], eps, s_self, sh_self)
     for i, block in enumerate(blocks):
         s_self, sh_self, g_self, s_ff, sh_ff, g_ff = chunks(i)
         attn, cross, ff = block["self_attn"], block["cross_attn"], block["ff"]
@@ -248,18 +325,18 @@ def _blocks_q8(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tensor,
                                             attn["k_norm"]["weight"], static["hip_cos"], static["hip_sin"],
                                             static["hip_mask"], cfg.num_heads, cfg.head_dim, cfg.rope_dim // 2,
                                             cfg.qk_norm_eps, workspace=static.get("hip_workspace"))
-        h, *rows = ew.residual_rms_q8(h, product(ew.quantize_rows(a), attn["to_out"]),
-                                      block["cross_attend_norm"]["weight"], eps, gate=g_self)
+        h, *rows = residual_rms(h, product(quantize_rows(a), attn["to_out"]), block["cross_attend_norm"]["weight"], eps,
+                                gate=g_self)
         c = xattn.cross_attention(product(rows, cross["to_q"]), static["cross"][i], cross["q_norm"]["weight"],
                                   cfg.qk_norm_eps)
-        h, *rows = ew.residual_rms_q8(h, product(ew.quantize_rows(c), cross["to_out"]), block["ff_norm"]["weight"], eps,
-                                      local=static["local"][i], memory=cfg.num_memory_tokens, scale=s_ff, shift=sh_ff)
-        f = product(ew.glu_q8(product(rows, ff["glu_proj"]), ff["glu_proj"]["q8_bias"]), ff["proj_out"])
+        h, *rows = residual_rms(h, product(quantize_rows(c), cross["to_out"]), block["ff_norm"]["weight"], eps,
+                                local=static["local"][i], memory=cfg.num_memory_tokens, scale=s_ff, shift=sh_ff)
+        f = product(glu(product(rows, ff["glu_proj"]), ff["glu_proj"][f"{form}_bias"]), ff["proj_out"])
         bias = ff["proj_out"]["bias"].to(dt)
         if i + 1 < depth:
             ns, nsh = chunks(i + 1)[:2]
-            h, *rows = ew.residual_rms_q8(h, f, blocks[i + 1]["pre_norm"]["weight"], eps, gate=g_ff, x_bias=bias,
-                                          scale=ns, shift=nsh)
+            h, *rows = residual_rms(h, f, blocks[i + 1]["pre_norm"]["weight"], eps, gate=g_ff, x_bias=bias,
+                                    scale=ns, shift=nsh)
         else:
             h = ew.gated_residual(h, f, gate=g_ff, x_bias=bias)
     return h
@@ -275,7 +352,7 @@ def block_forward(h: torch.Tensor, block: dict, static: dict, gcond: torch.Tenso
     if adaln is None:
         adaln = block["to_scale_shift_gate"].to(compute) + gcond
     scale_self, shift_self, gate_self, scale_ff, shift_ff, gate_ff = adaln[:, None, :].chunk(6, dim=-1)
-    if use_hip(cfg, h):
+    if use_hip(cfg, h) or use_packed(cfg, h):
         return _block_fused(h, block, static, (scale_self, shift_self, gate_self, scale_ff, shift_ff, gate_ff), index,
                             cfg, projections)
     x = xla_chain.rms(h, block["pre_norm"]["weight"], cfg.norm_eps)
@@ -284,7 +361,7 @@ def block_forward(h: torch.Tensor, block: dict, static: dict, gcond: torch.Tenso
     h = h + x * torch.sigmoid(1 - gate_self)
 
     x = xla_chain.rms(h, block["cross_attend_norm"]["weight"], cfg.norm_eps)
-    h = h + cross_attention(x, block, static["cross"][index], cfg)
+    h = h + cross_attention(x, block, static["cross"][index], cfg, offsets=static.get("offsets"))
 
     # the memory tokens receive no local condition (sa3jax/dit.py:239-241)
     memory = cfg.num_memory_tokens
@@ -312,7 +389,7 @@ def _blocks_fused(h: torch.Tensor, blocks: list, static: dict, adaln: torch.Tens
         s_self, sh_self, g_self, s_ff, sh_ff, g_ff = chunks(i)
         a = self_attention(x, block, static, cfg, projections=projections)
         h, x = ew.residual_rms(h, a, block["cross_attend_norm"]["weight"], eps, gate=g_self)
-        c = cross_attention(x, block, static["cross"][i], cfg)
+        c = cross_attention(x, block, static["cross"][i], cfg, offsets=static.get("offsets"))
         h, x = ew.residual_rms(h, c, block["ff_norm"]["weight"], eps, local=static["local"][i],
                                memory=cfg.num_memory_tokens, scale=s_ff, shift=sh_ff)
         ff = block["ff"]
@@ -339,7 +416,7 @@ def _block_fused(h: torch.Tensor, block: dict, static: dict, adaln: tuple, index
     h = ew.gated_residual(h, x, gate=gate_self)
 
     x = ew.rms_modulate(h, block["cross_attend_norm"]["weight"], cfg.norm_eps)
-    x = cross_attention(x, block, static["cross"][index], cfg)
+    x = cross_attention(x, block, static["cross"][index], cfg, offsets=static.get("offsets"))
     h = ew.gated_residual(h, x, local=static["local"][index], memory=cfg.num_memory_tokens)
 
     x = ew.rms_modulate(h, block["ff_norm"]["weight"], cfg.norm_eps, scale_ff, shift_ff)
@@ -398,32 +475,35 @@ def dit_forward(params: dict, x: torch.Tensor, t: torch.Tensor, static: dict, cf
                 projections: str = "torch") -> torch.Tensor:
     """One denoiser evaluation (sa3jax/dit.py:340-361): `(B, io_channels, T)` latents and `(B,)` timesteps -> the
     velocity, same shape, in the compute dtype. `static` comes from `prepare_static`. `projections` is passed to
-    `self_attention`, or "q8": the blocks' projections on 8-bit rows and weights and the conditioning layers on the
-    weights that `quantize_params` gave them, with `params` (of `static` too) from it; `attention="hip"` only."""
+    `self_attention`, or "q8" ("mx4"): the blocks' projections on 8-bit (microscaled 4-bit) rows and weights and the
+    conditioning layers on the weights that `quantize_params` gave them, with `params` (of `static` too) from it;
+    `attention="hip"` and the differential model only."""
     net = params["transformer"]
     compute = dtype.compute
-    q8 = projections == "q8"
-    if q8 and any("q8" not in b["ff"]["proj_out"] for b in net["blocks"]):
-        raise ValueError('projections="q8" needs the params of quantize_params')
+    quantized = projections in QUANTIZED
+    if quantized and any(projections not in b["ff"]["proj_out"] for b in net["blocks"]):
+        raise ValueError(f'projections="{projections}" needs the params of quantize_params(weights="{projections}")')
     h = x.to(compute)
     h = conv1x1(h, params["preprocess_conv"]["weight"]) + h
     h = linear(h.transpose(1, 2), net["project_in"]["weight"])
     memory = net["memory_tokens"].to(compute).expand(h.shape[0], cfg.num_memory_tokens, cfg.embed_dim)
     h = torch.cat([memory, h], dim=1)
 
-    if q8 and not use_hip(cfg, h):
-        raise ValueError('projections="q8" needs attention="hip" and the differential model')
-    embed = _sequential_q4 if q8 else sequential
+    if quantized and not use_hip(cfg, h):
+        raise ValueError(f'projections="{projections}" needs attention="hip" and the differential model')
+    embed = _sequential_q4 if quantized else sequential
     timestep = embed(params["to_timestep_embed"], expo_fourier(t.to(compute), cfg.fourier_dim))
     gcond = embed(net["global_cond_embedder"], static["gcond_proj"] + timestep)
 
     adaln = static["adaln"][:, None, :] + gcond[None] if "adaln" in static else None  # every block's, one launch
     blocks = static.get("blocks", net["blocks"])
-    if q8:
-        if not blocks or adaln is None or "q8" not in blocks[0]["ff"]["proj_out"]:
-            raise ValueError('projections="q8" needs prepare_static to be given the params of quantize_params')
-        h = _blocks_q8(h, blocks, static, adaln, cfg)
-    elif adaln is not None and blocks and use_hip(cfg, h) and ew.residual_rms_supported(h.dtype, cfg.embed_dim):
+    if quantized:
+        if not blocks or adaln is None or projections not in blocks[0]["ff"]["proj_out"]:
+            raise ValueError(f'projections="{projections}" needs prepare_static to be given the params of '
+                             "quantize_params")
+        h = _blocks_quantized(h, blocks, static, adaln, cfg, projections)
+    elif (adaln is not None and blocks and (use_hip(cfg, h) or use_packed(cfg, h))
+          and ew.residual_rms_supported(h.dtype, cfg.embed_dim)):
         h = _blocks_fused(h, blocks, static, adaln, cfg, projections)
     else:
         for index, block in enumerate(blocks):
