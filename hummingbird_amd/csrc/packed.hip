@@ -3,7 +3,8 @@
 //
 //   out[t, h] = sum_b softmax_b(scale q[t, h] . k[b, h / gs]) v[b, h / gs],   gs = H / G,
 //
-// over the keys b of t's sequence, those at or before t's place at the end of them when `causal`. A row with no key is zero.
+// over the keys b of t's sequence, those at or before t's place at the end of them when `causal`. A row with no key, or
+// with nothing but scores of minus infinity, is zero.
 //
 // A workgroup computes a tile of rows of one sequence for one head of keys; a row is one query's one head, the gs heads that
 // share the keys next to each other, so that a tile reads its keys once whatever gs is and one new token fills gs rows.
@@ -60,16 +61,28 @@ struct Tile {
   int k0, lk;      // and keys
 };
 
-// Slot u's tile of R rows. Lane i of a wave looks at sequence 64 n + i.
-__device__ __forceinline__ Tile find_tile(const Args& a, int u, int R) {
+// Slot u's tile of R rows. Lane i of a wave looks at sequence 64 n + i. `sorted`: up to 64 sequences in the order of their
+// lengths, the longest first.
+__device__ __forceinline__ Tile find_tile(const Args& a, int u, int R, bool sorted) {
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int i0 = 0; i0 < a.N; i0 += 64) {
     const int i = i0 + lane;
-    int q0 = 0, lq = 0;
+    int number = i, q0 = 0, lq = 0;
     if (i < a.N) {
       q0 = clamp_to(a.off[i], 0, a.T);
       lq = clamp_to(a.off[i + 1], q0, a.T) - q0;
+    }
+    if (sorted) {
+      int rank = 0;
+      for (int j = 0; j < a.N; ++j) {
+        const int other = __builtin_amdgcn_readlane(lq, j);
+        rank += other > lq || (other == lq && j < lane);
+      }
+      if (lane >= a.N) rank = lane;  // 0 to N - 1 are the sequences'
+      number = __builtin_amdgcn_ds_permute(4 * rank, number);
+      q0 = __builtin_amdgcn_ds_permute(4 * rank, q0);
+      lq = __builtin_amdgcn_ds_permute(4 * rank, lq);
     }
     const int tiles = static_cast<int>((static_cast<int64_t>(lq) * a.gs + R - 1) / R);
     int upto = tiles;
@@ -83,7 +96,7 @@ __device__ __forceinline__ Tile find_tile(const Args& a, int u, int R) {
       const int who = __ffsll(static_cast<unsigned long long>(past)) - 1;
       Tile t;
       t.found = true;
-      const int seq = __builtin_amdgcn_readfirstlane(i0 + who);
+      const int seq = __builtin_amdgcn_readfirstlane(__shfl(number, who, kWave));
       t.q0 = __builtin_amdgcn_readfirstlane(__shfl(q0, who, kWave));
       t.lq = __builtin_amdgcn_readfirstlane(__shfl(lq, who, kWave));
       const int n = __builtin_amdgcn_readfirstlane(__shfl(tiles, who, kWave));
@@ -248,7 +261,7 @@ struct Rows {
   static constexpr bool kWide = std::is_same<E, E16<Bf16Io>>::value;
   static constexpr float kSlack = kWide ? 100.f : 8.f;
   __device__ __forceinline__ void softmax(int ct, f32x16 (&sc)[RT], u32x4 (&p)[RT][2], int k0, float c, bool masked,
-                                          bool look) {
+                                          bool first, bool careful) {
     const int lh = (threadIdx.x & 63) >> 5;
     if (masked) {
 #pragma unroll
@@ -256,7 +269,7 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[rt][r] : -INFINITY;
     }
-    if (look) {
+    if (!kWide || first || careful) {
       float top = -INFINITY;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -264,6 +277,8 @@ struct Rows {
         for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[rt][r]);
       const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
+      // a first tile with nothing but scores of minus infinity has no reference for the later ones: wild()
+      if (kWide && !careful && top == -INFINITY && k0 < lim[ct]) l[ct] = NAN;
       const bool passed = top > m[ct] + kSlack;
       if (__any(passed)) {
         const float alpha = passed ? fast_exp2(m[ct] - top) : 1.f;
@@ -299,7 +314,7 @@ struct Rows {
     u32x4 p[NCT][RT][2];
     scores(sK, sc);
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) softmax(ct, sc[ct], p[ct], k0, c, masked, !kWide || first || careful);
+    for (int ct = 0; ct < NCT; ++ct) softmax(ct, sc[ct], p[ct], k0, c, masked, first, careful);
     if (__builtin_expect(masked && careful, 0)) return add_apart(sV, k0, sc, p);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
@@ -412,9 +427,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
   constexpr int R = 32 * NCT * NW;
   __shared__ __attribute__((aligned(16))) uint8_t smem[2 * L::kStage];
   const int lane = threadIdx.x & 63, lr = lane & 31, lh = lane >> 5, wv = wave_id();
-  // consecutive workgroups: the parts of one tile's keys, then the heads of keys, then the slots
-  const int part = blockIdx.x % a.splits, rest = blockIdx.x / a.splits, g = rest % a.G, u = rest / a.G;
-  const Tile t = find_tile(a, u, R);
+  // consecutive workgroups: the parts of one tile's keys, then the heads of keys, then the slots. fp32 tiles are bound by the
+  // matrix cores, and the CU with the longest ones ends last: where there are two a CU, the longest sequences come first and
+  // every other 256 workgroups (a CU has one of each) go the other way round, so that a long tile meets a short one (24
+  // prompts of up to 256 tokens, 16 heads of 64: 46 -> 41 us; 16-bit tiles gain nothing, and short ones lose a third).
+  int b = blockIdx.x;
+  const bool sorted = E::ES == 4 && a.N <= 64 && gridDim.x >= 512;
+  if (sorted && (b & 256) && (b | 255) < static_cast<int>(gridDim.x)) b ^= 255;
+  const int part = b % a.splits, rest = b / a.splits, g = rest % a.G, u = rest / a.G;
+  const Tile t = find_tile(a, u, R, sorted);
   const int row_bytes = D * E::ES;
   if (!t.found) {
     if (!a.zero_rest || part) return;
@@ -556,26 +577,40 @@ constexpr int kWaves = 4, kColumns = 1, kTileRows = 32 * kColumns * kWaves;
 int64_t slots_of(int64_t T, int N, int gs) { return (T * gs + kTileRows - 1) / kTileRows + N; }
 
 // Parts of the keys: where the tiles do not give every CU three workgroups, as many as do (16 new tokens, 8 heads of keys of
-// 128: 58 us against 63 with two a CU), of 256 keys in the mean at least.
-int splits_of(int64_t T, int64_t Tk, int N, int H, int G) {
-  const int64_t tiles = slots_of(T, N, H / G) * G, want = 3 * device_cus();
-  int64_t s = want / tiles;
-  const int64_t most = Tk / N / 256;
-  if (s > most) s = most;
+// 128: 58 us against 63 with two a CU), of 256 keys in the mean at least; 64 for fp32, whose 32 keys take 1.7 to 3.4 us where
+// 16-bit ones' 64 take 0.5 (7 sequences of new tokens over 2093 keys of 128: 49 -> 20 us; 16-bit parts of 128 keys cost up to
+// twice what they save). fp32 also splits for balance, to six workgroups a CU of 1024 keys (3223 tokens: 424 -> 377 us).
+int splits_of(int dtype, int64_t T, int64_t Tk, int N, int H, int G) {
+  const int64_t tiles = slots_of(T, N, H / G) * G, want = 3 * device_cus(), mean = Tk / N;
+  auto smaller = [](int64_t x, int64_t y) { return x < y ? x : y; };
+  int64_t s = smaller(want / tiles, mean / (dtype == HB_F32 ? 64 : 256));
+  if (dtype == HB_F32) {
+    const int64_t even = smaller(2 * want / tiles, mean / 1024);
+    if (even > s) s = even;
+  }
   if (s > 64) s = 64;
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-size_t workspace_of(int64_t T, int64_t Tk, int N, int H, int G, int D) {
-  const int s = splits_of(T, Tk, N, H, G);
+size_t workspace_of(int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D) {
+  const int s = splits_of(dtype, T, Tk, N, H, G);
   return s == 1 ? 0 : static_cast<size_t>(s) * static_cast<size_t>(T) * H * (D + 2) * 4;
 }
 
 template <class E, int D>
 void launch(hipStream_t stream, const Args& a) {
-  constexpr int kPerSimd = D == 64 ? 3 : 2;
-  hipLaunchKernelGGL((attend_kernel<E, D, kColumns, kWaves, kPerSimd>), dim3(static_cast<unsigned>(a.slots) * a.G * a.splits),
-                     dim3(64 * kWaves), 0, stream, a);
+  const unsigned grid = static_cast<unsigned>(a.slots) * a.G * a.splits;
+  auto attend = [&](auto per_simd) {
+    hipLaunchKernelGGL((attend_kernel<E, D, kColumns, kWaves, decltype(per_simd)::value>), dim3(grid), dim3(64 * kWaves), 0,
+                       stream, a);
+  };
+  // fp32 heads of 128 do without spills with a wave a SIMD (12 prompts of 161 to 312 tokens, 32 heads: 171 -> 147 us), but
+  // tiles of one wave's rows leave the other SIMDs to a second workgroup, where there is one (29 sequences of 1 to 5 new
+  // tokens over 63 keys, 16 heads: 18.6 us, 28 with one).
+  if constexpr (D == 64) attend(std::integral_constant<int, 3>{});
+  else if (E::ES == 2 || (grid > static_cast<unsigned>(device_cus()) && static_cast<int64_t>(a.T) * a.gs <= 32ll * a.N))
+    attend(std::integral_constant<int, 2>{});
+  else if constexpr (E::ES == 4) attend(std::integral_constant<int, 1>{});
   if (a.splits > 1)
     hipLaunchKernelGGL((join_kernel<E, D>), dim3(static_cast<unsigned>((static_cast<int64_t>(a.T) * a.H + 3) / 4)),
                        dim3(256), 0, stream, a);
@@ -603,7 +638,7 @@ extern "C" {
 size_t hb_packed_workspace_size(int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D) {
   clear_error();
   if (packed::check_sizes("packed_workspace_size", dtype, T, Tk, N, H, G, D)) return 0;
-  return packed::workspace_of(T, Tk, N, H, G, D);
+  return packed::workspace_of(dtype, T, Tk, N, H, G, D);
 }
 
 int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
@@ -650,7 +685,7 @@ int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_strid
       !(T == 1 || H == 1 || oo.ts >= (H - 1) * oo.hs + D || oo.hs >= (T - 1) * oo.ts + D))
     return fail(HB_ERR_STRIDE, "%s: the rows of out overlap", what);
   const int64_t ob = oo.bytes, table = (static_cast<int64_t>(N) + 1) * 4;
-  const size_t need = packed::workspace_of(T, Tk, N, H, G, D);
+  const size_t need = packed::workspace_of(dtype, T, Tk, N, H, G, D);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
     return fail(HB_ERR_WORKSPACE, "%s needs %zu bytes of workspace, 16-byte aligned", what, need);
   auto misaligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; };
@@ -678,7 +713,7 @@ int hb_packed_attention(hipStream_t stream, const void* q, int64_t q_token_strid
   a.off = offsets, a.koff = key_offsets, a.klen = key_lengths;
   a.causal = causal != 0, a.zero_rest = zero_rest != 0, a.c = scale * kLog2e;
   a.T = static_cast<int>(T), a.Tk = static_cast<int>(Tk), a.N = N, a.H = H, a.G = G, a.gs = H / G;
-  a.slots = static_cast<int>(packed::slots_of(T, N, H / G)), a.splits = packed::splits_of(T, Tk, N, H, G);
+  a.slots = static_cast<int>(packed::slots_of(T, N, H / G)), a.splits = packed::splits_of(dtype, T, Tk, N, H, G);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o ? a.part_o + static_cast<int64_t>(a.splits) * T * H * D : nullptr;
   auto run = [&](auto e) {

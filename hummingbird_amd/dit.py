@@ -67,12 +67,13 @@ def _plain_self_attention(qkv: torch.Tensor, attn: dict, static: dict, cfg: DiTC
     of q and k (sa3jax/dit.py:45-98) in torch, the value mask, then `packed_attention` with a sequence per batch
     entry."""
     batch, length, _ = qkv.shape
-    q, k, v = (t.unflatten(-1, (cfg.num_heads, cfg.head_dim)) for t in qkv.chunk(3, dim=-1))
-    cos, sin = (t[:, None, :] for t in (static["cos"], static["sin"]))
-    q, k = (xla_chain.rope(xla_chain.rms(t, attn[n]["weight"], cfg.qk_norm_eps), cos, sin, qkv.dtype)
-            for t, n in ((q, "q_norm"), (k, "k_norm")))
-    v = v * static["valid"].to(qkv.dtype)[:, :, None, None]
-    out = packed_attention(*(t.flatten(0, 1) for t in (q, k, v)), static["offsets"], causal=False)
+    rows = qkv.unflatten(-1, (3, cfg.num_heads, cfg.head_dim))
+    weight = torch.stack([attn["q_norm"]["weight"], attn["k_norm"]["weight"]])[:, None]
+    # q and k in the same launches, about fifteen a block
+    qk = xla_chain.rms(rows[:, :, :2], weight, cfg.qk_norm_eps)
+    qk = xla_chain.rope(qk, static["cos"][:, None, None], static["sin"][:, None, None], qkv.dtype).flatten(0, 1)
+    v = rows[:, :, 2] * static["valid"].to(qkv.dtype)[:, :, None, None]
+    out = packed_attention(qk[:, 0], qk[:, 1], v.flatten(0, 1), static["offsets"], causal=False)
     return out.reshape(batch, length, -1)
 
 
@@ -256,15 +257,21 @@ def quantize_params(params: dict, conditioning: str = "q4", weights: str = "q8")
     """`params` with what `dit_forward(projections="q8")` reads beside the weights: the blocks' projections as 8-bit
     rows (`elementwise.quantize_rows`, a scale per output feature), under `"q8"` of each layer, and the GLU's bias in
     fp32 under `"q8_bias"`; with `weights="mx4"` what `dit_forward(projections="mx4")` reads, microscaled 4-bit rows
-    (`projection.quantize_q4`) under `"mx4"` and `"mx4_bias"`; with `conditioning="q4"` also the timestep and global conditioning layers as 4-bit weights
-    (`projection.quantize_q4`, with the bias in fp32), under `"q4"`. `conditioning="keep"` leaves those layers on the
-    weights as they are: they are a few rows of work, but every block reads their result, and their 4 bits make most of
-    the error. (Medium width, random weights: the output is 9 %, 19 % and 26 % of its norm off the 16-bit one's at 2, 12
-    and 24 blocks with "q4", 4 %, 9 % and 12 % with "keep"; a render of 1422 tokens takes 44.7 and 45.0 ms.)
-    The other tensors are shared, not copied. The 16-bit weights stay beside the 8-bit ones (2.4 and 1.2 GB of the medium
-    model), so that the other `projections` still run; where only "q8" does, the `"weight"` entries of the layers that
-    have a `"q8"` may be deleted before `prepare_static`. Done once per model, on the weights' device; `prepare_static`
-    then takes the result as its `params`. The layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
+    (`projection.quantize_q4`), under `"mx4"` and `"mx4_bias"`. With `conditioning="q4"` also the timestep and global
+    conditioning layers as 4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q4"`.
+    `conditioning="keep"` leaves those layers on the weights as they are: they are a few rows of work, but every block
+    reads their result, and their 4 bits make most of the 8-bit form's error. Medium width, random weights, the output's
+    distance from the 16-bit one at 2, 12 and 24 blocks as a part of its norm, and a render of 1422 tokens in 8 steps (62.7
+    ms with 16 bits):
+
+        "q8"   "q4"   9 %, 19 %, 26 %   43.6 ms        "mx4"  "q4"   18 %, 42 %, 56 %  39.7 ms
+               "keep" 4 %,  9 %, 12 %   44.0 ms               "keep" 16 %, 39 %, 52 %  40.1 ms
+
+    The other tensors are shared, not copied. The 16-bit weights stay beside the others (2.4 GB of the medium model, 1.2 the
+    8-bit and 0.6 the 4-bit ones), so that the other `projections` still run; where only one does, the `"weight"` entries of
+    the layers that have its form may be deleted before `prepare_static`. `params` may have the other form already: both
+    are kept. Done once per model, on the weights' device; `prepare_static` then takes the result as its `params`. The
+    layers' input widths must be multiples of 16 (8-bit) and 32 (4-bit)."""
     if conditioning not in ("q4", "keep"):
         raise ValueError(f'conditioning must be "q4" or "keep", got {conditioning!r}')
     if weights not in QUANTIZED:

@@ -42,7 +42,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     have room behind them. `offsets` and `key_offsets` are `(N + 1,)` ascending, `key_lengths` `(N,)`, int32 on the device;
     they are read there, so nothing waits for them and a captured call follows their contents. With `causal` query a of
     lq sees the keys b <= a + lk - lq of lk: the queries are the last of the keys' tokens (one new token: lq = 1).
-    A query that sees no key gives zeros; keys that a query does not see take no part in it, whatever their values.
+    A query that sees no key, or only keys of a score of minus infinity, gives zeros; keys that a query does not see take no
+    part in it, whatever their values.
     `scale` (default `D ** -0.5`) is positive.
 
     `out`, if given, is written and returned, its tokens of no sequence (before `offsets[0]`, from `offsets[N]` on) left as

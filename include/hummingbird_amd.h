@@ -395,9 +395,9 @@ int hb_proj_mx4(hipStream_t stream, const void* x, int64_t x_row_stride, const v
  * head h / (H / G).
  *   out[t, h] = sum_b softmax_b(scale q[t, h] . k[b]) v[b]
  * over the keys of t's sequence; with `causal` != 0 over those up to t's place when the queries are the last of them:
- * query a of lq sees keys b <= a + lk - lq. A row that sees no key is zero. A key that a row does not see takes no part in
- * it, whatever its values are. Tokens of no sequence (before offsets[0], from offsets[N] on) are left as they were in out,
- * or zeroed with `zero_rest` != 0.
+ * query a of lq sees keys b <= a + lk - lq. A row that sees no key, or only keys of a score of
+ * minus infinity, is zero. A key that a row does not see takes no part in it, whatever its values are. Tokens of no
+ * sequence (before offsets[0], from offsets[N] on) are left as they were in out, or zeroed with `zero_rest` != 0.
  *   offsets, key_offsets : N + 1 ascending ints on the device; key_lengths: N ints or NULL. They are read by the kernel, so a
  *                          captured call follows their contents. Entries outside [0, T] ([0, Tk]) are taken as the nearest
  *                          one inside; where they do not ascend, which values are written is not specified.

@@ -154,6 +154,39 @@ def test_scores_far_above_the_first_ones(name):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+def test_scores_of_minus_infinity(name):
+    """Keys whose scores are minus infinity weigh nothing, a first tile of them too, whatever the later scores are; a row of
+    nothing else is zero."""
+    announce("packed scores of minus infinity", name)
+    D, n = 64, 200
+    q, k, v = make(name, n, n, 2, 1, D, 19)
+    q[..., :2] = 1.0
+    for shift in (-300.0, 0.0, 300.0):
+        kk = (k * 0.1).contiguous()
+        kk[..., 1] = shift
+        kk[:130, :, 0] = float("-inf")
+        got = pa.packed_attention(q, kk, v, offsets([n]), causal=False, scale=1.0)
+        check(got, q, kk[130:], v[130:], [n], [n - 130], [0], False, 1.0, name, shift)
+        got = pa.packed_attention(q, kk, v, offsets([n]), causal=True, scale=1.0)
+        assert (got[:130] == 0).all()
+        check(got[130:], q[130:], kk[130:], v[130:], [n - 130], [n - 130], [0], True, 1.0, name, (shift, "causal"))
+
+
+@pytest.mark.parametrize("name", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_tiles_enough_for_two_a_cu(name, D):
+    """Sequences of very different lengths, enough tiles that fp32 ones are taken in another order; some empty, some equal."""
+    announce("packed many tiles", name, D)
+    for lengths in ([5, 0, 300, 131, 131, 0, 1, 250, 40, 129, 64, 128] * 2, [3] * 30 + [200] * 34, [70] * 65):
+        H = 24
+        q, k, v = make(name, sum(lengths), sum(lengths), H, H, D, 21)
+        starts = [sum(lengths[:j]) for j in range(len(lengths))]
+        for causal in (False, True):
+            got = pa.packed_attention(q, k, v, offsets(lengths), causal=causal)
+            check(got, q, k, v, lengths, lengths, starts, causal, D ** -0.5, name, (lengths[:3], causal))
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
 @pytest.mark.parametrize("D", [64, 128])
 def test_values_of_keys_that_are_not_seen(name, D):
     """NaN and infinities in keys and values that a row does not see (later ones of its own sequence, the next sequence's,
