@@ -71,7 +71,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         raise ValueError(f"offsets must be (N + 1,), got {tuple(offsets.shape)}")
     count = offsets.shape[0] - 1
     _table(offsets, "offsets", count + 1, dev)
-    key_offsets = offsets if key_offsets is None else _table(key_offsets, "key_offsets", count + 1, dev)
+    if key_offsets is None:
+        if keys < tokens:
+            raise ValueError(f"k and v have {keys} tokens, q {tokens}: without key_offsets they share q's sequences")
+        key_offsets = offsets
+    else:
+        _table(key_offsets, "key_offsets", count + 1, dev)
     if key_lengths is not None:
         _table(key_lengths, "key_lengths", count, dev)
     fresh = out is None

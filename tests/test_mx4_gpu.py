@@ -328,3 +328,92 @@ def test_captured_and_on_another_stream():
             assert torch.equal(layer(x), ref)
             torch.cuda.synchronize()
             assert torch.equal(out, ref)
+
+
+def test_rows_past_32_bits():
+    """Rows of an input, codes and an output whose places pass 2^32 bytes, the last of them checked."""
+    announce("mx4 past 32 bits")
+    gen = generator(12)
+    C, N = 8192, 270000
+    x = torch.empty(N, C, dtype=torch.bfloat16, device=DEV)
+    last = rand(gen, 50, C, dtype=torch.bfloat16)
+    x[-50:] = last
+    x[:50] = last
+    q, s = ew.quantize_rows_mx4(x)
+    wq, ws = ew.quantize_rows_mx4(last)
+    for part in (slice(0, 50), slice(N - 50, N)):
+        assert torch.equal(q[part], wq) and torch.equal(s[part], ws)
+    weight, bias = rand(gen, C, std=0.1, mean=1.0), rand(gen, C, std=0.1)
+    q, s = ew.rms_modulate_mx4(x[None], weight, 1e-5)
+    wq, ws = ew.rms_modulate_mx4(last[None], weight, 1e-5)
+    assert torch.equal(q[0, -50:], wq[0]) and torch.equal(s[0, -50:], ws[0])
+    h, q, s = ew.residual_rms_mx4(x[None], x[None], weight, 1e-5)
+    wh, wq, ws = ew.residual_rms_mx4(last[None], last[None], weight, 1e-5)
+    assert torch.equal(h[0, -50:], wh[0]) and torch.equal(q[0, -50:], wq[0]) and torch.equal(s[0, -50:], ws[0])
+    del h
+    q, s = ew.glu_mx4(x, bias)
+    wq, ws = ew.glu_mx4(last, bias)
+    assert torch.equal(q[-50:], wq) and torch.equal(s[-50:], ws)
+    del x
+    M, F, K = 140001, 16000, 64
+    x, xs = codes(gen, M, K)
+    w, ws = codes(gen, F, K)
+    out = pr.linear_mx4(x, xs, w, ws)
+    for part in (slice(0, 300), slice(M - 300, M)):
+        check_exact(x[part], xs[part], w, ws, None, torch.bfloat16, out[part])
+    del out
+    for rows in (7, 40, 300):  # rows 4 MB apart
+        far, fars = codes(gen, rows, K)
+        buf = torch.empty(rows * (1 << 22) + 64, dtype=torch.uint8, device=DEV)
+        y = buf.as_strided((rows, K // 2), (1 << 22, 1))
+        y.copy_(far)
+        check_exact(far, fars, w, ws, None, torch.bfloat16, pr.linear_mx4(y, fars, w, ws))
+        check_exact(w, ws, far, fars, None, torch.bfloat16, pr.linear_mx4(w, ws, y, fars))
+        fs = buf.as_strided((rows, K // 32), (1 << 22, 1), 33)
+        fs.copy_(fars)
+        check_exact(far, fars, w, ws, None, torch.bfloat16, pr.linear_mx4(far, fs, w, ws))
+        check_exact(w, ws, far, fars, None, torch.bfloat16, pr.linear_mx4(w, ws, far, fs))
+
+
+def test_wrapper_refusals():
+    announce("mx4 refusals")
+    gen = generator(13)
+    x, w = rand(gen, 2, 5, 64, dtype=torch.bfloat16), rand(gen, 64)
+    mod = rand(gen, 2, 64, dtype=torch.bfloat16)
+    refused = [(ew.quantize_rows_mx4, (x[..., :40],)), (ew.quantize_rows_mx4, (x[..., :0],)),
+               (ew.quantize_rows_mx4, (x.int(),)), (ew.quantize_rows_mx4, (x[..., ::2],)),
+               (ew.quantize_rows_mx4, (x.transpose(0, 1),)), (ew.glu_mx4, (x[..., :32],)), (ew.glu_mx4, (x[..., :63],)),
+               (ew.glu_mx4, (x, w[:32])), (ew.glu_mx4, (x, w.cpu())), (ew.rms_modulate_mx4, (x[0], w, 1e-5)),
+               (ew.rms_modulate_mx4, (x, w[:32], 1e-5)), (ew.rms_modulate_mx4, (x, w, -1.0)),
+               (ew.rms_modulate_mx4, (x, w, 1e-5, mod)), (ew.rms_modulate_mx4, (x, w, 1e-5, mod, mod.float())),
+               (ew.rms_modulate_mx4, (x, w, 1e-5, mod[:1], mod[:1])), (ew.rms_modulate_mx4, (x, w.cpu(), 1e-5)),
+               (ew.rms_modulate_mx4, (rand(gen, 1, 2, 16416), rand(gen, 16416), 1e-5)),
+               (ew.residual_rms_mx4, (x, x[:1], w, 1e-5)), (ew.residual_rms_mx4, (x, x.float(), w, 1e-5)),
+               (ew.residual_rms_mx4, (x, x.cpu(), w, 1e-5)), (ew.residual_rms_mx4, (x, x, w[:32], 1e-5))]
+    q, s = ew.quantize_rows_mx4(x)
+    a, b = codes(gen, 24, 64)
+    refused += [(pr.linear_mx4, args) for args in (
+        (q.int(), s, a, b), (q, s.int(), a, b), (q, s, a.char(), b), (q, s, a, b.float()), (q, s, a[:, :16], b),
+        (q[..., :16], s, a, b), (q[..., :24], s, a[:, :24], b), (q, s[..., :1], a, b), (q, s[:1], a, b),
+        (q, s, a, b[:, :1]), (q, s, a, b[:20]), (q, s, a.cpu(), b), (q, s.cpu(), a, b), (q.cpu(), s.cpu(), a.cpu(), b.cpu()),
+        (q, s, a, b, w), (q, s, a, b, w[:24].cpu()), (q, s, a, b, None, torch.int8), (q, s, a, b, None, torch.float64),
+        (q, s, a[None], b[None]), (q, s, a.t().contiguous().t(), b))]
+    for i, (call, args) in enumerate(refused):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            call(*args)
+            pytest.fail(f"call {i} ({call.__name__}) was taken")
+
+
+def test_no_rows_and_one():
+    """Empty batches are refused, as by the 8-bit forms; one row of one group is a row."""
+    announce("mx4 no rows")
+    x = torch.zeros(0, 64, device=DEV, dtype=torch.bfloat16)
+    for call in (ew.quantize_rows, ew.quantize_rows_mx4, ew.glu_mx4):
+        with pytest.raises(ValueError):
+            call(x)
+    u = torch.zeros(0, 32, device=DEV, dtype=torch.uint8)
+    a, b = codes(generator(14), 24, 64)
+    with pytest.raises(ValueError):
+        pr.linear_mx4(u, u[:, :2], a, b)
+    q, s = ew.quantize_rows_mx4(torch.full((1, 32), 6.0, device=DEV))
+    check_exact(q, s, q, s, None, torch.float32, pr.linear_mx4(q, s, q, s, dtype=torch.float32))

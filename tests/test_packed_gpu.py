@@ -326,3 +326,63 @@ def test_on_another_stream():
     assert torch.equal(got, want)
     again = [pa.packed_attention(q, k, v, off, koff) for _ in range(3)]
     assert all(torch.equal(t, want) for t in again)
+
+
+def test_tokens_and_heads_past_32_bits():
+    """Keys, values, queries and outputs whose places pass 2^32 bytes: a token of each every 2 MB, heads 3 GB apart."""
+    announce("packed past 32 bits")
+    n, D, step = 2300, 64, 1 << 20
+    for name in ("bf16", "fp32"):
+        buf = torch.empty(n * step + 3 * D, dtype=DTYPES[name], device=DEV)
+        q, k, v = make(name, n, n, 1, 1, D, 22)
+        far = [buf.as_strided((n, 1, D), (step, D, 1), i * D) for i in range(3)]
+        for f, t in zip(far, (q, k, v)):
+            f.copy_(t)
+        lengths = [1000, 1, 1299]
+        want = pa.packed_attention(q, k, v, offsets(lengths))
+        assert torch.equal(pa.packed_attention(*far, offsets(lengths)), want)
+        few = [q[-3:], q[:3]]
+        at, koff = offsets([1, 2]), offsets([1000, 1300])
+        for rows in few:
+            assert torch.equal(pa.packed_attention(rows, far[1], far[2], at, koff),
+                               pa.packed_attention(rows, k, v, at, koff))
+        far[0].fill_(5)
+        got = pa.packed_attention(q, k, v, offsets(lengths), out=far[0])
+        assert torch.equal(got.clone(), want) and torch.equal(far[1].clone(), k)
+        wide = buf.as_strided((40, 2, D), (D, 800 * step, 1))
+        x, y, z = make(name, 40, 40, 2, 2, D, 23)
+        wide.copy_(y)
+        assert torch.equal(pa.packed_attention(x, wide, z, offsets([40])), pa.packed_attention(x, y, z, offsets([40])))
+        del buf, far, wide
+
+
+def test_wrapper_refusals():
+    announce("packed refusals")
+    q, k, v = make("bf16", 10, 10, 4, 2, 64, 24)
+    at = offsets([10])
+    calls = [
+        (ValueError, (q[0], k, v, at), {}), (ValueError, (q, k[..., 0], v, at), {}),
+        (TypeError, (q, k.half(), v, at), {}), (TypeError, (q, k, v.float(), at), {}),
+        (TypeError, (q, k.cpu(), v, at), {}), (ValueError, (q.cpu(), k.cpu(), v.cpu(), at.cpu()), {}),
+        (TypeError, (q.int(), k.int(), v.int(), at), {}),
+        (ValueError, (q[..., :32], k[..., :32], v[..., :32], at), {}), (ValueError, (q[:, :3], k, v, at), {}),
+        (ValueError, (q, k, v[:9], at), {}), (ValueError, (q, k[:9], v[:9], at), {}),
+        (ValueError, (q, k[:, :, ::2], v[:, :, ::2], at), {}), (ValueError, (q[:, :0], k, v, at), {}),
+        (ValueError, (q, k[:, :0], v[:, :0], at), {}), (TypeError, (q, k, v, at.long()), {}),
+        (TypeError, (q, k, v, at.cpu()), {}), (ValueError, (q, k, v, at[:0]), {}), (ValueError, (q, k, v, at[None]), {}),
+        (ValueError, (q, k, v, torch.zeros(4, dtype=torch.int32, device=DEV)[::2]), {}),
+        (ValueError, (q, k, v, at, offsets([5, 5])), {}), (TypeError, (q, k, v, at, at.float()), {}),
+        (ValueError, (q, k, v, at, at, at), {}), (TypeError, (q, k, v, at, at, at[1:].long()), {}),
+        (ValueError, (q, k, v, at), dict(out=q[:9])), (ValueError, (q, k, v, at), dict(out=torch.empty_like(q).half())),
+        (ValueError, (q, k, v, at), dict(out=torch.empty(10, 4, 64, dtype=q.dtype))),
+        (ValueError, (q, k, v, at), dict(out=torch.empty(10, 4, 128, device=DEV, dtype=q.dtype)[..., ::2])),
+        (ValueError, (q, k, v, at), dict(out=q)), (ValueError, (q, k, v, at), dict(scale=0.0)),
+        (ValueError, (q, k, v, at), dict(scale=-1.0)), (ValueError, (q, k, v, at), dict(scale=float("nan"))),
+        (ValueError, (q, k, v, at), dict(out=torch.empty(1, 4, 64, device=DEV, dtype=q.dtype).expand(10, 4, 64))),
+        (ValueError, (torch.empty(10, 4, 66, device=DEV, dtype=q.dtype)[..., 1:65], k, v, at), {}),
+        (ValueError, (torch.empty(10, 4, 68, device=DEV, dtype=q.dtype)[..., :64], k, v, at), {}),
+    ]
+    for i, (error, args, more) in enumerate(calls):
+        with pytest.raises(error):
+            pa.packed_attention(*args, **more)
+            pytest.fail(f"call {i} was taken")
