@@ -579,13 +579,15 @@ int64_t slots_of(int64_t T, int N, int gs) { return (T * gs + kTileRows - 1) / k
 // Parts of the keys: where the tiles do not give every CU three workgroups, as many as do (16 new tokens, 8 heads of keys of
 // 128: 58 us against 63 with two a CU), of 256 keys in the mean at least; 64 for fp32, whose 32 keys take 1.7 to 3.4 us where
 // 16-bit ones' 64 take 0.5 (7 sequences of new tokens over 2093 keys of 128: 49 -> 20 us; 16-bit parts of 128 keys cost up to
-// twice what they save). fp32 also splits for balance, to six workgroups a CU of 1024 keys (3223 tokens: 424 -> 377 us).
+// twice what they save). For balance as many as give six a CU, of 512 keys: fp32 tiles (3223 tokens: 424 -> 377 us) and
+// those of a wave's rows or fewer, which read at the memory's rate (one token of 16 sequences of up to 8249 keys, not in any
+// cache: 16 heads of 64 83 -> 72 us, 8 of 128 72 -> 69; other 16-bit tiles lose to it, 5828 tokens 121 -> 138).
 int splits_of(int dtype, int64_t T, int64_t Tk, int N, int H, int G) {
-  const int64_t tiles = slots_of(T, N, H / G) * G, want = 3 * device_cus(), mean = Tk / N;
+  const int64_t tiles = slots_of(T, N, H / G) * G, mean = Tk / N, cus = device_cus();
   auto smaller = [](int64_t x, int64_t y) { return x < y ? x : y; };
-  int64_t s = smaller(want / tiles, mean / (dtype == HB_F32 ? 64 : 256));
-  if (dtype == HB_F32) {
-    const int64_t even = smaller(2 * want / tiles, mean / 1024);
+  int64_t s = smaller(3 * cus / tiles, mean / (dtype == HB_F32 ? 64 : 256));
+  if (dtype == HB_F32 || T * (H / G) <= 32 * static_cast<int64_t>(N)) {
+    const int64_t even = smaller(6 * cus / tiles, mean / 512);
     if (even > s) s = even;
   }
   if (s > 64) s = 64;
