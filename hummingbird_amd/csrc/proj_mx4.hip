@@ -64,7 +64,9 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 // A workgroup of WF x WM waves computes FT features x MT rows in steps of 256 columns, which stream through kStages LDS
 // stages: code rows of 128 bytes whose 16-byte chunks are XOR-swizzled, then the rows' scales. A wave multiplies NF x NM
 // tiles of 32 x 32, of one 64-column block after the other, and reads the next block's operands meanwhile.
-// The scales are copied for kChunk steps at once, 32 bytes a row, into kBufs buffers of their own.
+// The scales are copied for kChunk steps at once, 32 bytes a row, into kBufs buffers of their own: blocks of 32 rows, the
+// rows' first 16 bytes and then their second ones, so that 32 rows' reads meet on a bank in twos (as rows of 32 bytes in fours:
+// 8249 x 1536 -> 12288 8.5 million conflict cycles, 3.6 so).
 // RAGGED: K ends inside two steps, or scale rows that are not aligned to 16 bytes. The scales of two steps then lie in two
 // 16-byte pieces, which are copied whole (each holds at least a byte of the row) and read from where they start.
 template <int FT_, int MT_, int WF_, int WM_, int WAVES_, int STAGES_ = 2>
@@ -81,7 +83,7 @@ template <class TL, bool RAGGED>
 struct Stage {
   static constexpr int kRows = TL::FT + TL::MT, kBytes = kRows * kStep;
   static constexpr int kChunk = RAGGED ? 2 : 4;  // steps whose scales are copied together
-  static constexpr int kScaleRow = 32, kScaleBytes = kRows * kScaleRow;
+  static constexpr int kScaleBytes = kRows * 32;
   // A chunk's copies start kStages steps before it, when the last reads of the chunk whose buffer it takes are over:
   // kBufs - 1 chunks, of two steps or (RAGGED) one where they are K's last, are kStages - 1 steps at least.
   static constexpr int kBufs = RAGGED ? TL::kStages : (TL::kStages + 2) / 2;
@@ -119,13 +121,13 @@ struct StageCopy {
       const int r = 8 * (wv + TL::NW * u) + r8;
       boff[u] = static_cast<uint32_t>((r < lastm ? r : lastm) * a.x_rs) + 16 * chunk;
     }
-    constexpr int kPieces = 2, kPer = 64 / kPieces;  // 16-byte pieces a row, rows a block
-    const int lane = threadIdx.x & 63, piece = lane % kPieces;
+    constexpr int kPer = 32;  // rows a block
+    const int lane = threadIdx.x & 63, piece = lane / kPer;
 #pragma unroll
     for (int u = 0; u < St::kBlocksS; ++u) {
       const int block = scale_block(u);
       const bool isa = block * kPer < TL::FT;
-      const int r = block * kPer + lane / kPieces - (isa ? 0 : TL::FT);
+      const int r = block * kPer + lane % kPer - (isa ? 0 : TL::FT);
       const int64_t last = isa ? lastf : lastm, rr = r < last ? r : last;
       const uint8_t* row = isa ? a.sw + (f0 + rr) * a.sw_rs : a.sx + (m0 + rr) * a.sx_rs;
       const int ahead = RAGGED ? static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) : 0;
@@ -178,10 +180,12 @@ struct Scales {
   // From the buffer `buf`, of the chunk's step `at`; `ahead`: where in its first piece the row starts.
   __device__ __forceinline__ void read(int t, const uint8_t* buf, int at, int fw, int mw, uint32_t ahead) {
     const int lr = threadIdx.x & 31, lh = (threadIdx.x & 63) >> 5;
-    const int row = t < TL::NF ? fw + 32 * t + lr : TL::FT + mw + 32 * (t - TL::NF) + lr;
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(buf + St::kScaleRow * row + 8 * at + 4 * lh + (ahead & ~3u));
+    const int first = t < TL::NF ? fw + 32 * t : TL::FT + mw + 32 * (t - TL::NF);  // of its block's rows
 #pragma unroll
-    for (int j = 0; j < kDwords; ++j) raw[t][j] = p[j];
+    for (int j = 0; j < kDwords; ++j) {
+      const int o = 8 * at + 4 * lh + (RAGGED ? static_cast<int>(ahead & ~3u) : 0) + 4 * j;  // byte of the row's 32
+      raw[t][j] = *reinterpret_cast<const uint32_t*>(buf + 32 * first + 512 * (o >> 4) + 16 * lr + (o & 15));
+    }
   }
   // Out of the dwords that hold them, those past K (`mask`) left out.
   __device__ __forceinline__ uint32_t get(int t, uint32_t ahead, uint32_t mask) const {
@@ -294,12 +298,12 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     int64_t m0;
     origin(tile, f0, m0);
     f32x16 acc[TL::NF][TL::NM];
+    // the first step's products start from zero (8249 x 1536 -> 12288: 116 us, 114 without registers to clear)
+    constexpr bool kPeel = kTiles <= 4;
+    if constexpr (!kPeel)
 #pragma unroll
-    for (int i = 0; i < TL::NF; ++i)
-#pragma unroll
-      for (int j = 0; j < TL::NM; ++j) acc[i][j] = f32x16{};
-#pragma unroll 1
-    for (int s = 0; s < nk; ++s) {
+      for (int i = 0; i < kTiles; ++i) acc[i / TL::NM][i % TL::NM] = f32x16{};
+    auto step = [&](int s, auto first) {
       chunk();  // with the copies that go on among the first block's products
       uint32_t mask = ~0u;  // the bytes of a lane half's scales that lie before K
       if constexpr (RAGGED) {
@@ -339,7 +343,9 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
               copy.one(kFrom + u, cs, a.K, J == 3 ? to : late);
           }
           const int ti = i / TL::NM, tj = i % TL::NM;
-          acc[ti][tj] = mfma_32x32x64<J>(blk[J & 1].a[ti], blk[J & 1].b[tj], acc[ti][tj], sc[ti], sc[TL::NF + tj]);
+          acc[ti][tj] = mfma_32x32x64<J>(blk[J & 1].a[ti], blk[J & 1].b[tj],
+                                         J == 0 && kPeel && decltype(first)::value ? f32x16{} : acc[ti][tj], sc[ti],
+                                         sc[TL::NF + tj]);
           __builtin_amdgcn_sched_barrier(0);
         }
         if constexpr (J == 0) advance();
@@ -349,7 +355,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
       block(std::integral_constant<int, 2>{});
       block(std::integral_constant<int, 3>{});
       late = to;
-    }
+    };
+    if constexpr (kPeel) step(0, std::true_type{});
+#pragma unroll 1
+    for (int s = kPeel ? 1 : 0; s < nk; ++s) step(s, std::false_type{});
 #pragma unroll
     for (int n = 0; n < TL::NF; ++n) {
       __builtin_amdgcn_sched_barrier(0);  // the biases of one n at a time: registers
