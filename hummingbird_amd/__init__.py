@@ -7,6 +7,8 @@
 * `hummingbird_amd.config.DiTConfig` / `SameConfig` with `attention="hip"`, and the call sites
   `hummingbird_amd.dit.self_attention` and `hummingbird_amd.same_l.attention`
   (reference: sa3jax/dit.py:185-200, sa3jax/same_l.py:151-169)
+* `hummingbird_amd.packed_attention.packed_attention` -- softmax attention over packed sequences: the model without the
+  second branch (`DiTConfig.differential = False`, sa3jax/dit.py:131-176), prompts and new tokens
 
 The kernels live in `libhummingbird_amd.so` (C ABI: include/hummingbird_amd.h), built with
 `python -m hummingbird_amd._build`. As in the reference package, the operators are reached through their

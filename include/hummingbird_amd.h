@@ -20,6 +20,10 @@
  *   hb_quant_rows, hb_rms_modulate_q8, hb_residual_rms_q8, hb_glu_q8, hb_proj_q8, hb_proj_q4
  *                      the denoiser's norms, GLU and projections on 8-bit rows and 8- or 4-bit weights (no
  *                      counterpart in the reference, which keeps 16-bit weights);
+ *   hb_quant_rows_mx4, hb_rms_modulate_mx4, hb_residual_rms_mx4, hb_glu_mx4, hb_proj_mx4
+ *                      the same on microscaled 4-bit rows and weights;
+ *   hb_packed_attention          softmax attention over packed sequences, whose lengths are on the device: the model
+ *                      without the second branch (sa3jax/dit.py:131-176), prompts, new tokens over their keys;
  *   hb_rope_tables     replaces  band_attention.rope_tables / dit._rope_tables
  *                      (sa3jax/band_attention.py:43-58, sa3jax/dit.py:82-87) in a kernel-native layout.
  *
