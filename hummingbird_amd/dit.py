@@ -59,7 +59,7 @@ class PackedContext(NamedTuple):
 
 def _even_offsets(batch: int, length: int, device: torch.device) -> torch.Tensor:
     """Where `batch` sequences of `length` tokens start, and the last one ends."""
-    return torch.arange(0, batch * length + 1, max(length, 1), dtype=torch.int32, device=device)[:batch + 1]
+    return torch.arange(batch + 1, dtype=torch.int32, device=device) * length
 
 
 def _plain_self_attention(qkv: torch.Tensor, attn: dict, static: dict, cfg: DiTConfig) -> torch.Tensor:
