@@ -298,11 +298,6 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     int64_t m0;
     origin(tile, f0, m0);
     f32x16 acc[TL::NF][TL::NM];
-    // the first step's products start from zero (8249 x 1536 -> 12288: 116 us, 114 without registers to clear)
-    constexpr bool kPeel = kTiles <= 4;
-    if constexpr (!kPeel)
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) acc[i / TL::NM][i % TL::NM] = f32x16{};
     auto step = [&](int s, auto first) {
       chunk();  // with the copies that go on among the first block's products
       uint32_t mask = ~0u;  // the bytes of a lane half's scales that lie before K
@@ -344,7 +339,7 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
           }
           const int ti = i / TL::NM, tj = i % TL::NM;
           acc[ti][tj] = mfma_32x32x64<J>(blk[J & 1].a[ti], blk[J & 1].b[tj],
-                                         J == 0 && kPeel && decltype(first)::value ? f32x16{} : acc[ti][tj], sc[ti],
+                                         J == 0 && decltype(first)::value ? f32x16{} : acc[ti][tj], sc[ti],
                                          sc[TL::NF + tj]);
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -356,9 +351,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
       block(std::integral_constant<int, 3>{});
       late = to;
     };
-    if constexpr (kPeel) step(0, std::true_type{});
+    // the first step's products start from zero (8249 x 1536 -> 12288: 116 us with registers to clear, 114 so)
+    step(0, std::true_type{});
 #pragma unroll 1
-    for (int s = kPeel ? 1 : 0; s < nk; ++s) step(s, std::false_type{});
+    for (int s = 1; s < nk; ++s) step(s, std::false_type{});
 #pragma unroll
     for (int n = 0; n < TL::NF; ++n) {
       __builtin_amdgcn_sched_barrier(0);  // the biases of one n at a time: registers
@@ -487,22 +483,24 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
 //   Small     up to 3/4 Medium tiles a CU (1422 x 1536, K = 6144: 18.8 against 21.3; but 2584 x 1536, K = 6144: 30.9 against
 //             23.1), with four stages where a CU has one such tile and more than four steps (400 x 1536, K = 6144: 11.6
 //             against 14.6);
-//   Huge      K of 4096 and more, and 3/4 tiles a CU at least: its products take half as many LDS reads (8249 x 1536,
-//             K = 6144: 51.1 against 56.6; 8192^3: 266 against 316), but one workgroup has the CU and nothing runs beside its
-//             epilogue (8249 x 12288: 128 against 119);
-//   Medium    the rest, two workgroups a CU (against 128 x 256 tiles 2584 x 12288: 42.1 and 47.2, 5168 x 7680: 49.7 and 49.1,
-//             8249 x 12288: 119 and 125; 128 x 64: 48.6, 58.7, 144).
+//   Huge      K of 4096 and more, and a tile for half of the CUs: eight waves that share their copies and read a quarter
+//             less from LDS (8192^3: 245 against 316, 20000 x 4096 -> 1536: 69 and 79, 3000 x 6144 -> 3000: 42 and 48); from
+//             K = 1536 on where they fill their rounds to seven eighths (8249 x 12288: 115 against 119, 5168 x 12288: 66 and
+//             73; but after a norm, at a higher clock, 5168 x 7680, 630 tiles: 56 and 53, 2584 x 12288, 528: 42.5 and 37.9), as
+//             one workgroup has the CU and little runs beside its epilogue (8192 x 512 -> 8192: 53 and 40);
+//   Medium    the rest, two workgroups a CU (against 128 x 64 tiles 2584 x 12288: 42.1 and 48.6, 5168 x 7680: 49.7 and 58.7).
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
   using Small = Tile<64, 64, 2, 2, 3>;
   using Medium = Tile<128, 128, 2, 2, 2>;
-  using Huge = Tile<256, 256, 2, 2, 1>;
+  using Huge = Tile<256, 256, 4, 2, 2>;
   const int64_t cus = device_cus(), small = tiles_of<Small>(a);
   if (a.M <= 16) return launch_few_rows<T, 1>(stream, a);
   if (a.M <= 32 && small <= cus / 4) return launch_few_rows<T, 2>(stream, a);
   if (small <= cus && a.K > 4 * kCols) return launch_tiled<T, Tile<64, 64, 2, 2, 1, 4>>(stream, a);
   if (tiles_of<Medium>(a) <= cus * 3 / 4) return launch_tiled<T, Small>(stream, a);
-  if (a.K >= 4096 && tiles_of<Huge>(a) >= cus * 3 / 4) return launch_tiled<T, Huge>(stream, a);
+  const int64_t huge = tiles_of<Huge>(a), places = (huge + cus - 1) / cus * cus;
+  if (a.K >= 4096 ? huge >= cus / 2 : a.K >= 1536 && huge >= places * 7 / 8) return launch_tiled<T, Huge>(stream, a);
   launch_tiled<T, Medium>(stream, a);
 }
 
