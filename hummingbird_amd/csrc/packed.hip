@@ -15,7 +15,7 @@
 // with P rounded to it (its sum is of the rounded values); fp32 on the fp32 cores with P in fp32. Statistics and sums are fp32.
 //
 // Bound by the matrix cores and, at 64 dims, the exponentials beside them: bf16, 8249 and 7001 tokens, causal, 16 heads of
-// 128 to 4 508 us (1.0 PFLOP/s), 4 x 1300 tokens, 16 heads of 64 45 us (646 TFLOP/s); one new token by the keys' bytes: 16
+// 128 to 4 503 us (1.0 PFLOP/s), 4 x 1300 tokens, 16 heads of 64 44 us (655 TFLOP/s); one new token by the keys' bytes: 16
 // sequences, 287 MB 65 us (4.4 TB/s).
 //
 // The lengths are read on the device: the grid has a slot for every tile that the rows could need (a sequence wastes less

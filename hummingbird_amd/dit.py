@@ -261,11 +261,11 @@ def quantize_params(params: dict, conditioning: str = "q4", weights: str = "q8")
     conditioning layers as 4-bit weights (`projection.quantize_q4`, with the bias in fp32), under `"q4"`.
     `conditioning="keep"` leaves those layers on the weights as they are: they are a few rows of work, but every block
     reads their result, and their 4 bits make most of the 8-bit form's error. Medium width, random weights, the output's
-    distance from the 16-bit one at 2, 12 and 24 blocks as a part of its norm, and a render of 1422 tokens in 8 steps (62.7
+    distance from the 16-bit one at 2, 12 and 24 blocks as a part of its norm, and a render of 1422 tokens in 8 steps (62.3
     ms with 16 bits):
 
-        "q8"   "q4"   9 %, 19 %, 26 %   43.6 ms        "mx4"  "q4"   18 %, 42 %, 56 %  39.7 ms
-               "keep" 4 %,  9 %, 12 %   44.0 ms               "keep" 16 %, 39 %, 52 %  40.1 ms
+        "q8"   "q4"   9 %, 19 %, 26 %   42.9 ms        "mx4"  "q4"   18 %, 42 %, 56 %  38.8 ms
+               "keep" 4 %,  9 %, 12 %   43.4 ms               "keep" 16 %, 39 %, 52 %  39.2 ms
 
     The other tensors are shared, not copied. The 16-bit weights stay beside the others (2.4 GB of the medium model, 1.2 the
     8-bit and 0.6 the 4-bit ones), so that the other `projections` still run; where only one does, the `"weight"` entries of

@@ -302,6 +302,29 @@ def test_product_sums_are_fp32(M):
     assert float((err / mag).mean()) < 2.0 ** -21
 
 
+@pytest.mark.parametrize("M", [4, 64, 300])
+def test_product_sums_across_scales(M):
+    """Groups of very different scales: nothing of the small ones is cut off before the sum is rounded. A large and a small
+    product in two groups give their sum exactly while it has 24 bits; random rows, whose groups' own sums are exact, are
+    within a rounding per group."""
+    announce("linear_mx4 sums across scales", M)
+    gen = generator(15, M)
+    for big, low in ((0, 4), (0, 1), (0, 2), (1, 5), (4, 0), (7, 3)):
+        for d in range(19):
+            x, xs = torch.zeros(M, 128, dtype=torch.uint8, device=DEV), torch.full((M, 8), 127, dtype=torch.uint8, device=DEV)
+            w, ws = torch.zeros(64, 128, dtype=torch.uint8, device=DEV), torch.full((64, 8), 127, dtype=torch.uint8, device=DEV)
+            x[:, 16 * big], w[:, 16 * big], x[:, 16 * low], w[:, 16 * low], xs[:, low] = 7, 7, 2, 2, 127 - d
+            assert (pr.linear_mx4(x, xs, w, ws, dtype=torch.float32) == 36 + 2.0 ** -d).all(), (big, low, d)
+    K = 256
+    for spread in (0, 5, 10, 16, 30):
+        x, xs = codes(gen, M, K, 127 - spread, 127)
+        w, ws = codes(gen, 64, K, 127 - spread, 127)
+        out = pr.linear_mx4(x, xs, w, ws, dtype=torch.float32).double()
+        a, b = values(x, xs), values(w, ws)
+        err, mag = (out - a @ b.t().contiguous()).abs(), a.abs() @ b.abs().t().contiguous()
+        assert (err <= (K // 32 + 1) * 2.0 ** -24 * mag).all(), spread
+
+
 def test_captured_and_on_another_stream():
     """Two graphs of one layer, replayed in turn with eager calls between, and a call on a stream of its own."""
     announce("mx4 graphs")
