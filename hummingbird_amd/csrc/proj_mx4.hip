@@ -247,10 +247,15 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     aim();
   };
   constexpr int kTiles = TL::NF * TL::NM, kReads = Block<TL>::kReads, kCopies = StageCopy<TL, RAGGED>::kCopies;
-  // A step has four blocks of kTiles products. When its last block is in registers everywhere and the next step's copies
-  // have landed (the one barrier of a step, before the last block's products), the stage is free: the step kStages on is
-  // copied into it, kFirst copies among the last block's products and the others among the next step's first.
-  constexpr int kFirst = 3 * kCopies / 4;
+  // A step has four blocks of kTiles products. With one product a block (kWhole) a step's products take less time than a read
+  // from LDS, so all of a step's operands are in registers when it begins: the barrier comes first, the stage is free for
+  // the step kStages on, and each block's registers take the next step's operands behind its product (in a graph, 154 x
+  // 4096 -> 1024: 9.1 -> 8.6 us, 400 x 6144 -> 1536: 12.6 -> 11.7).
+  // With more, the reads run a block ahead of the products. When a step's last block is in registers everywhere and the next
+  // step's copies have landed (the one barrier of a step, before the last block's products), the stage is free: the step
+  // kStages on is copied into it, kFirst copies among the last block's products and the others among the next step's first.
+  constexpr bool kWhole = kTiles == 1;
+  constexpr int kFirst = kWhole ? kCopies : 3 * kCopies / 4;
   auto chunk = [&]() {
     if (cs % St::kChunk == 0) copy.scales(cs, __builtin_amdgcn_readfirstlane(lds0 + cbuf));
   };
@@ -259,10 +264,10 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   for (int i = 0; i < TL::kStages; ++i) {
 #pragma unroll
     for (int u = 0; u < (i == TL::kStages - 1 ? kFirst : kCopies); ++u) {
-      if (u == 0 && i < TL::kStages - 1) chunk();
+      if (u == 0 && (kWhole || i < TL::kStages - 1)) chunk();
       copy.one(u, cs, a.K, lds0 + i * St::kBytes);
     }
-    if (i < TL::kStages - 1) advance();
+    if (kWhole || i < TL::kStages - 1) advance();
   }
   wait_copies<(TL::kStages - 2) * kCopies + kFirst>();
   wait_lds();
@@ -286,10 +291,14 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
   };
   find_ahead(blockIdx.x);
   uint32_t sbuf = kScales0;  // the buffer of the next scales
-  Block<TL> blk[2];
+  Block<TL> blk[kWhole ? 4 : 2];
   Scales<TL, RAGGED> next;
 #pragma unroll
-  for (int i = 0; i < kReads; ++i) blk[0].read(i, smem, fw, mw, 0), next.read(i, smem + sbuf, 0, fw, mw, ahead[i]);
+  for (int i = 0; i < kReads; ++i) {
+#pragma unroll
+    for (int j = 0; j < (kWhole ? 4 : 1); ++j) blk[j].read(i, smem, fw, mw, j);
+    next.read(i, smem + sbuf, 0, fw, mw, ahead[i]);
+  }
 
   uint32_t b = 0;                                                                     // byte offset of the step's stage
   uint32_t late = __builtin_amdgcn_readfirstlane(lds0 + (TL::kStages - 1) * St::kBytes);  // the stage whose copies go on
@@ -299,6 +308,11 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
     origin(tile, f0, m0);
     f32x16 acc[TL::NF][TL::NM];
     auto step = [&](int s, auto first) {
+      if constexpr (kWhole) {
+        wait_copies<(TL::kStages - 2) * kCopies>();
+        wait_lds();
+        barrier();
+      }
       chunk();  // with the copies that go on among the first block's products
       uint32_t mask = ~0u;  // the bytes of a lane half's scales that lie before K
       if constexpr (RAGGED) {
@@ -318,6 +332,21 @@ __global__ __launch_bounds__(64 * TL::NW) __attribute__((amdgpu_waves_per_eu(TL:
       b = b == (TL::kStages - 1) * St::kBytes ? 0 : b + St::kBytes;
       auto block = [&](auto which) {
         constexpr int J = decltype(which)::value;
+        if constexpr (kWhole) {
+          if constexpr (J == 0) {
+#pragma unroll
+            for (int u = 0; u < kCopies; ++u) copy.one(u, cs, a.K, to);
+            advance();
+          }
+          acc[0][0] = mfma_32x32x64<J>(blk[J].a[0], blk[J].b[0], J == 0 && decltype(first)::value ? f32x16{} : acc[0][0],
+                                       sc[0], sc[1]);
+#pragma unroll
+          for (int r = 0; r < kReads; ++r) {
+            blk[J].read(r, smem + b, fw, mw, J);
+            if constexpr (J == 0) next.read(r, smem + sbuf, at, fw, mw, ahead[r]);
+          }
+          return;
+        }
         if constexpr (J == 3) {
           wait_copies<(TL::kStages - 2) * kCopies>();
           wait_lds();
@@ -481,8 +510,8 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
 // Which kernel, as measured (us, of which a call's host part is 7.7; K = 1536 unless said). In order:
 //   few rows  up to 16 rows, and up to 32 of a narrow product (24 x 1536, K = 6144: 9.5 against 11.0 Small);
 //   Small     up to 3/4 Medium tiles a CU (1422 x 1536, K = 6144: 18.8 against 21.3; but 2584 x 1536, K = 6144: 30.9 against
-//             23.1), with four stages where a CU has one such tile and more than four steps (400 x 1536, K = 6144: 11.6
-//             against 14.6);
+//             23.1), with three stages where a CU has one such tile and K is 4096 or more (400 x 1536, K = 6144, in a graph:
+//             11.5 against 12.2; 333 x 1001, K = 1056: 6.1 and 5.9);
 //   Huge      K of 4096 and more, and a tile for half of the CUs: eight waves that share their copies and read a quarter
 //             less from LDS (8192^3: 245 against 316, 20000 x 4096 -> 1536: 69 and 79, 3000 x 6144 -> 3000: 42 and 48); from
 //             K = 1536 on where they fill their rounds to seven eighths (8249 x 12288: 115 against 119, 5168 x 12288: 66 and
@@ -497,7 +526,7 @@ void launch(hipStream_t stream, const Args& a) {
   const int64_t cus = device_cus(), small = tiles_of<Small>(a);
   if (a.M <= 16) return launch_few_rows<T, 1>(stream, a);
   if (a.M <= 32 && small <= cus / 4) return launch_few_rows<T, 2>(stream, a);
-  if (small <= cus && a.K > 4 * kCols) return launch_tiled<T, Tile<64, 64, 2, 2, 1, 4>>(stream, a);
+  if (small <= cus && a.K >= 4096) return launch_tiled<T, Tile<64, 64, 2, 2, 1, 3>>(stream, a);
   if (tiles_of<Medium>(a) <= cus * 3 / 4) return launch_tiled<T, Small>(stream, a);
   const int64_t huge = tiles_of<Huge>(a), places = (huge + cus - 1) / cus * cus;
   if (a.K >= 4096 ? huge >= cus / 2 : a.K >= 1536 && huge >= places * 7 / 8) return launch_tiled<T, Huge>(stream, a);

@@ -214,7 +214,8 @@ SHAPES = [(1, 32, 1), (7, 1536, 7680), (16, 96, 17), (17, 64, 15), (31, 1056, 51
           (65, 288, 65), (100, 2048, 129), (129, 1536, 257), (257, 1024, 1001), (700, 1536, 1536), (700, 1056, 1537),
           (1422, 1536, 1536), (1300, 512, 4096), (2584, 800, 1536), (2049, 1536, 7680), (1025, 1504, 12288),
           (3900, 4096, 3300), (3841, 4128, 3329), (24, 4096, 1000), (300, 2048, 1000), (4000, 1536, 8190),
-          (4001, 1568, 8190), (2900, 4096, 3000)]
+          (4001, 1568, 8190), (2900, 4096, 3000),
+          (90, 4128, 200), (1400, 544, 1500)]
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
