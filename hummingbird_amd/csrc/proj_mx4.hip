@@ -517,7 +517,8 @@ void launch_few_rows(hipStream_t stream, const Args& a) {
 //             K = 1536 on where they fill their rounds to seven eighths (8249 x 12288: 115 against 119, 5168 x 12288: 66 and
 //             73; but after a norm, at a higher clock, 5168 x 7680, 630 tiles: 56 and 53, 2584 x 12288, 528: 42.5 and 37.9), as
 //             one workgroup has the CU and little runs beside its epilogue (8192 x 512 -> 8192: 53 and 40);
-//   Medium    the rest, two workgroups a CU (against 128 x 64 tiles 2584 x 12288: 42.1 and 48.6, 5168 x 7680: 49.7 and 58.7).
+//   Medium    the rest, two workgroups a CU, or one of eight waves where that is all there is (in a graph, 2584 x 1536: 9.3
+//             against 9.7; 1422 x 2600: 9.3 and 9.6) (against 128 x 64 tiles 2584 x 12288: 42.1 and 48.6, 5168 x 7680: 49.7 and 58.7).
 template <typename T>
 void launch(hipStream_t stream, const Args& a) {
   using Small = Tile<64, 64, 2, 2, 3>;
@@ -530,6 +531,7 @@ void launch(hipStream_t stream, const Args& a) {
   if (tiles_of<Medium>(a) <= cus * 3 / 4) return launch_tiled<T, Small>(stream, a);
   const int64_t huge = tiles_of<Huge>(a), places = (huge + cus - 1) / cus * cus;
   if (a.K >= 4096 ? huge >= cus / 2 : a.K >= 1536 && huge >= places * 7 / 8) return launch_tiled<T, Huge>(stream, a);
+  if (tiles_of<Medium>(a) <= cus) return launch_tiled<T, Tile<128, 128, 4, 2, 2>>(stream, a);
   launch_tiled<T, Medium>(stream, a);
 }
 

@@ -74,7 +74,7 @@ def run(h, net, attend, seen=None):
     return h
 
 
-def checker(name):
+def comparing(name):
     half_step = torch.finfo(DTYPES[name]).eps / 2
     least = 2.0 ** -24 if name == "fp16" else 0.0  # half's subnormals
 
@@ -125,7 +125,7 @@ def test_prompts_and_new_tokens(name):
             cache[where] = t
         return out
 
-    h = run(rand(generator(21), T, E, dtype=dtype), net, prompts, checker(name))
+    h = run(rand(generator(21), T, E, dtype=dtype), net, prompts, comparing(name))
     assert torch.isfinite(h).all()
     slot_offsets, one_each = offsets(slots), offsets([1] * len(slots))
     for step in range(room):
@@ -140,7 +140,7 @@ def test_prompts_and_new_tokens(name):
             check(out, q, *caches[i], [1] * len(slots), held, starts, True, scale, name, f"token {step}, layer {i}")
             return out
 
-        h = run(rand(generator(22, step), len(slots), E, dtype=dtype), net, tokens, checker(name))
+        h = run(rand(generator(22, step), len(slots), E, dtype=dtype), net, tokens, comparing(name))
         assert torch.isfinite(h).all()
 
 
