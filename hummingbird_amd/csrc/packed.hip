@@ -220,16 +220,17 @@ struct Rows {
       for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] = f32x16{};
     }
   }
-  // A total or a sum that is NaN or infinite.
+  // A total of 2^100 or more, a sum of 2^120 or more, or a NaN in either: what is added later (the total's other half, the
+  // parts' totals and sums) stays in range for the others. The total is the whole row's, of both halves of the wave.
   __device__ __forceinline__ bool wild() const {
     bool found = false;
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
-      found |= !(l[ct] < INFINITY);
+      found |= !(l[ct] + __shfl_xor(l[ct], 32, kWave) < 0x1p100f);
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) found |= !(fabsf(o[ct][dt][i]) < INFINITY);
+        for (int i = 0; i < 16; ++i) found |= !(fabsf(o[ct][dt][i]) < 0x1p120f);
     }
     return found;
   }
@@ -424,7 +425,7 @@ struct Rows {
 
 // A NaN or an infinity in the values of a key that a row does not see meets a probability of zero, and their product is NaN;
 // a score 2^127 above the reference gives an infinity. Both are rare: the sums are taken as they come, and a workgroup that
-// finds a NaN or an infinity in them repeats its tile with care. The other rows get the same sums as before, bit for bit.
+// finds a NaN or a large one in them repeats its tile with care. The other rows get the same sums as before, bit for bit.
 template <class E, int D, int NCT, int NW, int WAVES>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) void attend_kernel(const Args a) {
   using L = Lds<E, D>;

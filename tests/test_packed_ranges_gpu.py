@@ -1,0 +1,122 @@
+"""Attention over packed sequences on the GPU where scores and values span the range of their types: scores far above those
+that came first, alone and in parts that are joined, values whose sums pass the range, rows beside such ones. Against the
+plain fp64 implementation of `test_packed_gpu`, with its tolerances."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from hummingbird_amd import _lib
+from hummingbird_amd import packed_attention as pa
+from tests import test_packed_gpu as plain
+
+pytestmark = pytest.mark.gpu
+DEV, DTYPES, CODES = plain.DEV, plain.DTYPES, {"bf16": 0, "fp32": 1, "fp16": 2}
+
+
+def scored(name, scores, D=64):
+    """Keys `(n, 1, D)` whose products with queries of 4 in their first two values, scaled by 1/4, are `scores` `(n,)`
+    exactly: multiples of 1/4 up to 128 in magnitude, a whole number and a fraction, each of 8 bits at most."""
+    k = torch.zeros(scores.shape[0], 1, D, device=DEV)
+    k[:, 0, 0] = torch.trunc(scores)
+    k[:, 0, 1] = scores - k[:, 0, 0]
+    return k.to(DTYPES[name])
+
+
+def queries(name, n, D=64):
+    q = torch.zeros(n, 1, D, device=DEV)
+    q[..., :2] = 4.0
+    return q.to(DTYPES[name])
+
+
+def values(name, n, size, seed, D=64):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    return (size * (0.5 + 0.5 * torch.rand(n, 1, D, generator=gen, device=DEV))).to(DTYPES[name])
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("size", [2.0 ** -10, 0.25, 1.0])
+def test_scores_above_the_first_tile(name, size):
+    """64 keys of score 0 and then 64 of x, x from 60 to 100 in quarters: totals that pass 2^128 in a lane's half of the
+    keys, in the two halves together and not at all."""
+    plain.announce("packed scores above the first tile", name, size)
+    x = torch.arange(60, 100.25, 0.25, device=DEV)
+    n = x.numel()
+    k = scored(name, torch.stack([torch.zeros_like(x), x], dim=1).repeat_interleave(64, dim=1).reshape(-1))
+    v = values(name, 128 * n, size, 1)
+    lq, lk = [3] * n, [128] * n
+    q, starts = queries(name, 3 * n), [128 * i for i in range(n)]
+    for causal in (False, True):
+        got = pa.packed_attention(q, k, v, plain.offsets(lq), plain.offsets(lk), causal=causal, scale=0.25)
+        plain.check(got, q, k, v, lq, lk, starts, causal, 0.25, name, causal)
+
+
+def split(name, T, Tk, N, D=64):
+    """How many parts a call of one head has (0: one)."""
+    return _lib.load().hb_packed_workspace_size(CODES[name], T, Tk, N, 1, 1, D) // (T * (D + 2) * 4)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("size", [2.0 ** -10, 1.0])
+def test_parts_of_far_references(name, size):
+    """One token over keys in parts, most of them x below, x from 60 to 100: of two keys that weigh alike one lies behind
+    its part's first tile, which is x below it, and the other begins its part."""
+    plain.announce("packed parts of far references", name, size)
+    low = -torch.arange(60, 101, 1, device=DEV, dtype=torch.float32)
+    n, keys = low.numel(), 5000
+    assert split(name, n, n * keys, n)
+    scores = low[:, None].repeat(1, keys)
+    scores[:, 100], scores[:, 320] = -0.25, 0.0
+    q, k, v = queries(name, n), scored(name, scores.reshape(-1)), values(name, n * keys, size, 2)
+    starts = [keys * i for i in range(n)]
+    got = pa.packed_attention(q, k, v, plain.offsets([1] * n), plain.offsets([keys] * n), scale=0.25)
+    plain.check(got, q, k, v, [1] * n, [keys] * n, starts, True, 0.25, name, "far references")
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_parts_with_large_totals(name):
+    """Parts that all begin with 64 keys of score 0 and go on with x, x from 60 to 100: totals of 2^100 to 2^128 each,
+    which are added; parts that begin with scores of minus infinity; every row in one part, most of its keys low."""
+    plain.announce("packed parts with large totals", name)
+    x = torch.arange(60, 101, 1, device=DEV, dtype=torch.float32)
+    n, keys = x.numel(), 5000
+    assert split(name, n, n * keys, n)
+    at = torch.arange(keys, device=DEV)
+    q, v = queries(name, n), values(name, n * keys, 1.0, 3)
+    starts = [keys * i for i in range(n)]
+    for what, first in (("zero", 0.0), ("minus infinity", float("-inf"))):
+        scores = torch.where(at % 64 % 5 == 0 if what == "zero" else at < 320, first, x[:, None].expand(n, keys))
+        scores[:, :64] = first
+        scores[:, at % 320 < 64] = first
+        k = scored(name, torch.nan_to_num(scores, neginf=0.0).reshape(-1))
+        k[..., 0].masked_fill_(torch.isinf(scores).reshape(-1, 1), float("-inf"))
+        got = pa.packed_attention(q, k, v, plain.offsets([1] * n), plain.offsets([keys] * n), scale=0.25)
+        plain.check(got, q, k, v, [1] * n, [keys] * n, starts, True, 0.25, name, what)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+def test_bits_do_not_depend_on_the_neighbours(name):
+    """Rows of the tile in which one is repeated (a NaN in a value that the others do not see, scores of another row that
+    pass the range) have the bits that they have without it, whatever their own scores' range."""
+    plain.announce("packed bits beside", name)
+    n, D = 128, 64
+    q, k, v = plain.make(name, n, n, 1, 1, D, 31)
+    q, k = q * 0.5, k * 0.5
+    q[..., 0] = 4.0
+    at = plain.offsets([n])
+    for x in (0.0, 3.0, 60.0, 70.0, 73.0, 76.0, 80.0, 83.0, 86.0, 88.0, 95.0):
+        kk = k.clone()
+        kk[:, :, 0] = 0.0
+        kk[64:, :, 0] = x
+        want = pa.packed_attention(q, kk, v, at, causal=True, scale=0.25)
+        vv = v.clone()
+        vv[127] = float("nan")
+        got = pa.packed_attention(q, kk, vv, at, causal=True, scale=0.25)
+        assert torch.equal(got[:127], want[:127]), x
+        assert torch.isnan(got[127]).all() and torch.isfinite(want).all()
+        qq = q.clone()
+        qq[100, :, 0] = 400.0  # its scores pass the first tile's by a hundred times as much
+        for causal in (False, True):
+            want = pa.packed_attention(q, kk, v, at, causal=causal, scale=0.25)
+            got = pa.packed_attention(qq, kk, v, at, causal=causal, scale=0.25)
+            assert torch.equal(got[:100], want[:100]) and torch.equal(got[101:], want[101:]), (x, causal)
