@@ -506,13 +506,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
     if (a.splits > 1) {
       const int64_t at = (static_cast<int64_t>(part) * a.T + token[ct]) * a.H + head[ct];
       float* po = a.part_o + at * D;
+      // The join weighs a part by 2^(its reference - the largest one), which is lost where it is no normal number. A
+      // reference under a total of 2^32 and more is raised by the total's exponent (the factor is exact); under a smaller
+      // one a lost part is less than 2^-90 of the result's weights.
+      const bool raise = total >= 0x1p32f && total < INFINITY;
+      const int up = raise ? static_cast<int>(__float_as_uint(total) >> 23) - 127 : 0;
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * i + 4 * lh) =
-              f32x4{w.o[ct][dt][4 * i], w.o[ct][dt][4 * i + 1], w.o[ct][dt][4 * i + 2], w.o[ct][dt][4 * i + 3]};
-      if (lh == 0) a.part_ml[2 * at] = w.m[ct], a.part_ml[2 * at + 1] = total;
+              f32x4{w.o[ct][dt][4 * i] * down, w.o[ct][dt][4 * i + 1] * down, w.o[ct][dt][4 * i + 2] * down,
+                    w.o[ct][dt][4 * i + 3] * down};
+      if (lh == 0) a.part_ml[2 * at] = w.m[ct] + static_cast<float>(up), a.part_ml[2 * at + 1] = total * down;
       continue;
     }
     const float inv = total == 0.f ? 0.f : __frcp_rn(total);

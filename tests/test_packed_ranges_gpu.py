@@ -74,6 +74,26 @@ def test_parts_of_far_references(name, size):
 
 
 @pytest.mark.parametrize("name", list(DTYPES))
+def test_parts_that_weigh_little(name):
+    """A part with a key of score 0 and others whose first tiles lie x below, x from 80 to 92, with one key each 69.25 above that (99.9
+    binary orders): a weight of 2e-5 to 1e-10 each, under values so large that together they are seen."""
+    plain.announce("packed parts that weigh little", name)
+    low = -torch.arange(80, 92.25, 0.25, device=DEV)
+    n, keys = low.numel(), 5000
+    each = -(-keys // split(name, n, n * keys, n))
+    each += -each % 64  # 16-bit parts' keys
+    assert each >= 64
+    scores = low[:, None].repeat(1, keys)
+    scores[:, each + 150::each] = low[:, None] + 69.25
+    scores[:, 0] = 0.0
+    q, k, v = queries(name, n), scored(name, scores.reshape(-1)), values(name, n * keys, 1.0, 2)
+    v.view(n, keys, 64)[:, each + 150::each] *= 2.0 ** (19 if name != "fp16" else 15)
+    starts = [keys * i for i in range(n)]
+    got = pa.packed_attention(q, k, v, plain.offsets([1] * n), plain.offsets([keys] * n), scale=0.25)
+    plain.check(got, q, k, v, [1] * n, [keys] * n, starts, True, 0.25, name, "weigh little")
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
 def test_parts_with_large_totals(name):
     """Parts that all begin with 64 keys of score 0 and go on with x, x from 60 to 100: totals of 2^100 to 2^128 each,
     which are added; parts that begin with scores of minus infinity; every row in one part, most of its keys low."""
