@@ -203,6 +203,13 @@ __device__ __forceinline__ u32x4 v_operand(const uint8_t* sV, int dt, int g) {
   return u32x4{ux[0], ux[1], uy[0], uy[1]};
 }
 
+// How a tile's rows are computed. kPlain takes every sum as it comes. Rows that come out with a NaN or in need of range
+// (Rows::again) are computed again by themselves: kApart the same way but that a NaN or an infinity in the values of a key
+// reaches only the rows that see it (else its product with their probability of zero is a NaN), and those that still are out
+// of range kExact, from the largest score of each row. Both are rare, and the other rows keep what they have: no row's bits
+// depend on its neighbours, or on keys that it does not see.
+enum Pass { kPlain, kApart, kExact };
+
 // The rows of a wave, NCT times 32 of them, MFMA columns: what it holds between key tiles.
 template <class E, int D, int NCT>
 struct Rows {
@@ -211,28 +218,32 @@ struct Rows {
   f32x16 o[NCT][D / 32];
   float m[NCT], l[NCT];
   int lim[NCT];  // keys that this lane's row sees
+  uint64_t taken[NCT] = {};  // which of o's values took a NaN or an infinity of V's in the rows computed again: 16 dt + i
 
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void clear(int ct) {
+    m[ct] = -INFINITY, l[ct] = 0.f;
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) {
-      m[ct] = -INFINITY, l[ct] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] = f32x16{};
-    }
+    for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] = f32x16{};
   }
-  // A total of 2^100 or more, a sum of 2^120 or more, or a NaN in either: what is added later (the total's other half, the
-  // parts' totals and sums) stays in range for the others. The total is the whole row's, of both halves of the wave.
-  __device__ __forceinline__ bool wild() const {
-    bool found = false;
+  // Clears the rows that are to be computed again, and lets the others see no key, so that they stay as they are. Those with a
+  // NaN, a total of 2^100 or more (the whole row's, of both halves of the wave) or a sum of 2^120 or more that it did not take
+  // from V: what is added to the others later (the parts' totals and sums) stays in range. Whether this wave has one.
+  __device__ __forceinline__ bool again() {
+    const int lane = threadIdx.x & 63;
+    bool any = false;
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
-      found |= !(l[ct] + __shfl_xor(l[ct], 32, kWave) < 0x1p100f);
+      bool found = !(l[ct] + __shfl_xor(l[ct], 32, kWave) < 0x1p100f);
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) found |= !(fabsf(o[ct][dt][i]) < 0x1p120f);
+        for (int i = 0; i < 16; ++i) found |= !(fabsf(o[ct][dt][i]) < 0x1p120f) && !(taken[ct] >> (16 * dt + i) & 1);
+      const uint64_t lanes = __ballot(found);
+      any |= lanes != 0;
+      if (((lanes >> 32 | lanes) >> (lane & 31)) & 1) clear(ct);
+      else lim[ct] = 0;
     }
-    return found;
+    return any;
   }
 
   // The scores of 32 RT keys.
@@ -262,11 +273,11 @@ struct Rows {
   // The scores' probabilities: 16-bit ones in p, fp32 ones in the scores' place. The reference m is a row's maximum over the
   // first tile, and follows the maximum only where that has passed it by 2^kSlack: larger probabilities lose nothing while
   // they are in range, and o is seldom multiplied. bf16 ones are to 2^127: the maximum of the tiles after the first is not
-  // looked at (causal, 8192 tokens, 24 heads of 64: 246 -> 233 us) unless `careful`. No row's sums depend on its neighbours.
+  // looked at (causal, 8192 tokens, 24 heads of 64: 246 -> 233 us).
   static constexpr bool kWide = std::is_same<E, E16<Bf16Io>>::value;
   static constexpr float kSlack = kWide ? 100.f : 8.f;
   __device__ __forceinline__ void softmax(int ct, f32x16 (&sc)[RT], u32x4 (&p)[RT][2], int k0, float c, bool masked,
-                                          bool first, bool careful) {
+                                          bool first) {
     const int lh = (threadIdx.x & 63) >> 5;
     if (masked) {
 #pragma unroll
@@ -274,7 +285,7 @@ struct Rows {
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[rt][r] : -INFINITY;
     }
-    if (!kWide || first || careful) {
+    if (!kWide || first) {
       float top = -INFINITY;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -282,8 +293,8 @@ struct Rows {
         for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[rt][r]);
       const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-      // a first tile with nothing but scores of minus infinity has no reference for the later ones: wild()
-      if (kWide && !careful && top == -INFINITY && k0 < lim[ct]) l[ct] = NAN;
+      // a first tile with nothing but scores of minus infinity has no reference for the later ones: again()
+      if (kWide && top == -INFINITY && k0 < lim[ct]) l[ct] = NAN;
       const bool passed = top > m[ct] + kSlack;
       if (__any(passed)) {
         const float alpha = passed ? fast_exp2(m[ct] - top) : 1.f;
@@ -311,16 +322,78 @@ struct Rows {
       }
   }
 
-  // One key tile; `masked`: some row does not see all of its keys from k0 on. `careful`: every maximum is looked at, and V's
-  // NaNs and infinities reach only the rows that see their keys.
-  __device__ __forceinline__ void step(const uint8_t* sK, const uint8_t* sV, int k0, float c, bool masked, bool first,
-                                       bool careful) {
+  // The same by the largest score so far, whose distances are taken before they are multiplied by c. The probabilities are
+  // 2^-order() at most, so that no sum of them and values passes the largest value; half's, whose values are below 2^16, are
+  // not scaled. m: that score itself.
+  __device__ __forceinline__ int order(int ct) const {
+    if constexpr (std::is_same<E, E16<F16Io>>::value) return 0;
+    else return 33 - __clz(lim[ct]);  // 2^order > 2 lim
+  }
+  __device__ __forceinline__ void softmax_exact(int ct, f32x16 (&sc)[RT], u32x4 (&p)[RT][2], int k0, float c) {
+    const int lh = (threadIdx.x & 63) >> 5;
+    float top = -INFINITY;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sc[rt][r] = k0 + acc_key(rt, r, lh) < lim[ct] ? sc[rt][r] : -INFINITY;
+        top = fmaxf(top, sc[rt][r]);
+      }
+    const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+    if (top > m[ct]) {
+      const float alpha = fast_exp2((m[ct] - top) * c);
+      m[ct] = top;
+      l[ct] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] *= alpha;
+    }
+    const float base = m[ct] == -INFINITY ? 0.f : m[ct], down = static_cast<float>(-order(ct));
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float e0 = fast_exp2(__fmaf_rn(sc[rt][r] - base, c, down));
+        const float e1 = fast_exp2(__fmaf_rn(sc[rt][r + 1] - base, c, down));
+        if constexpr (E::ES == 2) {
+          const uint32_t w = E::Io::pack2(e0, e1);
+          p[rt][r >> 3][(r & 7) >> 1] = w;
+          l[ct] = add_pair<typename E::Io>(w, l[ct]);
+        } else {
+          sc[rt][r] = e0, sc[rt][r + 1] = e1;
+          l[ct] += e0 + e1;
+        }
+      }
+  }
+  // After kExact: its rows' references in binary orders, as the others'. Where c m is rounded by no more than an order the
+  // sums take the rest; a larger m is one of scores that are rounded by as much.
+  __device__ __forceinline__ void to_orders(float c) {
+    constexpr float kMost = 0x1.fffffep127f;
+#pragma unroll
+    for (int ct = 0; ct < NCT; ++ct) {
+      if (lim[ct] == 0 || m[ct] == -INFINITY) continue;
+      const float base = fminf(fmaxf(m[ct] * c, -kMost), kMost), up = static_cast<float>(order(ct)), ref = base + up;
+      const float rest = __fmaf_rn(m[ct], c, -base) + (base - (ref - up));
+      const float f = fabsf(rest) <= 1.f ? fast_exp2(rest) : 1.f;
+      m[ct] = ref;
+      l[ct] *= f;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] *= f;
+    }
+  }
+
+  // One key tile; `masked`: some row does not see all of its keys from k0 on.
+  template <int PASS>
+  __device__ __forceinline__ void step(const uint8_t* sK, const uint8_t* sV, int k0, float c, bool masked, bool first) {
     f32x16 sc[NCT][RT];
     u32x4 p[NCT][RT][2];
     scores(sK, sc);
 #pragma unroll
-    for (int ct = 0; ct < NCT; ++ct) softmax(ct, sc[ct], p[ct], k0, c, masked, first, careful);
-    if (__builtin_expect(masked && careful, 0)) return add_apart(sV, k0, sc, p);
+    for (int ct = 0; ct < NCT; ++ct) {
+      if constexpr (PASS == kExact) softmax_exact(ct, sc[ct], p[ct], k0, c);
+      else softmax(ct, sc[ct], p[ct], k0, c, masked || PASS != kPlain, first);
+    }
+    if constexpr (PASS != kPlain) return add_apart(sV, k0, sc, p);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
       if constexpr (E::ES == 2) {
@@ -358,7 +431,11 @@ struct Rows {
       auto add = [&](int key, int ct, const f32x16& x) {
         const bool seen = k0 + key < lim[ct];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[ct][dt][i] = seen ? o[ct][dt][i] + x[i] : o[ct][dt][i];
+        for (int i = 0; i < 16; ++i) {
+          if (!seen || x[i] == 0.f) continue;
+          o[ct][dt][i] += x[i];
+          taken[ct] |= uint64_t(1) << (16 * dt + i);
+        }
       };
       if constexpr (E::ES == 2) {
         u32x4 wild[2 * RT];
@@ -423,9 +500,6 @@ struct Rows {
   }
 };
 
-// A NaN or an infinity in the values of a key that a row does not see meets a probability of zero, and their product is NaN;
-// a score 2^127 above the reference gives an infinity. Both are rare: the sums are taken as they come, and a workgroup that
-// finds a NaN or a large one in them repeats its tile with care. The other rows get the same sums as before, bit for bit.
 template <class E, int D, int NCT, int NW, int WAVES>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, WAVES))) void attend_kernel(const Args a) {
   using L = Lds<E, D>;
@@ -461,7 +535,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
     return a.causal ? clamp_to(at + 1 + t.lk - t.lq, 0, t.lk) : t.lk;
   };
   const int all = __builtin_amdgcn_readfirstlane(sees(t.index * R + R - 1));  // of the workgroup's rows
-  const int most = r0 < rows ? __builtin_amdgcn_readfirstlane(sees(r0 + 32 * NCT - 1)) : 0;  // of the wave's: the last
+  int most = r0 < rows ? __builtin_amdgcn_readfirstlane(sees(r0 + 32 * NCT - 1)) : 0;  // of the wave's: the last
   const int least = __builtin_amdgcn_readfirstlane(sees(r0));                               // and the first one
   const int each = ((all + a.splits - 1) / a.splits + E::KT - 1) / E::KT * E::KT;
   const int begin = part * each, end = begin + each < all ? begin + each : all;
@@ -480,23 +554,36 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
     for (int i = 0; i < Rows<E, D, NCT>::kQ; ++i) w.q[ct][i] = ld16(p + 32 * i + 16 * lh);
   }
   const uint32_t lds0 = lds_addr(smem);
-  for (bool careful = false;; careful = true) {
-    w.clear();
-    if (begin < end) {
-      const KeyCopy<E, D, NW> copy(a, t, g);
-      copy(begin, lds0);
-      int stage = 0;
-      for (int k0 = begin; k0 < end; k0 += E::KT, stage ^= 1) {
-        // vmcnt(0): this wave's copies of the tile. As the builtin, which the compiler counts: after assembly it would wait for
-        // the queries' loads inside the loop, and with them for the copies of the next tile (one token 89 -> 65 us).
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-        __syncthreads();  // everybody's, and the other stage is free
-        if (k0 + E::KT < end) copy(k0 + E::KT, lds0 + (stage ^ 1) * L::kStage);
-        const uint8_t* s = smem + stage * L::kStage;
-        if (k0 < most) w.step(s, s + L::kTile, k0, a.c, k0 + E::KT > least, k0 == begin, careful);
-      }
+  auto run = [&](auto pass) {
+    if (begin >= end) return;
+    const KeyCopy<E, D, NW> copy(a, t, g);
+    copy(begin, lds0);
+    int stage = 0;
+    for (int k0 = begin; k0 < end; k0 += E::KT, stage ^= 1) {
+      // vmcnt(0): this wave's copies of the tile. As the builtin, which the compiler counts: after assembly it would wait for
+      // the queries' loads inside the loop, and with them for the copies of the next tile (one token 89 -> 65 us).
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      __syncthreads();  // everybody's, and the other stage is free
+      if (k0 + E::KT < end) copy(k0 + E::KT, lds0 + (stage ^ 1) * L::kStage);
+      const uint8_t* s = smem + stage * L::kStage;
+      if (k0 < most) w.template step<decltype(pass)::value>(s, s + L::kTile, k0, a.c, k0 + E::KT > least, k0 == begin);
     }
-    if (careful || !__syncthreads_or(w.wild())) break;  // (and the stages are free)
+  };
+  // Whether the workgroup has rows to compute again (and once all know it the stages are free).
+  auto again = [&]() {
+    const bool here = w.again();
+    if (!here) most = 0;
+    return __syncthreads_or(here);
+  };
+#pragma unroll
+  for (int ct = 0; ct < NCT; ++ct) w.clear(ct);
+  run(std::integral_constant<int, kPlain>{});
+  if (again()) {
+    run(std::integral_constant<int, kApart>{});
+    if (again()) {
+      run(std::integral_constant<int, kExact>{});
+      if (a.splits > 1) w.to_orders(a.c);
+    }
   }
 
 #pragma unroll

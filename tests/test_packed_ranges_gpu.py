@@ -140,3 +140,27 @@ def test_bits_do_not_depend_on_the_neighbours(name):
             want = pa.packed_attention(q, kk, v, at, causal=causal, scale=0.25)
             got = pa.packed_attention(qq, kk, v, at, causal=causal, scale=0.25)
             assert torch.equal(got[:100], want[:100]) and torch.equal(got[101:], want[101:]), (x, causal)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+def test_large_values(name):
+    """Values of 2^40 to 2^127 under scores that rise by 0 to 70 after the first tile: each result is a mean of values,
+    and finite."""
+    plain.announce("packed large values", name)
+    x = torch.tensor([0.0, 5.0, 30.0, 42.0, 50.0, 55.0, 60.0, 65.0, 69.0, 70.0], device=DEV)
+    n = x.numel()
+    for keys, lq in ((192, 2), (3000, 1)):
+        scores = torch.zeros(n, keys, device=DEV)
+        scores[:, 64:] = x[:, None]
+        k, q = scored(name, scores.reshape(-1)), queries(name, lq * n)
+        starts = [keys * i for i in range(n)]
+        for e in (40, 90, 119, 121, 127):
+            v = values(name, n * keys, 2.0 ** e, 4)
+            v[::4] = -v[::4]
+            got = pa.packed_attention(q, k, v, plain.offsets([lq] * n), plain.offsets([keys] * n), scale=0.25)
+            assert torch.isfinite(got).all(), (keys, e)
+            plain.check(got, q, k, v, [lq] * n, [keys] * n, starts, True, 0.25, name, (keys, e))
+        top = torch.full_like(v, torch.finfo(v.dtype).max * (1 - 2.0 ** -7))
+        got = pa.packed_attention(q, k, top, plain.offsets([lq] * n), plain.offsets([keys] * n), scale=0.25)
+        assert torch.isfinite(got).all()
+        assert ((got.double() - top[:1].double()).abs() <= 2.0 ** -7 * top[:1].double()).all()
