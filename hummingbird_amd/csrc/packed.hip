@@ -225,15 +225,17 @@ struct Rows {
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) o[ct][dt] = f32x16{};
   }
-  // Clears the rows that are to be computed again, and lets the others see no key, so that they stay as they are. Those with a
-  // NaN, a total of 2^100 or more (the whole row's, of both halves of the wave) or a sum of 2^120 or more that it did not take
-  // from V: what is added to the others later (the parts' totals and sums) stays in range. Whether this wave has one.
-  __device__ __forceinline__ bool again() {
+  // Clears the rows that are to be computed again, and lets the others see no key, so that they stay as they are. Whether this
+  // wave has one. They are those with a NaN, a total of 2^100 or more (the whole row's, of both halves of the wave) or a sum of
+  // 2^120 or more that it did not take from V, so that what is added to the others later (the parts' totals and sums) stays in
+  // range; and of the rows that see a key those with a reference of 2^24 or more, whose rounding is whole binary orders of
+  // every probability, or of minus infinity. `begin`: the first key.
+  __device__ __forceinline__ bool again(int begin) {
     const int lane = threadIdx.x & 63;
     bool any = false;
 #pragma unroll
     for (int ct = 0; ct < NCT; ++ct) {
-      bool found = !(l[ct] + __shfl_xor(l[ct], 32, kWave) < 0x1p100f);
+      bool found = !(l[ct] + __shfl_xor(l[ct], 32, kWave) < 0x1p100f) || (begin < lim[ct] && !(fabsf(m[ct]) < 0x1p24f));
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -293,8 +295,6 @@ struct Rows {
         for (int r = 0; r < 16; ++r) top = fmaxf(top, sc[rt][r]);
       const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
       top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * c;
-      // a first tile with nothing but scores of minus infinity has no reference for the later ones: again()
-      if (kWide && top == -INFINITY && k0 < lim[ct]) l[ct] = NAN;
       const bool passed = top > m[ct] + kSlack;
       if (__any(passed)) {
         const float alpha = passed ? fast_exp2(m[ct] - top) : 1.f;
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
     const int r = r0 + 32 * ct + lr, rc = r < rows ? r : rows - 1, at = rc / a.gs;
     token[ct] = t.q0 + at;
     head[ct] = g * a.gs + rc - at * a.gs;
-    w.lim[ct] = sees(r);
+    w.lim[ct] = r0 < rows ? sees(r) : 0;  // (a wave past the last row sees nothing)
     const uint8_t* p = a.q + token[ct] * a.q_ts + head[ct] * a.q_hs;
 #pragma unroll
     for (int i = 0; i < Rows<E, D, NCT>::kQ; ++i) w.q[ct][i] = ld16(p + 32 * i + 16 * lh);
@@ -571,7 +571,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
   };
   // Whether the workgroup has rows to compute again (and once all know it the stages are free).
   auto again = [&]() {
-    const bool here = w.again();
+    const bool here = w.again(begin);
     if (!here) most = 0;
     return __syncthreads_or(here);
   };

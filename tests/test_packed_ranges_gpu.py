@@ -164,3 +164,25 @@ def test_large_values(name):
         got = pa.packed_attention(q, k, top, plain.offsets([lq] * n), plain.offsets([keys] * n), scale=0.25)
         assert torch.isfinite(got).all()
         assert ((got.double() - top[:1].double()).abs() <= 2.0 ** -7 * top[:1].double()).all()
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("keys", [100, 5000])
+def test_scores_past_two_to_the_24(name, keys):
+    """Scores whose rounding in the exponent's units is whole binary orders: all are 251 x 239 x 2^e or, for every second
+    key, half of that, exactly, so that the result is the mean of the values of the others. The tolerance of `check` without
+    the scores' part: a probability's rounding twice, n steps of fp32 and the output's rounding."""
+    plain.announce("packed scores past 2^24", name, keys)
+    v = values(name, keys, 1.0, 5)
+    tol = 2 * (2 * plain.HELD[name] + 2 * keys * 2.0 ** -24 + plain.HALF_STEP[name])
+    for e in (4, 8, 10, 11, 12, 13, 14, 15, 16) + (() if name == "fp16" else (18, 20, 26, 50)):
+        k = torch.zeros(keys, 1, 64, device=DEV)
+        k[0::2, 0, 0], k[1::2, 0, 0] = 251 * 2.0 ** (e // 2), 251 * 2.0 ** (e // 2 - 1)
+        for sign in (1.0, -1.0):
+            q = torch.zeros(1, 1, 64, device=DEV)
+            q[0, 0, 0] = sign * 239 * 2.0 ** (e - e // 2)
+            for scale in (1.0, 0.3, 0.7, 0.11):
+                got = pa.packed_attention(q.to(v.dtype), k.to(v.dtype), v, plain.offsets([1]), plain.offsets([keys]),
+                                          scale=scale)
+                want = v[0 if sign > 0 else 1::2].double().mean(0)
+                assert ((got[0].double() - want).abs() <= tol * want).all(), (e, sign, scale)
