@@ -532,7 +532,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(WAVES, 
   // the keys that row r sees; rows past the last as that one
   auto sees = [&](int r) {
     const int at = (r < rows ? r : rows - 1) / a.gs;
-    return a.causal ? clamp_to(at + 1 + t.lk - t.lq, 0, t.lk) : t.lk;
+    return a.causal ? clamp_to(at + (t.lk - t.lq) + 1, 0, t.lk) : t.lk;
   };
   const int all = __builtin_amdgcn_readfirstlane(sees(t.index * R + R - 1));  // of the workgroup's rows
   int most = r0 < rows ? __builtin_amdgcn_readfirstlane(sees(r0 + 32 * NCT - 1)) : 0;  // of the wave's: the last

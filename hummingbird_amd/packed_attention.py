@@ -44,10 +44,11 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     lq sees the keys b <= a + lk - lq of lk: the queries are the last of the keys' tokens (one new token: lq = 1).
     A query that sees no key, or only keys of a score of minus infinity, gives zeros; keys that a query does not see take no
     part in it, whatever their values.
-    `scale` (default `D ** -0.5`) is positive.
+    `scale` (default `D ** -0.5`) is positive. bf16 and half inputs multiply on their own type's cores, with the probabilities
+    rounded to that type; statistics and sums are fp32, and fp32 inputs are fp32 throughout.
 
     `out`, if given, is written and returned, its tokens of no sequence (before `offsets[0]`, from `offsets[N]` on) left as
-    they are; a new output has zeros there. D 64 or 128; bf16, half or fp32 (fp32 throughout); any strides of tokens and
+    they are; a new output has zeros there. D 64 or 128; bf16, half or fp32; any strides of tokens and
     heads that are multiples of 16 bytes (of k's and v's tokens up to 2^23 values), every tensor 16-byte aligned."""
     if not q.is_cuda:
         _require_gpu(q, "q")
