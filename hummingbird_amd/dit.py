@@ -67,6 +67,8 @@ def _plain_self_attention(qkv: torch.Tensor, attn: dict, static: dict, cfg: DiTC
     of q and k (sa3jax/dit.py:45-98) in torch, the value mask, then `packed_attention` with a sequence per batch
     entry."""
     batch, length, _ = qkv.shape
+    if static["valid"].shape != (batch, length):  # a batch of one would broadcast, and the other entries have no offsets
+        raise ValueError(f"static is of (B, L) = {tuple(static['valid'].shape)}, h of {(batch, length)}")
     rows = qkv.unflatten(-1, (3, cfg.num_heads, cfg.head_dim))
     weight = torch.stack([attn["q_norm"]["weight"], attn["k_norm"]["weight"]])[:, None]
     # q and k in the same launches, about fifteen a block
