@@ -186,3 +186,31 @@ def test_scores_past_two_to_the_24(name, keys):
                                           scale=scale)
                 want = v[0 if sign > 0 else 1::2].double().mean(0)
                 assert ((got[0].double() - want).abs() <= tol * want).all(), (e, sign, scale)
+
+
+@pytest.mark.parametrize("name", list(DTYPES))
+@pytest.mark.parametrize("D", [64, 128])
+def test_any_ranges(name, D):
+    """Scores spread over 1 to 300 and values over 2^40 each way (half: 2^7), a key of minus infinity and a value of NaN in the
+    middle of some sequences: each pass of the kernel for some rows of a tile and not for others, whole and in parts."""
+    plain.announce("packed any ranges", name, D)
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    for lq, lk, H, G in (([70, 5, 130], [70, 90, 130], 4, 2), ([3, 1], [3000, 2500], 8, 2), ([150], [1100], 3, 3)):
+        T, Tk = sum(lq), sum(lk)
+        starts = [sum(lk[:i]) for i in range(len(lk))]
+        for spread in (1.0, 30.0, 100.0, 300.0):
+            q, k, v = plain.make(name, T, Tk, H, G, D, int(spread))
+            row = torch.rand(T, H, 1, generator=gen, device=DEV)  # some rows' scores spread less
+            q = (q.float() * row * spread ** 0.5).to(q.dtype)
+            k = (k.float() * spread ** 0.5).to(q.dtype)
+            size = torch.rand(Tk, G, 1, generator=gen, device=DEV) * 2 - 1
+            v = (v.float() * torch.exp2(size * (7 if name == "fp16" else 40))).to(q.dtype)
+            for bad in (False, True):
+                if bad:
+                    k[starts[-1] + 7, 0] = 0
+                    k[starts[-1] + 7, 0, 3] = float("-inf")
+                    q[..., 3] = q[..., 3].abs() + 0.5
+                    v[starts[0] + 40, G - 1, 5] = float("nan")
+                for causal in (False, True):
+                    got = pa.packed_attention(q, k, v, plain.offsets(lq), plain.offsets(lk), causal=causal)
+                    plain.check(got, q, k, v, lq, lk, starts, causal, D ** -0.5, name, (lq, spread, bad, causal))
