@@ -111,7 +111,8 @@ def self_attention(h: torch.Tensor, block: dict, static: dict, cfg: DiTConfig,
     `projections` picks the GEMMs around the HIP kernel: "torch" (hipBLASLt, then the kernel's own key
     preparation) or "hip" (this package's matrix-core GEMMs with the key preparation in the to_qkv epilogue, so
     `qkv` is never stored; bf16 or fp16, head_dim 64, heads a multiple of 4). Both compute the same cast points; the
-    choice only affects speed."""
+    choice only affects speed. Where "hip" does not take a size, and in the plain model (`use_packed`), "torch" runs
+    under either."""
     attn = block["self_attn"]
     if dtype is not None:
         h = h.to(dtype.compute)
@@ -266,8 +267,10 @@ def quantize_params(params: dict, conditioning: str = "q4", weights: str = "q8")
     distance from the 16-bit one at 2, 12 and 24 blocks as a part of its norm, and a render of 1422 tokens in 8 steps (62.3
     ms with 16 bits):
 
-        "q8"   "q4"   9 %, 19 %, 26 %   42.9 ms        "mx4"  "q4"   18 %, 42 %, 56 %  38.8 ms
-               "keep" 4 %,  9 %, 12 %   43.4 ms               "keep" 16 %, 39 %, 52 %  39.2 ms
+        "q8"   "q4"   8-9 %, 19-21 %, 26-27 %   42.9 ms        "mx4"  "q4"   18 %, 42 %, 56 %  38.8 ms
+               "keep"   4 %,      9 %,    12 %   43.4 ms               "keep" 16 %, 39 %, 52 %  39.2 ms
+
+    (ranges: two sets of weights).
 
     The other tensors are shared, not copied. The 16-bit weights stay beside the others (2.4 GB of the medium model, 1.2 the
     8-bit and 0.6 the 4-bit ones), so that the other `projections` still run; where only one does, the `"weight"` entries of

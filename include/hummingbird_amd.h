@@ -411,7 +411,7 @@ int hb_proj_mx4(hipStream_t stream, const void* x, int64_t x_row_stride, const v
  *   dtype HB_BF16, HB_F16 (matrix products on operands of that type, probabilities rounded to it) or HB_F32 (fp32
  *   throughout); statistics and sums fp32. D 64 or 128; scale > 0; H up to 65535; N up to 2^20, T (H / G) and Tk up to
  *   2^30, and (ceil(T (H / G) / 128) + N) G below 2^24, the tiles that the lengths could need. Every workgroup looks for its
- *   sequence in the offsets, 64 at a time.
+ *   sequence in the offsets, 64 at a time: past some thousand sequences that is most of the time.
  *   workspace : >= hb_packed_workspace_size(...) bytes, 16-byte aligned; 0 (and NULL allowed) where the rows fill the card
  *               by themselves, else the keys are split and the parts joined from it. One call's at a time. */
 size_t hb_packed_workspace_size(int dtype, int64_t T, int64_t Tk, int N, int H, int G, int D);
